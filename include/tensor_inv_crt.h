@@ -1,7 +1,7 @@
 /*
  * tensor_inv_crt.h -- C ABI of libtensor_inv_crt.so, the B200 (sm_100a) implementation
  * of tensor_inv's CRT-emulated float64 matmul ("Ozaki scheme II" with the first N odd
- * primes as moduli).
+ * primes as moduli), and of the low-rank products that apply its factors.
  *
  * Conventions
  *   - Every pointer marked "device" is CUDA device memory on the current device.
@@ -296,6 +296,88 @@ int ti_lu_panel(double *W, int64_t ldw, int64_t n, int64_t j, int64_t jb, int64_
 int ti_lu_panel_ex(double *W, int64_t ldw, int64_t n, int64_t ncols, int64_t j, int64_t jb,
                    int64_t pc, int64_t *piv, void *workspace, size_t workspace_bytes,
                    void *stream);
+
+/* Element types of the operators below. */
+#define TI_TYPE_F16 0
+#define TI_TYPE_BF16 1
+#define TI_TYPE_F32 2
+#define TI_TYPE_F64 3
+
+/* Dropout of the operators below.  Element (row, col) of a matrix takes 16 bits of the block
+   Philox4x32-10(key = seed, counter = (col / 8, row, offset low, offset high)) -- half col % 8,
+   counted from the low half of the first word -- and is kept when they are >= cut, so it is
+   dropped with probability cut / 65536; kept values are multiplied by 65536 / (65536 - cut).
+   cut = 0: no dropout; cut = 65536: every element is dropped.  The mask is never stored: each
+   kernel that needs it makes it again from these numbers. */
+typedef struct ti_dropout_spec {
+    int32_t cut;              /* 0..65536 */
+    uint64_t seed;            /* the key, unless seed_ptr is given */
+    const uint64_t *seed_ptr; /* device: the key is read here when the kernels run (NULL: seed) */
+    uint64_t offset;
+} ti_dropout_spec_t;
+
+/*
+ * Y = dropout(X): Y[i][j] = kept(i, j) ? X[i][j] * 65536 / (65536 - cut) : 0, for rows x cols
+ * elements of type `dtype` (TI_TYPE_*); element (i, j) of X at X[i*sx0 + j*sx1], Y row-major
+ * with leading dimension ldy.  Applied to a gradient it is its own backward pass.  A dropped
+ * element is 0 whatever it held (NaN and infinities too).  rows < 2^32.
+ */
+int ti_dropout(int dtype, const void *X, int64_t sx0, int64_t sx1, void *Y, int64_t ldy,
+               int64_t rows, int64_t cols, const ti_dropout_spec_t *drop, void *stream);
+
+/*
+ * Operands of the low-rank products.  With i = index[t] (none: the row has no low-rank term),
+ * M the dropout mask of X and f_i = alpha * scale[i] * 65536 / (65536 - cut):
+ *   P[t] = f_i * (M X)[t] A[i]          (r values; zero for a row without a term)
+ *   Y[t] = X[t] W + P[t] B[i]
+ * X: t x k, W: k x n, A: s x k x r, B: s x r x n, all of type dtype (TI_TYPE_F16 or
+ * TI_TYPE_BF16) with any element strides.  Sums are held in float32.
+ */
+typedef struct ti_low_rank {
+    int dtype;
+    int64_t t, k, n, s, r;            /* r <= 256 */
+    const void *x;
+    int64_t sx0, sx1;
+    const void *w;
+    int64_t sw0, sw1;
+    const void *a;
+    int64_t sa0, sa1, sa2;
+    const void *b;
+    int64_t sb0, sb1, sb2;
+    const void *index;                /* device int32[t] or int64[t]; a value outside [0, s) means
+                                         no term; NULL: every row takes adapter 0 */
+    int index_bytes;                  /* 4 or 8 */
+    const float *scale;               /* device float32[s], or NULL for 1 */
+    float alpha;
+    ti_dropout_spec_t drop;
+} ti_low_rank_t;
+
+/* Workspace bytes of ti_low_rank_matmul (backward = 0) and ti_low_rank_backward (1). */
+int ti_low_rank_workspace_size(const ti_low_rank_t *op, int backward, size_t *bytes);
+
+/*
+ * Y (t x n, row-major, leading dimension ldy) and, unless P is NULL, the projection P (float32
+ * t x r, row-major), which the backward pass reads.
+ * workspace: ti_low_rank_workspace_size(op, 0) bytes, 256-byte aligned.
+ */
+int ti_low_rank_matmul(const ti_low_rank_t *op, void *Y, int64_t ldy, float *P, void *workspace,
+                       size_t workspace_bytes, void *stream);
+
+/*
+ * Gradients of ti_low_rank_matmul for dY (t x n, element strides sdy0, sdy1); W is fixed:
+ *   dP[t] = f_i * dY[t] B[i]^T
+ *   dX[t] = dY[t] W^T + M (dP[t] A[i]^T)            (t x k, leading dimension lddx)
+ *   dA[i] = sum over the rows t of adapter i of (M X)[t]^T dP[t]     (s x k x r)
+ *   dB[i] = sum over them of P[t]^T dY[t]                            (s x r x n)
+ * dA and dB are written through the given element strides; an adapter that no row takes gets
+ * zeros.  Each of dX, dA, dB may be NULL (not computed).  P: the forward pass's projection
+ * (may be NULL when dB is).  The sums over rows have a fixed order: results do not change from run
+ * to run.  workspace: ti_low_rank_workspace_size(op, 1) bytes, 256-byte aligned.
+ */
+int ti_low_rank_backward(const ti_low_rank_t *op, const void *dY, int64_t sdy0, int64_t sdy1,
+                         const float *P, void *dX, int64_t lddx, void *dA, int64_t sda0,
+                         int64_t sda1, int64_t sda2, void *dB, int64_t sdb0, int64_t sdb1,
+                         int64_t sdb2, void *workspace, size_t workspace_bytes, void *stream);
 
 #ifdef __cplusplus
 }

@@ -28,6 +28,11 @@ TI_OUT_ADD = 2
 TI_MODULI_PRIMES = 0
 TI_MODULI_WIDE = 1
 
+TI_TYPE_F16 = 0
+TI_TYPE_BF16 = 1
+TI_TYPE_F32 = 2
+TI_TYPE_F64 = 3
+
 TI_NONFINITE_EXP = -(2**31)
 TI_MAX_K = 135263
 TI_MAX_K_WIDE = 133144
@@ -44,7 +49,28 @@ class CrtOptions(ctypes.Structure):
                 ("lower", ctypes.c_int)]
 
 
+class DropoutSpec(ctypes.Structure):
+    """ti_dropout_spec_t."""
+
+    _fields_ = [("cut", ctypes.c_int32), ("seed", ctypes.c_uint64),
+                ("seed_ptr", ctypes.c_void_p), ("offset", ctypes.c_uint64)]
+
+
+class LowRank(ctypes.Structure):
+    """ti_low_rank_t."""
+
+    _fields_ = [("dtype", ctypes.c_int),
+                *[(f, ctypes.c_int64) for f in ("t", "k", "n", "s", "r")],
+                ("x", ctypes.c_void_p), ("sx0", ctypes.c_int64), ("sx1", ctypes.c_int64),
+                ("w", ctypes.c_void_p), ("sw0", ctypes.c_int64), ("sw1", ctypes.c_int64),
+                ("a", ctypes.c_void_p), *[(f, ctypes.c_int64) for f in ("sa0", "sa1", "sa2")],
+                ("b", ctypes.c_void_p), *[(f, ctypes.c_int64) for f in ("sb0", "sb1", "sb2")],
+                ("index", ctypes.c_void_p), ("index_bytes", ctypes.c_int),
+                ("scale", ctypes.c_void_p), ("alpha", ctypes.c_float), ("drop", DropoutSpec)]
+
+
 _opt = ctypes.POINTER(CrtOptions)
+_drop, _lr = ctypes.POINTER(DropoutSpec), ctypes.POINTER(LowRank)
 SIGNATURES = {
     "ti_status_string": (ctypes.c_char_p, [_int]),
     "ti_version": (ctypes.c_char_p, []),
@@ -78,6 +104,11 @@ SIGNATURES = {
     "ti_lu_panel_workspace_size": (_int, [ctypes.POINTER(_sz)]),
     "ti_lu_panel": (_int, [_p, _i64, _i64, _i64, _i64, _p, _p, _sz, _p]),
     "ti_lu_panel_ex": (_int, [_p, _i64, _i64, _i64, _i64, _i64, _i64, _p, _p, _sz, _p]),
+    "ti_dropout": (_int, [_int, _p, _i64, _i64, _p, _i64, _i64, _i64, _drop, _p]),
+    "ti_low_rank_workspace_size": (_int, [_lr, _int, ctypes.POINTER(_sz)]),
+    "ti_low_rank_matmul": (_int, [_lr, _p, _i64, _p, _p, _sz, _p]),
+    "ti_low_rank_backward": (_int, [_lr, _p, _i64, _i64, _p, _p, _i64, _p, _i64, _i64, _i64, _p,
+                                    _i64, _i64, _i64, _p, _sz, _p]),
 }
 
 _lib = None
@@ -230,3 +261,11 @@ def lu_panel_cols(W, j: int, jb: int, pc: int, piv, workspace, stream) -> None:
     check("ti_lu_panel_ex", lib().ti_lu_panel_ex(W.data_ptr(), W.stride(0), n, ncols, j, jb, pc,
                                                  piv.data_ptr(), workspace.data_ptr(),
                                                  workspace.numel(), stream.cuda_stream))
+
+
+def low_rank_workspace_size(op: LowRank, backward: bool) -> int:
+    out = ctypes.c_size_t(0)
+    check("ti_low_rank_workspace_size",
+          lib().ti_low_rank_workspace_size(ctypes.byref(op), 1 if backward else 0,
+                                           ctypes.byref(out)))
+    return out.value
