@@ -352,13 +352,17 @@ typedef struct ti_low_rank {
     ti_dropout_spec_t drop;
 } ti_low_rank_t;
 
-/* Workspace bytes of ti_low_rank_matmul (backward = 0) and ti_low_rank_backward (1). */
-int ti_low_rank_workspace_size(const ti_low_rank_t *op, int backward, size_t *bytes);
+/* Workspace bytes of ti_low_rank_matmul and of ti_low_rank_backward.  They hold the projection and
+   copies of the operands that the copy engines cannot read: those whose rows (or, for W, rows or
+   columns) are not contiguous, or not 16-byte aligned at 16-byte steps. */
+int ti_low_rank_workspace_size(const ti_low_rank_t *op, size_t *bytes);
+int ti_low_rank_backward_workspace_size(const ti_low_rank_t *op, const void *dY, int64_t sdy0,
+                                        int64_t sdy1, size_t *bytes);
 
 /*
  * Y (t x n, row-major, leading dimension ldy) and, unless P is NULL, the projection P (float32
  * t x r, row-major), which the backward pass reads.
- * workspace: ti_low_rank_workspace_size(op, 0) bytes, 256-byte aligned.
+ * workspace: ti_low_rank_workspace_size() bytes, 256-byte aligned.
  */
 int ti_low_rank_matmul(const ti_low_rank_t *op, void *Y, int64_t ldy, float *P, void *workspace,
                        size_t workspace_bytes, void *stream);
@@ -372,7 +376,7 @@ int ti_low_rank_matmul(const ti_low_rank_t *op, void *Y, int64_t ldy, float *P, 
  * dA and dB are written through the given element strides; an adapter that no row takes gets
  * zeros.  Each of dX, dA, dB may be NULL (not computed).  P: the forward pass's projection
  * (may be NULL when dB is).  The sums over rows have a fixed order: results do not change from run
- * to run.  workspace: ti_low_rank_workspace_size(op, 1) bytes, 256-byte aligned.
+ * to run.  workspace: ti_low_rank_backward_workspace_size() bytes, 256-byte aligned.
  */
 int ti_low_rank_backward(const ti_low_rank_t *op, const void *dY, int64_t sdy0, int64_t sdy1,
                          const float *P, void *dX, int64_t lddx, void *dA, int64_t sda0,

@@ -105,7 +105,8 @@ SIGNATURES = {
     "ti_lu_panel": (_int, [_p, _i64, _i64, _i64, _i64, _p, _p, _sz, _p]),
     "ti_lu_panel_ex": (_int, [_p, _i64, _i64, _i64, _i64, _i64, _i64, _p, _p, _sz, _p]),
     "ti_dropout": (_int, [_int, _p, _i64, _i64, _p, _i64, _i64, _i64, _drop, _p]),
-    "ti_low_rank_workspace_size": (_int, [_lr, _int, ctypes.POINTER(_sz)]),
+    "ti_low_rank_workspace_size": (_int, [_lr, ctypes.POINTER(_sz)]),
+    "ti_low_rank_backward_workspace_size": (_int, [_lr, _p, _i64, _i64, ctypes.POINTER(_sz)]),
     "ti_low_rank_matmul": (_int, [_lr, _p, _i64, _p, _p, _sz, _p]),
     "ti_low_rank_backward": (_int, [_lr, _p, _i64, _i64, _p, _p, _i64, _p, _i64, _i64, _i64, _p,
                                     _i64, _i64, _i64, _p, _sz, _p]),
@@ -263,9 +264,14 @@ def lu_panel_cols(W, j: int, jb: int, pc: int, piv, workspace, stream) -> None:
                                                  workspace.numel(), stream.cuda_stream))
 
 
-def low_rank_workspace_size(op: LowRank, backward: bool) -> int:
+def low_rank_workspace_size(op: LowRank, dY=None) -> int:
+    """Bytes for ti_low_rank_matmul, or for ti_low_rank_backward with the 2-D tensor dY."""
     out = ctypes.c_size_t(0)
-    check("ti_low_rank_workspace_size",
-          lib().ti_low_rank_workspace_size(ctypes.byref(op), 1 if backward else 0,
-                                           ctypes.byref(out)))
+    if dY is None:
+        check("ti_low_rank_workspace_size",
+              lib().ti_low_rank_workspace_size(ctypes.byref(op), ctypes.byref(out)))
+    else:
+        check("ti_low_rank_backward_workspace_size",
+              lib().ti_low_rank_backward_workspace_size(ctypes.byref(op), dY.data_ptr(),
+                                                        *dY.stride(), ctypes.byref(out)))
     return out.value

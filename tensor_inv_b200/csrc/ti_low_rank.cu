@@ -8,7 +8,7 @@
 // shared product plus a row of P times a factor) and wgrad (sums over an adapter's rows).
 #include "tensor_inv_crt.h"
 #include "ti_common.cuh"
-#include "ti_low_rank.cuh"
+#include "ti_lr_launch.cuh"
 
 namespace ti {
 
@@ -45,31 +45,27 @@ __global__ void project_kernel(Matrix16 M, int64_t rows, int64_t cols, Factor16 
     if (lane == 0) P[w] = acc;
 }
 
-// out[t][c] = sum_k M[t][k] W[k][c] + m(t, c) sum_j P[t][j] F[i][c][j], one thread per (t, c).
-template <typename T>
-__global__ void expand_kernel(Matrix16 M, int64_t rows, int64_t inner, Matrix16 W, int64_t cols,
-                              const float *P, Factor16 F, int64_t r, RowIndex index,
-                              Dropout drop, T *out, int64_t ldo) {
-    const int64_t e = blockIdx.x * int64_t(blockDim.x) + threadIdx.x;
-    if (e >= rows * cols) return;
-    const int64_t t = e / cols, c = e % cols;
-    const T *x = static_cast<const T *>(M.p) + t * M.s0;
-    const T *w = static_cast<const T *>(W.p) + c * W.s1;
-    float acc = 0.0f;
-    for (int64_t k = 0; k < inner; ++k) acc += to_float(x[k * M.s1]) * to_float(w[k * W.s0]);
-    const int i = index.at(t);
-    bool kept = i >= 0;
-    if (kept && drop.cut)
-        kept = dropout_kept(dropout_bits(drop, dropout_key(drop), static_cast<uint32_t>(t),
-                                         static_cast<uint32_t>(c >> 3)),
-                            static_cast<int>(c & 7), drop.cut);
-    if (kept) {
-        const T *f = static_cast<const T *>(F.p) + i * F.ss + c * F.sc;
-        float low = 0.0f;
-        for (int64_t j = 0; j < r; ++j) low += P[t * r + j] * to_float(f[j * F.sr]);
-        acc += low;
+// dst[i][j] = src[i][j], rows of `ld` elements: operands that a copy engine cannot read (odd strides or
+// addresses) are copied once.  32 x 32 tiles through shared memory, so that both sides are
+// coalesced whichever stride of src is 1.
+__global__ void pack_kernel(Matrix16 src, int64_t rows, int64_t cols, uint16_t *dst, int64_t ld) {
+    __shared__ uint16_t tile[32][33];
+    const uint16_t *s = static_cast<const uint16_t *>(src.p);
+    const int64_t tiles_c = (cols + 31) / 32, total = (rows + 31) / 32 * tiles_c;
+    const bool turned = src.s0 == 1 && src.s1 != 1;
+    for (int64_t u = blockIdx.x; u < total; u += gridDim.x) {
+        const int64_t r0 = u / tiles_c * 32, c0 = u % tiles_c * 32;
+        for (int y = threadIdx.y; y < 32; y += 8) {
+            const int64_t i = r0 + (turned ? threadIdx.x : y), j = c0 + (turned ? y : threadIdx.x);
+            if (i < rows && j < cols)
+                tile[turned ? threadIdx.x : y][turned ? y : threadIdx.x] = s[i * src.s0 + j * src.s1];
+        }
+        __syncthreads();
+        for (int y = threadIdx.y; y < 32; y += 8)
+            if (r0 + y < rows && c0 + threadIdx.x < cols)
+                dst[(r0 + y) * ld + c0 + threadIdx.x] = tile[y][threadIdx.x];
+        __syncthreads();
     }
-    out[t * ldo + c] = from_float<T>(acc);
 }
 
 // out[s][c][j] = sum over the rows t of adapter s of m(t, c) M[t][c] V[t][j].
@@ -116,44 +112,133 @@ unsigned blocks_for(int64_t n, int per) { return static_cast<unsigned>((n + per 
 
 int status(cudaError_t e) { return e == cudaSuccess ? TI_OK : TI_ERR_CUDA; }
 
-template <typename T>
-int forward(const ti_low_rank_t &op, void *Y, int64_t ldy, float *P, cudaStream_t st) {
-    const Matrix16 X{op.x, op.sx0, op.sx1}, W{op.w, op.sw0, op.sw1};
-    const RowIndex index{op.index, op.index_bytes == 8, op.s};
-    const Dropout drop = device_spec(op.drop);
-    project_kernel<T><<<blocks_for(op.t * op.r, 4), 128, 0, st>>>(
-        X, op.t, op.k, Factor16{op.a, op.sa0, op.sa1, op.sa2}, op.r, index, op.scale,
-        op.alpha * dropout_scale(drop.cut), drop, P);
-    if (op.n)
-        expand_kernel<T><<<blocks_for(op.t * op.n, 256), 256, 0, st>>>(
-            X, op.t, op.k, W, op.n, P, Factor16{op.b, op.sb0, op.sb2, op.sb1}, op.r, index,
-            Dropout{}, static_cast<T *>(Y), ldy);
-    return status(cudaGetLastError());
+int64_t round8(int64_t x) { return (x + 7) / 8 * 8; }
+
+// Hands out parts of the workspace; with no base it only counts bytes.
+struct Arena {
+    uint8_t *base;
+    size_t used;
+    void *take(size_t bytes) {
+        void *p = base ? base + used : nullptr;
+        used += align256(bytes);
+        return p;
+    }
+};
+
+// The matrix as `rows` rows of contiguous elements that a copy engine can read: itself, or a
+// packed copy in the workspace (launched unless the arena only counts).
+Matrix16 readable(const Matrix16 &M, int64_t rows, int64_t cols, Arena &arena, int sms,
+                  cudaStream_t st) {
+    const int64_t ld = round8(cols);
+    if (copyable(M.p, rows, M.s0, M.s1, cols)) return Matrix16{M.p, rows <= 1 ? ld : M.s0, 1};
+    void *dst = arena.take(sizeof(uint16_t) * static_cast<size_t>(rows * ld));
+    if (arena.base && rows && cols) {
+        const int64_t tiles = (rows + 31) / 32 * ((cols + 31) / 32), most = int64_t(sms) * 8;
+        pack_kernel<<<static_cast<unsigned>(tiles < most ? tiles : most), dim3(32, 8), 0, st>>>(
+            M, rows, cols, static_cast<uint16_t *>(dst), ld);
+    }
+    return Matrix16{dst, ld, 1};
+}
+
+// W (inner x cols) with one unit stride, readable in that orientation.
+Matrix16 readable_w(const Matrix16 &W, int64_t inner, int64_t cols, Arena &arena, int sms,
+                    cudaStream_t st) {
+    if (copyable(W.p, cols, W.s1, W.s0, inner))
+        return Matrix16{W.p, 1, cols <= 1 ? round8(inner) : W.s1};
+    if (W.s0 == 1 && W.s1 != 1) {
+        const Matrix16 t = readable(Matrix16{W.p, W.s1, W.s0}, cols, inner, arena, sms, st);
+        return Matrix16{t.p, 1, t.s0};
+    }
+    return readable(W, inner, cols, arena, sms, st);
+}
+
+struct Gradient {
+    const void *dY;
+    int64_t sdy0, sdy1;
+    const float *P;
+    void *dX;
+    int64_t lddx;
+    void *dA;
+    int64_t sda[3];
+    void *dB;
+    int64_t sdb[3];
+};
+
+// out = 0 where the inner dimension is empty (the low-rank term is then zero too)
+cudaError_t clear(void *out, int64_t ldo, int64_t rows, int64_t cols, cudaStream_t st) {
+    return cudaMemset2DAsync(out, 2 * ldo, 0, 2 * cols, rows, st);
 }
 
 template <typename T>
-int backward(const ti_low_rank_t &op, const Matrix16 &dY, const float *P, void *dX, int64_t lddx,
-             void *dA, const int64_t (&sda)[3], void *dB, const int64_t (&sdb)[3], float *dP,
-             cudaStream_t st) {
-    const Matrix16 X{op.x, op.sx0, op.sx1};
+int forward(const ti_low_rank_t &op, void *Y, int64_t ldy, float *P, Arena &arena, int sms,
+            int *err, cudaStream_t st) {
     const RowIndex index{op.index, op.index_bytes == 8, op.s};
     const Dropout drop = device_spec(op.drop);
-    if ((dX || dA) && op.t)
+    float *own = static_cast<float *>(arena.take(sizeof(float) * op.t * op.r));
+    if (!P) P = own;
+    const Matrix16 X = readable(Matrix16{op.x, op.sx0, op.sx1}, op.t, op.k, arena, sms, st);
+    const Matrix16 W = readable_w(Matrix16{op.w, op.sw0, op.sw1}, op.k, op.n, arena, sms, st);
+    if (!arena.base) return TI_OK;
+    project_kernel<T><<<blocks_for(op.t * op.r, 4), 128, 0, st>>>(
+        X, op.t, op.k, Factor16{op.a, op.sa0, op.sa1, op.sa2}, op.r, index, op.scale,
+        op.alpha * dropout_scale(drop.cut), drop, P);
+    cudaError_t e = cudaGetLastError();
+    if (e != cudaSuccess || !op.n) return status(e);
+    if (!op.k) return status(clear(Y, ldy, op.t, op.n, st));
+    return status(lr_expand_pairs(op.dtype == TI_TYPE_F16, X, op.t, op.k, W, op.n, P,
+                                  Factor16{op.b, op.sb0, op.sb2, op.sb1}, op.r, index, Dropout{}, Y,
+                                  ldy, err, st));
+}
+
+template <typename T>
+int backward(const ti_low_rank_t &op, const Gradient &g, Arena &arena, int sms, int *err,
+             cudaStream_t st) {
+    const RowIndex index{op.index, op.index_bytes == 8, op.s};
+    const Dropout drop = device_spec(op.drop);
+    float *dP = static_cast<float *>(arena.take(sizeof(float) * op.t * op.r));
+    const Matrix16 dY = readable(Matrix16{g.dY, g.sdy0, g.sdy1}, op.t, op.n, arena, sms, st);
+    const Matrix16 X = readable(Matrix16{op.x, op.sx0, op.sx1}, op.t, op.k, arena, sms, st);
+    const Matrix16 Wt = readable_w(Matrix16{op.w, op.sw1, op.sw0}, op.n, op.k, arena, sms, st);
+    if (!arena.base) return TI_OK;
+    cudaError_t e = cudaSuccess;
+    if ((g.dX || g.dA) && op.t)
         project_kernel<T><<<blocks_for(op.t * op.r, 4), 128, 0, st>>>(
             dY, op.t, op.n, Factor16{op.b, op.sb0, op.sb2, op.sb1}, op.r, index, op.scale,
             op.alpha * dropout_scale(drop.cut), Dropout{}, dP);
-    if (dX && op.t && op.k)
-        expand_kernel<T><<<blocks_for(op.t * op.k, 256), 256, 0, st>>>(
-            dY, op.t, op.n, Matrix16{op.w, op.sw1, op.sw0}, op.k, dP,
-            Factor16{op.a, op.sa0, op.sa1, op.sa2}, op.r, index, drop, static_cast<T *>(dX), lddx);
-    if (dA && op.k)
+    if (g.dX && op.t && op.k) {
+        if (!op.n)
+            e = clear(g.dX, g.lddx, op.t, op.k, st);
+        else
+            e = lr_expand_pairs(op.dtype == TI_TYPE_F16, dY, op.t, op.n, Wt, op.k, dP,
+                                Factor16{op.a, op.sa0, op.sa1, op.sa2}, op.r, index, drop, g.dX,
+                                g.lddx, err, st);
+        if (e != cudaSuccess) return status(e);
+    }
+    if (g.dA && op.k)
         wgrad_kernel<T><<<blocks_for(op.s * op.k * op.r, 256), 256, 0, st>>>(
-            X, op.t, op.k, dP, op.r, index, drop, static_cast<T *>(dA), sda[0], sda[1], sda[2]);
-    if (dB && op.n)
+            X, op.t, op.k, dP, op.r, index, drop, static_cast<T *>(g.dA), g.sda[0], g.sda[1],
+            g.sda[2]);
+    if (g.dB && op.n)
         wgrad_kernel<T><<<blocks_for(op.s * op.n * op.r, 256), 256, 0, st>>>(
-            dY, op.t, op.n, P, op.r, index, Dropout{}, static_cast<T *>(dB), sdb[0], sdb[2],
-            sdb[1]);
+            dY, op.t, op.n, g.P, op.r, index, Dropout{}, static_cast<T *>(g.dB), g.sdb[0],
+            g.sdb[2], g.sdb[1]);
     return status(cudaGetLastError());
+}
+
+int run_forward(const ti_low_rank_t &op, void *Y, int64_t ldy, float *P, Arena &arena, int sms,
+                int *err, cudaStream_t st) {
+    return op.dtype == TI_TYPE_F16 ? forward<__half>(op, Y, ldy, P, arena, sms, err, st)
+                                   : forward<__nv_bfloat16>(op, Y, ldy, P, arena, sms, err, st);
+}
+
+int run_backward(const ti_low_rank_t &op, const Gradient &g, Arena &arena, int sms, int *err,
+                 cudaStream_t st) {
+    return op.dtype == TI_TYPE_F16 ? backward<__half>(op, g, arena, sms, err, st)
+                                   : backward<__nv_bfloat16>(op, g, arena, sms, err, st);
+}
+
+bool bad_workspace(const void *ws, size_t have, size_t need) {
+    return need && (!ws || have < need || (reinterpret_cast<uintptr_t>(ws) & 255));
 }
 
 }  // namespace
@@ -163,18 +248,33 @@ using namespace ti;
 
 extern "C" {
 
-int ti_low_rank_workspace_size(const ti_low_rank_t *op, int backward, size_t *bytes) {
+int ti_low_rank_workspace_size(const ti_low_rank_t *op, size_t *bytes) {
     const int rc = check_op(op);
     if (rc != TI_OK || !bytes) return rc != TI_OK ? rc : TI_ERR_INVALID_ARGUMENT;
-    (void)backward;
-    *bytes = align256(sizeof(float) * static_cast<size_t>(op->t * op->r));
+    Arena count{nullptr, 0};
+    run_forward(*op, nullptr, 0, nullptr, count, 0, nullptr, nullptr);
+    *bytes = count.used;
+    return TI_OK;
+}
+
+int ti_low_rank_backward_workspace_size(const ti_low_rank_t *op, const void *dY, int64_t sdy0,
+                                        int64_t sdy1, size_t *bytes) {
+    const int rc = check_op(op);
+    if (rc != TI_OK || !bytes) return rc != TI_OK ? rc : TI_ERR_INVALID_ARGUMENT;
+    Arena count{nullptr, 0};
+    Gradient g{};
+    g.dY = dY;
+    g.sdy0 = sdy0;
+    g.sdy1 = sdy1;
+    run_backward(*op, g, count, 0, nullptr, nullptr);
+    *bytes = count.used;
     return TI_OK;
 }
 
 int ti_low_rank_matmul(const ti_low_rank_t *op, void *Y, int64_t ldy, float *P, void *workspace,
                        size_t workspace_bytes, void *stream) {
     size_t need = 0;
-    int rc = ti_low_rank_workspace_size(op, 0, &need);
+    int rc = ti_low_rank_workspace_size(op, &need);
     if (rc != TI_OK) return rc;
     int sms = 0, *err = nullptr;
     if ((rc = device_context(&sms, &err)) != TI_OK) return rc;
@@ -182,12 +282,9 @@ int ti_low_rank_matmul(const ti_low_rank_t *op, void *Y, int64_t ldy, float *P, 
     if ((op->k && (!op->x || !op->a || (op->n && !op->w))) || (op->n && (!op->b || !Y)) ||
         ldy < op->n)
         return TI_ERR_INVALID_ARGUMENT;
-    if (need && (!workspace || workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 255)))
-        return TI_ERR_WORKSPACE;
-    float *proj = P ? P : static_cast<float *>(workspace);
-    cudaStream_t st = static_cast<cudaStream_t>(stream);
-    return op->dtype == TI_TYPE_F16 ? forward<__half>(*op, Y, ldy, proj, st)
-                                    : forward<__nv_bfloat16>(*op, Y, ldy, proj, st);
+    if (bad_workspace(workspace, workspace_bytes, need)) return TI_ERR_WORKSPACE;
+    Arena arena{static_cast<uint8_t *>(workspace), 0};
+    return run_forward(*op, Y, ldy, P, arena, sms, err, static_cast<cudaStream_t>(stream));
 }
 
 int ti_low_rank_backward(const ti_low_rank_t *op, const void *dY, int64_t sdy0, int64_t sdy1,
@@ -195,7 +292,7 @@ int ti_low_rank_backward(const ti_low_rank_t *op, const void *dY, int64_t sdy0, 
                          int64_t sda1, int64_t sda2, void *dB, int64_t sdb0, int64_t sdb1,
                          int64_t sdb2, void *workspace, size_t workspace_bytes, void *stream) {
     size_t need = 0;
-    int rc = ti_low_rank_workspace_size(op, 1, &need);
+    int rc = ti_low_rank_backward_workspace_size(op, dY, sdy0, sdy1, &need);
     if (rc != TI_OK) return rc;
     int sms = 0, *err = nullptr;
     if ((rc = device_context(&sms, &err)) != TI_OK) return rc;
@@ -204,15 +301,12 @@ int ti_low_rank_backward(const ti_low_rank_t *op, const void *dY, int64_t sdy0, 
                    (dB && !P))))
         return TI_ERR_INVALID_ARGUMENT;
     if (dX && lddx < op->k) return TI_ERR_INVALID_ARGUMENT;
-    if (need && (!workspace || workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 255)))
-        return TI_ERR_WORKSPACE;
-    cudaStream_t st = static_cast<cudaStream_t>(stream);
-    const Matrix16 G{dY, sdy0, sdy1};
-    const int64_t sda[3] = {sda0, sda1, sda2}, sdb[3] = {sdb0, sdb1, sdb2};
-    float *dP = static_cast<float *>(workspace);
-    return op->dtype == TI_TYPE_F16
-               ? backward<__half>(*op, G, P, dX, lddx, dA, sda, dB, sdb, dP, st)
-               : backward<__nv_bfloat16>(*op, G, P, dX, lddx, dA, sda, dB, sdb, dP, st);
+    if (bad_workspace(workspace, workspace_bytes, need)) return TI_ERR_WORKSPACE;
+    const Gradient g{dY, sdy0, sdy1, P, dX, lddx, dA, {sda0, sda1, sda2}, dB, {sdb0, sdb1, sdb2}};
+    // a call without rows may come without a workspace: there is nothing to pack then
+    alignas(256) static uint8_t none[256];
+    Arena arena{workspace ? static_cast<uint8_t *>(workspace) : none, 0};
+    return run_backward(*op, g, arena, sms, err, static_cast<cudaStream_t>(stream));
 }
 
 }  // extern "C"

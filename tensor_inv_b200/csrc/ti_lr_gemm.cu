@@ -1,0 +1,685 @@
+// ti_lr_gemm.cu -- the expand form on CTA pairs: out = M W + P F, one persistent kernel.
+//
+//   out[t][c] = sum_k M[t][k] W[k][c] + m(t, c) sum_j P[t][j] F[i][c][j],   i = index[t]
+//
+// The shared product is a 16-bit GEMM on tcgen05 (kind::f16, float32 accumulators in TMEM) with
+// the shape of ti_gemm2.cu: a cluster of two CTAs owns a 256 x kBN output tile, CTA r loads rows
+// [128r, 128r+128) of M's tile and half of W's columns per 64-deep stage, and CTA 0 issues
+// M = 256 MMAs for both.  W is read in either orientation (K-major or N-major descriptors), so a
+// transposed view costs nothing.
+//
+// The low-rank term joins the same accumulator as extra steps of the inner dimension: for every
+// distinct adapter among the tile's 256 rows and every 16 of its ranks, one step multiplies the
+// rows' P (zero for the rows of other adapters) by the adapter's F.  A step costs as much as one
+// 64-deep step of the product, so r = 16 adds 1/64 at k = 4096.  P is float32: it enters as
+// kind::tf32 in two parts (its upper 11 bits and the rest; 2^-21 relative error) against F, whose
+// 16-bit values are exact in tf32.  That keeps fp16's range out of the projection, and the exact
+// zeros of foreign rows keep adapters apart -- except for 0 * inf: entries of P or F that are not
+// finite enter the MMA as zero and raise a flag, and the epilogue of such a tile adds their
+// products itself.
+// With dropout (dX) the mask applies to the low-rank term alone, so that term has its own
+// accumulator and the epilogue joins the two; tiles are then 128 columns wide, which keeps both
+// accumulators double buffered in the 512 TMEM columns.
+//
+// Roles (both CTAs): warp 0 TMA producer; warp 1 TMEM allocation and, in CTA 0, the MMA issuer;
+// warps 2..5 epilogue; warps 6..9 loaders of the low-rank steps, which have their own stage, so
+// they fill it while the product's steps run.  A low-rank step is taken after every fourth step
+// of the product while any are left: a fixed order, so results repeat bit for bit.
+// All waits are bounded; on timeout the error word is raised and the CTA leaves its loops.
+#include <atomic>
+#include <cstring>
+#include <type_traits>
+
+#include "ti_common.cuh"
+#include "ti_lr_launch.cuh"
+
+namespace ti {
+namespace {
+
+constexpr int kBM = 256, kBK = 64;
+constexpr int kHalf = 128;                       // rows of M per CTA
+constexpr int kABytes = kHalf * kBK * 2;         // 16 KB
+constexpr int kThreads = 320;
+constexpr int kEpiWarps = 4, kLoaders = 128;
+constexpr uint32_t kTmemCols = 512;
+constexpr int kEvery = 4;                        // product steps between two low-rank steps
+constexpr int kGroupM = 8;                       // raster: 8 row tiles (2048 rows) at a time
+constexpr int kRankStep = 16;
+
+template <int kBN>
+struct Shape {
+    static constexpr int kCols = kBN / 2;                   // columns of W per CTA
+    static constexpr int kBBytes = kCols * kBK * 2;
+    static constexpr int kStageBytes = kABytes + kBBytes;
+    static constexpr int kLowBytes = kHalf * 128 + kCols * 128;  // one low-rank step per CTA
+    static constexpr int kStages = kBN == 256 ? 6 : 8;
+    static constexpr size_t kSmem = size_t(kStages) * kStageBytes + kLowBytes + 1024 + 512;
+};
+
+struct Params {
+    int64_t rows, cols;
+    int num_kb, tiles_m, tiles_n;
+    int64_t total;
+    int w_nmajor;
+    uint32_t idesc16, idesc32;
+    const float *P;
+    int64_t r;
+    Factor16 F;
+    RowIndex index;
+    Dropout drop;
+    void *out;
+    int64_t ldo;
+    int vec;        // rows of out are 16-byte aligned
+    int *err;
+};
+
+__device__ __forceinline__ void tma_load_2d_pair(void *dst, const CUtensorMap *map, uint32_t bar,
+                                                 int c0, int c1) {
+    asm volatile(
+        "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes"
+        " [%0], [%1, {%3, %4}], [%2];" ::"r"(smem_u32(dst)),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(c0), "r"(c1)
+        : "memory");
+}
+
+__device__ __forceinline__ void umma_f16_pair(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc,
+                                              uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+
+__device__ __forceinline__ void umma_tf32_pair(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc,
+                                               uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::tf32 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+
+__device__ __forceinline__ bool try_wait_cluster(uint32_t bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(bar), "r"(parity)
+        : "memory");
+    return ok != 0;
+}
+
+// mbar_wait for a barrier that the other CTA's threads arrive on after writing shared memory.
+__device__ __forceinline__ bool mbar_wait_cluster(uint64_t *bar, uint32_t parity,
+                                                  volatile int *abort) {
+    const uint32_t a = smem_u32(bar);
+    if (try_wait_cluster(a, parity)) return true;
+    const unsigned long long t0 = globaltimer_ns();
+    while (!try_wait_cluster(a, parity)) {
+        if (*abort || globaltimer_ns() - t0 > kWaitTimeoutNs) return false;
+    }
+    return true;
+}
+
+__device__ __forceinline__ void loader_sync() {
+    asm volatile("bar.sync 1, %0;" ::"n"(kLoaders) : "memory");
+}
+
+// loader_sync that also tells every loader whether any of them saw `flag`.
+__device__ __forceinline__ bool loader_sync_or(bool flag) {
+    uint32_t any;
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\t"
+        "setp.ne.u32 p, %1, 0;\n\t"
+        "bar.red.or.pred q, 1, %2, p;\n\t"
+        "selp.u32 %0, 1, 0, q;\n\t}"
+        : "=r"(any)
+        : "r"(static_cast<uint32_t>(flag)), "n"(kLoaders)
+        : "memory");
+    return any != 0;
+}
+
+__device__ __forceinline__ void raise(const Params &P, volatile int *abort, int code) {
+    *abort = 1;
+    atomicCAS(P.err, 0, code);
+}
+
+__device__ __forceinline__ void drain_wait(const Params &P, uint64_t *bar, uint32_t parity) {
+    const uint32_t a = smem_u32(bar);
+    const unsigned long long t0 = globaltimer_ns();
+    while (!mbar_try_wait(a, parity)) {
+        if (globaltimer_ns() - t0 > kWaitTimeoutNs) {
+            atomicCAS(P.err, 0, kErrTimeoutDrain);
+            return;
+        }
+    }
+}
+
+// Tiles of the pair (both CTAs walk the same sequence); f(tm, tn) returns false to stop.
+template <class Fn>
+__device__ __forceinline__ void tiles(const Params &P, Fn &&f) {
+    const int64_t per_group = int64_t(kGroupM) * P.tiles_n;
+    for (int64_t u = blockIdx.x >> 1; u < P.total; u += gridDim.x >> 1) {
+        const int g = static_cast<int>(u / per_group);
+        const int first = g * kGroupM, size = min(kGroupM, P.tiles_m - first);
+        const int64_t in = u - g * per_group;
+        if (!f(first + static_cast<int>(in % size), static_cast<int>(in / size))) return;
+    }
+}
+
+__device__ __forceinline__ bool finite(float x) {
+    return (__float_as_uint(x) & 0x7F800000u) != 0x7F800000u;
+}
+
+// 16-byte chunk `c` (0..7) of 128-byte row `row` in a 128-byte-swizzled tile.
+__device__ __forceinline__ float4 *swizzled(uint8_t *tile, int row, int c) {
+    return reinterpret_cast<float4 *>(tile + row * 128 + ((c ^ (row & 7)) << 4));
+}
+
+// Columns [c0, c0 + 32) of one row of a tile whose P or F holds entries that are not finite:
+// adds the products that the MMA left out.
+template <typename T>
+__device__ __noinline__ void add_nonfinite(const Params &P, int64_t row, int64_t c0, float *acc) {
+    const int i = P.index.at(row);
+    if (i < 0) return;
+    const T *f = static_cast<const T *>(P.F.p) + i * P.F.ss;
+    for (int c = 0; c < 32 && c0 + c < P.cols; ++c)
+        for (int64_t j = 0; j < P.r; ++j) {
+            const float p = P.P[row * P.r + j];
+            const float b = to_float(f[(c0 + c) * P.F.sc + j * P.F.sr]);
+            if (!finite(p) || !finite(b)) acc[c] += p * b;
+        }
+}
+
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float a, float b);
+template <>
+__device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float a, float b) {
+    __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<uint32_t *>(&v);
+}
+template <>
+__device__ __forceinline__ uint32_t pack2<__half>(float a, float b) {
+    __half2 v = __floats2half2_rn(a, b);
+    return *reinterpret_cast<uint32_t *>(&v);
+}
+
+template <typename T, int kBN, bool kDrop>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
+    lr_gemm_kernel(const __grid_constant__ CUtensorMap tmM, const __grid_constant__ CUtensorMap tmW,
+                   const __grid_constant__ Params P) {
+    using S = Shape<kBN>;
+    static_assert(!kDrop || kBN == 128, "two accumulators, double buffered, in 512 columns");
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t *smem = reinterpret_cast<uint8_t *>(
+        (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    uint8_t *sA = smem;
+    uint8_t *sB = sA + S::kStages * kABytes;
+    uint8_t *sP = sB + S::kStages * S::kBBytes;   // low-rank step: 128 rows of P, hi | lo
+    uint8_t *sF = sP + kHalf * 128;               //                kCols rows of F
+    uint64_t *full = reinterpret_cast<uint64_t *>(sF + S::kCols * 128);  // CTA 0
+    uint64_t *empty = full + S::kStages;
+    uint64_t *tfull = empty + S::kStages;   // [2] both CTAs: accumulator ready
+    uint64_t *tempty = tfull + 2;           // [2] CTA 0: drained by both epilogues
+    uint64_t *lfull = tempty + 2;           // CTA 0: low-rank step written in both CTAs
+    uint64_t *lempty = lfull + 1;           // both CTAs: low-rank step taken
+    uint64_t *drain = lempty + 1;
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(drain + 1);
+    volatile int *abort = reinterpret_cast<volatile int *>(tmem_slot + 1);
+    volatile int *message = abort + 1;      // CTA 0: 8-wide steps in this low-rank step, 0: no more
+    volatile int *fix = message + 1;        // [4] by tile: entries that are not finite
+    int *least = const_cast<int *>(fix) + 4;  // [2][4] loaders' smallest adapter, by warp
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t rank = cluster_rank();
+    constexpr int kAccCols = kDrop ? 2 * kBN : kBN;  // TMEM columns per buffer
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < S::kStages; ++s) {
+            mbar_init(&full[s], 1);
+            mbar_init(&empty[s], 1);
+        }
+        for (int a = 0; a < 2; ++a) {
+            mbar_init(&tfull[a], 1);
+            mbar_init(&tempty[a], 2 * kEpiWarps);
+        }
+        mbar_init(lfull, 2);
+        mbar_init(lempty, 1);
+        mbar_init(drain, 1);
+        *abort = 0;
+        fence_barrier_init();
+        prefetch_tensormap(&tmM);
+        prefetch_tensormap(&tmW);
+    }
+    if (warp == 1) {
+        tmem_alloc_pair(tmem_slot, kTmemCols);
+        tmem_relinquish_pair();
+    }
+    tc_fence_before();
+    __syncthreads();
+    cluster_sync_all();
+    tc_fence_after();
+    const uint32_t tmem_base = *tmem_slot;
+
+    if (warp == 0) {
+        if (lane == 0) {
+            // ---------------- TMA producer (both CTAs) ----------------
+            int stage = 0;
+            uint32_t phase = 0, issued_mask = 0, issued_phase = 0;
+            bool ok = true;
+            tiles(P, [&](int tm, int tn) {
+                const int row0 = tm * kBM + static_cast<int>(rank) * kHalf;
+                const int col0 = tn * kBN + static_cast<int>(rank) * S::kCols;
+                for (int kb = 0; kb < P.num_kb; ++kb) {
+                    if (!mbar_wait(&empty[stage], phase ^ 1, abort)) {
+                        raise(P, abort, kErrTimeoutProducer);
+                        ok = false;
+                        return false;
+                    }
+                    if (rank == 0) mbar_arrive_expect_tx(&full[stage], 2 * S::kStageBytes);
+                    const uint32_t fb = map_to_rank(smem_u32(&full[stage]), 0);
+                    tma_load_2d_pair(sA + stage * kABytes, &tmM, fb, kb * kBK, row0);
+                    uint8_t *b = sB + stage * S::kBBytes;
+                    if (P.w_nmajor) {
+#pragma unroll
+                        for (int h = 0; h < S::kCols / 64; ++h)
+                            tma_load_2d_pair(b + h * 8192, &tmW, fb, col0 + 64 * h, kb * kBK);
+                    } else {
+                        tma_load_2d_pair(b, &tmW, fb, kb * kBK, col0);
+                    }
+                    issued_mask |= 1u << stage;
+                    issued_phase = (issued_phase & ~(1u << stage)) | (phase << stage);
+                    if (++stage == S::kStages) {
+                        stage = 0;
+                        phase ^= 1;
+                    }
+                }
+                return true;
+            });
+            if (!ok) {
+                // every issued copy lands before the pair may exit; CTA 0 sees both CTAs' bytes
+                if (rank == 0) {
+                    for (int s = 0; s < S::kStages; ++s)
+                        if ((issued_mask >> s) & 1) drain_wait(P, &full[s], (issued_phase >> s) & 1);
+                } else {
+                    const unsigned long long t0 = globaltimer_ns();
+                    while (globaltimer_ns() - t0 < 1000000ull) {
+                    }
+                }
+            }
+        }
+    } else if (warp == 1) {
+        if (lane == 0 && rank == 0) {
+            // ---------------- MMA issuer (CTA 0) ----------------
+            int stage = 0;
+            uint32_t phase = 0, lphase = 0;
+            bool ok = true, any_issued = false;
+            int64_t unit = 0;
+            const uint64_t pdesc = make_sw128_kmajor_desc(smem_u32(sP));
+            const uint64_t fdesc = make_sw128_kmajor_desc(smem_u32(sF));
+            tiles(P, [&](int, int) {
+                const int acc = static_cast<int>(unit & 1);
+                const uint32_t acc_phase = static_cast<uint32_t>((unit >> 1) & 1);
+                ++unit;
+                if (!mbar_wait(&tempty[acc], acc_phase ^ 1, abort)) {
+                    raise(P, abort, kErrTimeoutMma);
+                    ok = false;
+                    return false;
+                }
+                tc_fence_after();
+                const uint32_t d = tmem_base + static_cast<uint32_t>(acc * kAccCols);
+                const uint32_t dlow = kDrop ? d + kBN : d;
+                bool more = true;         // low-rank steps may follow
+                uint32_t have_low = kDrop ? 0u : 1u;  // the low-rank accumulator holds something
+                // takes one low-rank step, or the loaders' word that there are no more
+                auto low_step = [&]() {
+                    if (!mbar_wait_cluster(lfull, lphase, abort)) {
+                        raise(P, abort, kErrTimeoutMma);
+                        ok = false;
+                        return false;
+                    }
+                    lphase ^= 1;
+                    tc_fence_after();
+                    const int n8 = *message;
+                    for (int part = 0; part < 2; ++part)  // upper bits, then the rest
+                        for (int h = 0; h < n8; ++h) {
+                            umma_tf32_pair(dlow, pdesc + 4 * part + 2 * h, fdesc + 2 * h,
+                                           P.idesc32, have_low);
+                            have_low = 1;
+                        }
+                    umma_commit_pair(lempty);
+                    more = n8 != 0;
+                    return true;
+                };
+                for (int kb = 0; kb < P.num_kb; ++kb) {
+                    if (!mbar_wait(&full[stage], phase, abort)) {
+                        raise(P, abort, kErrTimeoutMma);
+                        ok = false;
+                        return false;
+                    }
+                    tc_fence_after();
+                    const uint64_t adesc = make_sw128_kmajor_desc(smem_u32(sA + stage * kABytes));
+                    const uint32_t sb = smem_u32(sB + stage * S::kBBytes);
+                    const uint64_t bdesc = P.w_nmajor ? make_sw128_mnmajor_desc(sb, 8192)
+                                                      : make_sw128_kmajor_desc(sb);
+                    const uint32_t bstep = P.w_nmajor ? 128 : 2;  // 16 inner elements further
+#pragma unroll
+                    for (int kk = 0; kk < kBK / 16; ++kk)
+                        umma_f16_pair(d, adesc + 2 * kk, bdesc + bstep * kk, P.idesc16,
+                                      (kb | kk) != 0 ? 1u : 0u);
+                    any_issued = true;
+                    umma_commit_pair(&empty[stage]);
+                    if (++stage == S::kStages) {
+                        stage = 0;
+                        phase ^= 1;
+                    }
+                    if (more && kb % kEvery == kEvery - 1 && !low_step()) return false;
+                }
+                while (more)
+                    if (!low_step()) return false;
+                umma_commit_pair(&tfull[acc]);
+                return true;
+            });
+            if (!ok && any_issued) {
+                umma_commit_pair(drain);
+                drain_wait(P, drain, 0);
+            }
+        }
+    } else if (warp < 2 + kEpiWarps) {
+        // ---------------- epilogue (warps 2..5, both CTAs) ----------------
+        const int q = warp & 3;  // TMEM lane quadrant this warp may access
+        int64_t unit = 0;
+        const uint64_t key = kDrop ? dropout_key(P.drop) : 0;
+        T *out = static_cast<T *>(P.out);
+        tiles(P, [&](int tm, int tn) {
+            const int acc = static_cast<int>(unit & 1);
+            const uint32_t acc_phase = static_cast<uint32_t>((unit >> 1) & 1);
+            const int slot = static_cast<int>(unit & 3);
+            ++unit;
+            if (!mbar_wait(&tfull[acc], acc_phase, abort)) {
+                raise(P, abort, kErrTimeoutEpilogue);
+                return false;
+            }
+            tc_fence_after();
+            const int64_t row = int64_t(tm) * kBM + int64_t(rank) * kHalf + q * 32 + lane;
+            const bool fixup = fix[slot] != 0;
+            const bool has_low = !kDrop || (row < P.rows && P.index.at(row) >= 0);
+            const uint32_t tbase = tmem_base + (static_cast<uint32_t>(q * 32) << 16) +
+                                   static_cast<uint32_t>(acc * kAccCols);
+#pragma unroll 1
+            for (int c = 0; c < kBN / 32; ++c) {
+                const int64_t col0 = int64_t(tn) * kBN + c * 32;
+                if (col0 >= P.cols) break;  // the same for the whole warp
+                uint32_t v[32];
+                float *y = reinterpret_cast<float *>(v);
+                tmem_ld_32x32b_x32(tbase + c * 32, v);
+                if constexpr (kDrop) {
+                    uint32_t low[32];
+                    tmem_ld_32x32b_x32(tbase + kBN + c * 32, low);
+                    tmem_wait_ld();
+                    if (has_low) {
+                        float *l = reinterpret_cast<float *>(low);
+                        if (fixup) add_nonfinite<T>(P, row, col0, l);
+#pragma unroll
+                        for (int b = 0; b < 4; ++b) {
+                            const uint4 bits =
+                                dropout_bits(P.drop, key, static_cast<uint32_t>(row),
+                                             static_cast<uint32_t>(col0 >> 3) + b);
+#pragma unroll
+                            for (int j = 0; j < 8; ++j)
+                                if (dropout_kept(bits, j, P.drop.cut)) y[8 * b + j] += l[8 * b + j];
+                        }
+                    }
+                } else {
+                    tmem_wait_ld();
+                    if (fixup && row < P.rows) add_nonfinite<T>(P, row, col0, y);
+                }
+                if (row < P.rows) {
+                    T *dst = out + row * P.ldo + col0;
+                    if (P.vec && col0 + 32 <= P.cols) {
+                        uint32_t pk[16];
+#pragma unroll
+                        for (int j = 0; j < 16; ++j) pk[j] = pack2<T>(y[2 * j], y[2 * j + 1]);
+#pragma unroll
+                        for (int j = 0; j < 4; ++j)
+                            reinterpret_cast<uint4 *>(dst)[j] =
+                                make_uint4(pk[4 * j], pk[4 * j + 1], pk[4 * j + 2], pk[4 * j + 3]);
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < 32; ++j)
+                            if (col0 + j < P.cols) dst[j] = from_float<T>(y[j]);
+                    }
+                }
+            }
+            // the whole warp has read its accumulator rows: one arrive per warp on CTA 0
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive_remote(map_to_rank(smem_u32(&tempty[acc]), 0));
+            return true;
+        });
+    } else {
+        // ---------------- loaders of the low-rank steps (warps 6..9, both CTAs) ----------------
+        const int lt = threadIdx.x - 32 * (2 + kEpiWarps);
+        const uint32_t lfull0 = map_to_rank(smem_u32(lfull), 0);
+        int64_t unit = 0;
+        uint32_t phase = 0;
+        int turn = 0;
+        const T *F = static_cast<const T *>(P.F.p);
+        tiles(P, [&](int tm, int tn) {
+            const int slot = static_cast<int>(unit & 3);
+            ++unit;
+            const int64_t row0 = int64_t(tm) * kBM + lt;  // this thread's rows of the pair's tile
+            const int i0 = row0 < P.rows ? P.index.at(row0) : -1;
+            const int i1 = row0 + kHalf < P.rows ? P.index.at(row0 + kHalf) : -1;
+            const int mine = rank ? i1 : i0;
+            const int64_t row = row0 + int64_t(rank) * kHalf;
+            if (lt == 0) fix[slot] = 0;
+            int cur = -1;
+            while (true) {
+                // the next adapter in increasing order: the smallest index above `cur`
+                const unsigned none = 0x7FFFFFFFu;
+                const unsigned c0 = i0 > cur ? static_cast<unsigned>(i0) : none;
+                const unsigned c1 = i1 > cur ? static_cast<unsigned>(i1) : none;
+                const unsigned m = __reduce_min_sync(0xFFFFFFFFu, min(c0, c1));
+                if (lane == 0) least[4 * turn + (lt >> 5)] = static_cast<int>(m);
+                loader_sync();
+                const int *l = least + 4 * turn;
+                turn ^= 1;
+                cur = min(min(l[0], l[1]), min(l[2], l[3]));
+                if (cur == static_cast<int>(none)) break;
+                for (int64_t j0 = 0; j0 < P.r; j0 += kRankStep) {
+                    const int nj = static_cast<int>(min(int64_t(kRankStep), P.r - j0));
+                    float p[kRankStep], f[kRankStep];
+                    bool odd = false;
+                    const float *prow = P.P + row * P.r + j0;
+#pragma unroll
+                    for (int j = 0; j < kRankStep; ++j)
+                        p[j] = mine == cur && j < nj ? prow[j] : 0.0f;
+                    // columns of this CTA's half and, for the check alone, of the other half
+#pragma unroll
+                    for (int h = 0; h < kBN / kLoaders; ++h) {
+                        const int local = h == 0 ? lt : lt + kLoaders;
+                        const int half = local / S::kCols;  // 0: own, 1: the other CTA's
+                        const int64_t col = int64_t(tn) * kBN +
+                                            (half ^ static_cast<int>(rank)) * S::kCols +
+                                            local % S::kCols;
+                        const T *src = F + cur * P.F.ss + col * P.F.sc + j0 * P.F.sr;
+                        float g[kRankStep];
+#pragma unroll
+                        for (int j = 0; j < kRankStep; ++j)
+                            g[j] = col < P.cols && j < nj ? to_float(src[j * P.F.sr]) : 0.0f;
+#pragma unroll
+                        for (int j = 0; j < kRankStep; ++j) {
+                            if (!finite(g[j])) {
+                                odd = true;
+                                g[j] = 0.0f;
+                            }
+                            if (h == 0) f[j] = g[j];
+                        }
+                    }
+                    float lo[kRankStep];
+#pragma unroll
+                    for (int j = 0; j < kRankStep; ++j) {
+                        if (!finite(p[j])) {
+                            odd = true;
+                            p[j] = 0.0f;
+                        }
+                        const float hi = __uint_as_float(__float_as_uint(p[j]) & 0xFFFFE000u);
+                        lo[j] = p[j] - hi;  // exact
+                        p[j] = hi;
+                    }
+                    // a wait that gave up is acted on at the barrier, by all loaders alike
+                    const bool gave_up = !mbar_wait(lempty, phase ^ 1, abort);
+                    if (gave_up) raise(P, abort, kErrTimeoutProducer);
+                    phase ^= 1;
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) {
+                        *swizzled(sP, lt, c) =
+                            make_float4(p[4 * c], p[4 * c + 1], p[4 * c + 2], p[4 * c + 3]);
+                        *swizzled(sP, lt, 4 + c) =
+                            make_float4(lo[4 * c], lo[4 * c + 1], lo[4 * c + 2], lo[4 * c + 3]);
+                        if (lt < S::kCols)
+                            *swizzled(sF, lt, c) =
+                                make_float4(f[4 * c], f[4 * c + 1], f[4 * c + 2], f[4 * c + 3]);
+                    }
+                    if (odd) fix[slot] = 1;
+                    if (lt == 0) *message = (nj + 7) / 8;
+                    fence_proxy_async_smem();
+                    if (loader_sync_or(gave_up)) return false;
+                    if (lt == 0) mbar_arrive_remote(lfull0);
+                }
+            }
+            const bool gave_up = !mbar_wait(lempty, phase ^ 1, abort);
+            if (gave_up) raise(P, abort, kErrTimeoutProducer);
+            phase ^= 1;
+            if (loader_sync_or(gave_up)) return false;
+            if (lt == 0) {
+                *message = 0;
+                mbar_arrive_remote(lfull0);
+            }
+            return true;
+        });
+    }
+
+    // Both CTAs leave their loops before either frees TMEM or exits: CTA 0's MMAs read CTA
+    // 1's shared memory and CTA 1's epilogue and loaders arrive on CTA 0's barriers.
+    tc_fence_before();
+    __syncthreads();
+    cluster_sync_all();
+    if (warp == 1) {
+        __syncwarp();
+        tc_fence_after();
+        tmem_dealloc_pair(tmem_base, kTmemCols);
+    }
+}
+
+// Instruction descriptors: D float32, A K-major, B K-major or N-major (bit 16).
+constexpr uint32_t idesc(int type, int n, bool b_nmajor) {
+    return (1u << 4) | (static_cast<uint32_t>(type) << 7) | (static_cast<uint32_t>(type) << 10) |
+           (b_nmajor ? 1u << 16 : 0u) | (static_cast<uint32_t>(n >> 3) << 17) |
+           (static_cast<uint32_t>(kBM >> 4) << 24);
+}
+
+template <typename T, int kBN, bool kDrop>
+cudaError_t launch(const CUtensorMap &tmM, const CUtensorMap &tmW, const Params &P,
+                   cudaStream_t stream) {
+    using S = Shape<kBN>;
+    // per device: pairs that fit at once (0: not asked yet)
+    constexpr int kMaxDev = 64;
+    static std::atomic<int> capacity[kMaxDev];
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    if (dev < 0 || dev >= kMaxDev) return cudaErrorInvalidDevice;
+    auto kernel = lr_gemm_kernel<T, kBN, kDrop>;
+    int pairs = capacity[dev].load(std::memory_order_acquire);
+    if (pairs == 0) {
+        e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                 static_cast<int>(S::kSmem));
+        if (e != cudaSuccess) return e;
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3(2 * 1024);
+        cfg.blockDim = dim3(kThreads);
+        cfg.dynamicSmemBytes = S::kSmem;
+        cudaLaunchAttribute attr;
+        attr.id = cudaLaunchAttributeClusterDimension;
+        attr.val.clusterDim.x = 2;
+        attr.val.clusterDim.y = 1;
+        attr.val.clusterDim.z = 1;
+        cfg.attrs = &attr;
+        cfg.numAttrs = 1;
+        e = cudaOccupancyMaxActiveClusters(&pairs, kernel, &cfg);
+        if (e != cudaSuccess) return e;
+        if (pairs < 1) return cudaErrorNotSupported;
+        capacity[dev].store(pairs, std::memory_order_release);
+    }
+    const int64_t grid = P.total < pairs ? P.total : pairs;
+    kernel<<<static_cast<unsigned>(2 * grid), kThreads, S::kSmem, stream>>>(tmM, tmW, P);
+    return cudaGetLastError();
+}
+
+template <typename T>
+cudaError_t expand(const Matrix16 &M, int64_t rows, int64_t inner, const Matrix16 &W, int64_t cols,
+                   const float *Pj, const Factor16 &F, int64_t r, const RowIndex &index,
+                   const Dropout &drop, void *out, int64_t ldo, int *err, cudaStream_t stream) {
+    const int bn = drop.cut ? 128 : 256;
+    Params P;
+    std::memset(&P, 0, sizeof(P));
+    P.rows = rows;
+    P.cols = cols;
+    P.num_kb = static_cast<int>((inner + kBK - 1) / kBK);
+    P.tiles_m = static_cast<int>((rows + kBM - 1) / kBM);
+    P.tiles_n = static_cast<int>((cols + bn - 1) / bn);
+    P.total = int64_t(P.tiles_m) * P.tiles_n;
+    P.w_nmajor = W.s0 != 1;
+    const int type = std::is_same<T, __half>::value ? 0 : 1;
+    P.idesc16 = idesc(type, bn, P.w_nmajor);
+    P.idesc32 = idesc(2, bn, false);
+    P.P = Pj;
+    P.r = r;
+    P.F = F;
+    P.index = index;
+    P.drop = drop;
+    P.out = out;
+    P.ldo = ldo;
+    P.vec = ldo % 8 == 0 && (reinterpret_cast<uintptr_t>(out) & 15) == 0;
+    P.err = err;
+    CUtensorMap tmM, tmW;
+    if (!make_map16(&tmM, M.p, inner, rows, M.s0, kBK, kHalf)) return cudaErrorInvalidValue;
+    if (P.w_nmajor ? !make_map16(&tmW, W.p, cols, inner, W.s0, 64, kBK)
+                   : !make_map16(&tmW, W.p, inner, cols, W.s1, kBK, bn / 2))
+        return cudaErrorInvalidValue;
+    return drop.cut ? launch<T, 128, true>(tmM, tmW, P, stream)
+                    : launch<T, 256, false>(tmM, tmW, P, stream);
+}
+
+}  // namespace
+
+bool make_map16(CUtensorMap *map, const void *base, int64_t inner, int64_t outer, int64_t ld,
+                int box_inner, int box_outer) {
+    EncodeTiledFn enc = get_encode_fn();
+    if (!enc) return false;
+    cuuint64_t dims[2] = {static_cast<cuuint64_t>(inner), static_cast<cuuint64_t>(outer)};
+    cuuint64_t strides[1] = {static_cast<cuuint64_t>(ld) * 2};
+    cuuint32_t box[2] = {static_cast<cuuint32_t>(box_inner), static_cast<cuuint32_t>(box_outer)};
+    cuuint32_t estr[2] = {1, 1};
+    return enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT16, 2, const_cast<void *>(base), dims, strides, box,
+               estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+               CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+cudaError_t lr_expand_pairs(bool half, const Matrix16 &M, int64_t rows, int64_t inner,
+                            const Matrix16 &W, int64_t cols, const float *P, const Factor16 &F,
+                            int64_t r, const RowIndex &index, const Dropout &drop, void *out,
+                            int64_t ldo, int *err, cudaStream_t stream) {
+    return half ? expand<__half>(M, rows, inner, W, cols, P, F, r, index, drop, out, ldo, err, stream)
+                : expand<__nv_bfloat16>(M, rows, inner, W, cols, P, F, r, index, drop, out, ldo, err,
+                                        stream);
+}
+
+}  // namespace ti

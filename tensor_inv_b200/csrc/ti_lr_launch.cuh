@@ -1,0 +1,27 @@
+// ti_lr_launch.cuh -- the launchers of the low-rank products' kernels.
+#pragma once
+
+#include <cuda.h>
+
+#include "ti_low_rank.cuh"
+
+namespace ti {
+
+// Tensor map of a matrix of 16-bit elements, `outer` rows of `inner` contiguous ones `ld` apart,
+// 128-byte swizzle; base and rows 16-byte aligned.
+bool make_map16(CUtensorMap *map, const void *base, int64_t inner, int64_t outer, int64_t ld,
+                int box_inner, int box_outer);
+
+// Whether a copy engine can read the matrix as `rows` rows of contiguous elements.
+inline bool copyable(const void *p, int64_t rows, int64_t ld, int64_t s_inner, int64_t inner) {
+    return (inner <= 1 || s_inner == 1) && (reinterpret_cast<uintptr_t>(p) & 15) == 0 &&
+           (rows <= 1 || (ld % 8 == 0 && ld >= inner));
+}
+
+// out = M W + P F (ti_lr_gemm.cu): M with unit s1, W with one unit stride, both copyable.
+cudaError_t lr_expand_pairs(bool half, const Matrix16 &M, int64_t rows, int64_t inner,
+                            const Matrix16 &W, int64_t cols, const float *P, const Factor16 &F,
+                            int64_t r, const RowIndex &index, const Dropout &drop, void *out,
+                            int64_t ldo, int *err, cudaStream_t stream);
+
+}  // namespace ti

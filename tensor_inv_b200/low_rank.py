@@ -87,8 +87,8 @@ def _describe(X, W, A, B, index, scale, alpha, p, seed, offset):
     return op, (X, W, A, B, index, scale, seed)
 
 
-def _workspace(op, backward, device):
-    return torch.empty(max(nat.low_rank_workspace_size(op, backward), 256), dtype=torch.uint8,
+def _workspace(op, device, dY=None):
+    return torch.empty(max(nat.low_rank_workspace_size(op, dY), 256), dtype=torch.uint8,
                        device=device)
 
 
@@ -99,7 +99,7 @@ def _forward(X, W, A, B, index, scale, alpha, p, seed, offset, want_p):
     if op.t == 0:
         return Y, P
     with torch.cuda.device(X.device):
-        ws = _workspace(op, False, X.device)
+        ws = _workspace(op, X.device)
         st = nat.lib().ti_low_rank_matmul(
             ctypes.byref(op), Y.data_ptr(), op.n, None if P is None else P.data_ptr(),
             ws.data_ptr(), ws.numel(), torch.cuda.current_stream(X.device).cuda_stream)
@@ -131,7 +131,7 @@ def _backward(dY, X, W, A, B, index, scale, alpha, p, seed, offset, P, needs):
     dA = torch.empty_like(A) if want_a else None
     dB = torch.empty_like(B) if want_b else None
     with torch.cuda.device(dev):
-        ws = _workspace(op, True, dev)
+        ws = _workspace(op, dev, dY)
         st = nat.lib().ti_low_rank_backward(
             ctypes.byref(op), dY.data_ptr(), *dY.stride(), None if P is None else P.data_ptr(),
             None if dX is None else dX.data_ptr(), op.k,

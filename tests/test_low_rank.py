@@ -404,7 +404,7 @@ def test_what_lies_beside_the_output_is_left(T):
     op, keep = _describe(X, W, A, B, index, scale, 1.0, 0.0, None, 0)
     for ld in (N, N + 5, 80, 96):
         out = torch.full((T + 4, ld), 7.0, dtype=X.dtype, device="cuda")
-        ws = _workspace(op, False, X.device)
+        ws = _workspace(op, X.device)
         st = nat.lib().ti_low_rank_matmul(ctypes.byref(op), out.data_ptr(), ld, None,
                                           ws.data_ptr(), ws.numel(),
                                           torch.cuda.current_stream().cuda_stream)
@@ -524,7 +524,7 @@ def test_c_entry_statuses():
         for name, value in kw.items():
             setattr(op, name, value)
         op.drop.cut = cut
-        return nat.lib().ti_low_rank_workspace_size(ctypes.byref(op), 1, ctypes.byref(size))
+        return nat.lib().ti_low_rank_workspace_size(ctypes.byref(op), ctypes.byref(size))
 
     assert ask() == nat.TI_OK and size.value > 0
     for bad in (dict(dtype=2), dict(dtype=-1), dict(t=-1), dict(k=-1), dict(n=-1), dict(s=0),
@@ -532,7 +532,7 @@ def test_c_entry_statuses():
         assert ask(**bad) == nat.TI_ERR_INVALID_ARGUMENT, bad
     for big in (dict(r=257), dict(t=2**31), dict(k=2**31), dict(n=2**31), dict(s=2**31)):
         assert ask(**big) == nat.TI_ERR_UNSUPPORTED, big
-    assert nat.lib().ti_low_rank_workspace_size(None, 0, ctypes.byref(size)) == \
+    assert nat.lib().ti_low_rank_workspace_size(None, ctypes.byref(size)) == \
         nat.TI_ERR_INVALID_ARGUMENT
     spec = nat.DropoutSpec(cut=70000)
     assert nat.lib().ti_dropout(1, None, 1, 1, None, 1, 1, 1, ctypes.byref(spec), None) == \
