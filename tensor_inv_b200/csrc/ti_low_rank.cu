@@ -16,35 +16,6 @@ int device_context(int *num_sms, int **err);
 
 namespace {
 
-// P[t][j] = f * sum_c m(t, c) M[t][c] F[i][c][j], one warp per (t, j).
-template <typename T>
-__global__ void project_kernel(Matrix16 M, int64_t rows, int64_t cols, Factor16 F, int64_t r,
-                               RowIndex index, const float *scale, float alpha, Dropout drop,
-                               float *P) {
-    const int64_t w = (blockIdx.x * int64_t(blockDim.x) + threadIdx.x) >> 5;
-    const int lane = threadIdx.x & 31;
-    if (w >= rows * r) return;
-    const int64_t t = w / r, j = w % r;
-    const int i = index.at(t);
-    float acc = 0.0f;
-    if (i >= 0) {
-        const T *x = static_cast<const T *>(M.p) + t * M.s0;
-        const T *f = static_cast<const T *>(F.p) + i * F.ss + j * F.sr;
-        const uint64_t key = drop.cut ? dropout_key(drop) : 0;
-        for (int64_t c = lane; c < cols; c += 32) {
-            if (drop.cut) {
-                const uint4 bits = dropout_bits(drop, key, static_cast<uint32_t>(t),
-                                                static_cast<uint32_t>(c >> 3));
-                if (!dropout_kept(bits, static_cast<int>(c & 7), drop.cut)) continue;
-            }
-            acc += to_float(x[c * M.s1]) * to_float(f[c * F.sc]);
-        }
-        for (int o = 16; o; o >>= 1) acc += __shfl_xor_sync(0xFFFFFFFFu, acc, o);
-        acc *= alpha * (scale ? scale[i] : 1.0f);
-    }
-    if (lane == 0) P[w] = acc;
-}
-
 // dst[i][j] = src[i][j], rows of `ld` elements: operands that a copy engine cannot read (odd strides or
 // addresses) are copied once.  32 x 32 tiles through shared memory, so that both sides are
 // coalesced whichever stride of src is 1.
@@ -179,13 +150,13 @@ int forward(const ti_low_rank_t &op, void *Y, int64_t ldy, float *P, Arena &aren
     const Matrix16 X = readable(Matrix16{op.x, op.sx0, op.sx1}, op.t, op.k, arena, sms, st);
     const Matrix16 W = readable_w(Matrix16{op.w, op.sw0, op.sw1}, op.k, op.n, arena, sms, st);
     if (!arena.base) return TI_OK;
-    project_kernel<T><<<blocks_for(op.t * op.r, 4), 128, 0, st>>>(
-        X, op.t, op.k, Factor16{op.a, op.sa0, op.sa1, op.sa2}, op.r, index, op.scale,
-        op.alpha * dropout_scale(drop.cut), drop, P);
-    cudaError_t e = cudaGetLastError();
+    const bool half = op.dtype == TI_TYPE_F16;
+    const cudaError_t e = lr_project(half, X, op.t, op.k,
+                                     Factor16{op.a, op.sa0, op.sa1, op.sa2}, op.r, index, op.scale,
+                                     op.alpha * dropout_scale(drop.cut), drop, P, sms, st);
     if (e != cudaSuccess || !op.n) return status(e);
     if (!op.k) return status(clear(Y, ldy, op.t, op.n, st));
-    return status(lr_expand_pairs(op.dtype == TI_TYPE_F16, X, op.t, op.k, W, op.n, P,
+    return status(lr_expand_pairs(half, X, op.t, op.k, W, op.n, P,
                                   Factor16{op.b, op.sb0, op.sb2, op.sb1}, op.r, index, Dropout{}, Y,
                                   ldy, err, st));
 }
@@ -201,15 +172,17 @@ int backward(const ti_low_rank_t &op, const Gradient &g, Arena &arena, int sms, 
     const Matrix16 Wt = readable_w(Matrix16{op.w, op.sw1, op.sw0}, op.n, op.k, arena, sms, st);
     if (!arena.base) return TI_OK;
     cudaError_t e = cudaSuccess;
-    if ((g.dX || g.dA) && op.t)
-        project_kernel<T><<<blocks_for(op.t * op.r, 4), 128, 0, st>>>(
-            dY, op.t, op.n, Factor16{op.b, op.sb0, op.sb2, op.sb1}, op.r, index, op.scale,
-            op.alpha * dropout_scale(drop.cut), Dropout{}, dP);
+    const bool half = op.dtype == TI_TYPE_F16;
+    if ((g.dX || g.dA) && op.t) {
+        e = lr_project(half, dY, op.t, op.n, Factor16{op.b, op.sb0, op.sb2, op.sb1}, op.r, index,
+                       op.scale, op.alpha * dropout_scale(drop.cut), Dropout{}, dP, sms, st);
+        if (e != cudaSuccess) return status(e);
+    }
     if (g.dX && op.t && op.k) {
         if (!op.n)
             e = clear(g.dX, g.lddx, op.t, op.k, st);
         else
-            e = lr_expand_pairs(op.dtype == TI_TYPE_F16, dY, op.t, op.n, Wt, op.k, dP,
+            e = lr_expand_pairs(half, dY, op.t, op.n, Wt, op.k, dP,
                                 Factor16{op.a, op.sa0, op.sa1, op.sa2}, op.r, index, drop, g.dX,
                                 g.lddx, err, st);
         if (e != cudaSuccess) return status(e);

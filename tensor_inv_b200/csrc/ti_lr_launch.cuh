@@ -18,6 +18,14 @@ inline bool copyable(const void *p, int64_t rows, int64_t ld, int64_t s_inner, i
            (rows <= 1 || (ld % 8 == 0 && ld >= inner));
 }
 
+// Up to this many rows, project runs a cluster per row, above it tiles of 128 rows.
+constexpr int64_t kProjectRowsLimit = 256;
+
+// P = f (m M) F (ti_lr_project.cu): M with unit s1 and copyable.
+cudaError_t lr_project(bool half, const Matrix16 &M, int64_t rows, int64_t cols, const Factor16 &F,
+                       int64_t r, const RowIndex &index, const float *scale, float alpha,
+                       const Dropout &drop, float *P, int num_sms, cudaStream_t stream);
+
 // out = M W + P F (ti_lr_gemm.cu): M with unit s1, W with one unit stride, both copyable.
 cudaError_t lr_expand_pairs(bool half, const Matrix16 &M, int64_t rows, int64_t inner,
                             const Matrix16 &W, int64_t cols, const float *P, const Factor16 &F,

@@ -1,0 +1,467 @@
+// ti_lr_project.cu -- the project form: P[t] = f * (m M)[t] F[i], i = index[t].
+//
+//   P[t][j] = alpha * scale[i] * sum_c m(t, c) M[t][c] F[i][c][j]        (float32, t x r)
+//
+// One pass over M: 2 r operations per element against 2 bytes, so M's bytes bound it for the
+// ranks that adapters have, and the legacy tensor path (mma.sync, operands in registers) is fast
+// enough -- what counts is that M goes from memory to registers once, with the mask applied on the
+// way, and never through shared memory.  Two kernels:
+//   tiles: 128 rows x a slice of the inner dimension per CTA; a cluster of up to 8 CTAs shares the
+//          rows and adds its slices through distributed shared memory.  A tile walks the distinct
+//          adapters of its rows (one, for the runs of rows that prompts and training steps have)
+//          and every row keeps the result of its own.
+//   rows:  one row per cluster, plain multiply-adds: for few rows each with an adapter of its own
+//          F's bytes bound it, and no product is shared between rows.
+#include <type_traits>
+
+#include "ti_common.cuh"
+#include "ti_lr_launch.cuh"
+
+namespace ti {
+namespace {
+
+struct ProjectParams {
+    const void *M;
+    int64_t ld, rows, cols;
+    Factor16 F;
+    int64_t r;
+    RowIndex index;
+    const float *scale;
+    float alpha;
+    Dropout drop;
+    float *P;
+    int64_t slice;  // inner elements per CTA, a multiple of 128 (tiles) or 256 (rows)
+    int mode;       // how F is read: kFC vectors along c, kFR vectors along j, kFScalar
+};
+
+enum { kFScalar = 0, kFC = 1, kFR = 2 };
+
+__device__ __forceinline__ uint32_t keep2(uint32_t x, uint32_t bits, uint32_t cut2) {
+    return x & __vcmpgeu2(bits, cut2);  // halves whose 16 bits are below the cut become 0
+}
+
+// 8 elements of a row with the mask applied; cut = 65536 (everything dropped) has no 16-bit form.
+__device__ __forceinline__ uint4 masked(uint4 v, const Dropout &d, uint64_t key, uint32_t row,
+                                        uint32_t block) {
+    if (d.cut > 65535u) return make_uint4(0, 0, 0, 0);
+    const uint4 b = dropout_bits(d, key, row, block);
+    const uint32_t cut2 = d.cut * 0x10001u;
+    return make_uint4(keep2(v.x, b.x, cut2), keep2(v.y, b.y, cut2), keep2(v.z, b.z, cut2),
+                      keep2(v.w, b.w, cut2));
+}
+
+// 8 consecutive elements at `p`, of which the first n exist (n <= 0: none)
+__device__ __forceinline__ uint4 load8(const uint16_t *p, int64_t n) {
+    if (n >= 8) return __ldg(reinterpret_cast<const uint4 *>(p));
+    uint32_t w[4] = {0, 0, 0, 0};
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+        if (e < n) w[e >> 1] |= static_cast<uint32_t>(p[e]) << (16 * (e & 1));
+    return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+template <typename T>
+__device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2,
+                                         uint32_t a3, uint32_t b0, uint32_t b1);
+template <>
+__device__ __forceinline__ void mma16816<__nv_bfloat16>(float (&d)[4], uint32_t a0, uint32_t a1,
+                                                        uint32_t a2, uint32_t a3, uint32_t b0,
+                                                        uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
+        "{%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+template <>
+__device__ __forceinline__ void mma16816<__half>(float (&d)[4], uint32_t a0, uint32_t a1,
+                                                 uint32_t a2, uint32_t a3, uint32_t b0,
+                                                 uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
+        "{%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// A float in the shared memory of CTA `rank` of the cluster, at this CTA's address `p`.
+__device__ __forceinline__ float load_remote(const float *p, uint32_t rank) {
+    float v;
+    asm volatile("ld.shared::cluster.f32 %0, [%1];"
+                 : "=f"(v)
+                 : "r"(map_to_rank(smem_u32(p), rank))
+                 : "memory");
+    return v;
+}
+
+__device__ __forceinline__ uint32_t cluster_size() {
+    uint32_t n;
+    asm volatile("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(n));
+    return n;
+}
+
+constexpr int kTileRows = 128, kTileThreads = 256, kGroups = 2;  // two groups share the slice
+constexpr int kChunk = 64;             // inner elements per group and step
+constexpr int kFStride = kChunk + 32;  // F's rows in shared memory: 16-byte reads hit all banks
+
+template <int kNT>
+constexpr size_t tile_smem() {
+    return sizeof(uint16_t) * kGroups * 8 * kNT * kFStride + sizeof(float) * kTileRows * 8 * kNT;
+}
+
+// Copies F[cur][c0 .. c0+64)[j0 .. j0+8*kNT) to shared memory as rows of one j (128 threads).
+template <int kNT>
+__device__ __forceinline__ void stage_factor(const ProjectParams &P, int cur, int64_t c0,
+                                             int64_t end, int64_t j0, uint16_t *dst, int gt) {
+    const uint16_t *F = static_cast<const uint16_t *>(P.F.p) + cur * P.F.ss;
+    if (P.mode == kFC) {
+        for (int v = gt; v < 8 * kNT * (kChunk / 8); v += 128) {
+            const int j = v / (kChunk / 8), c = v % (kChunk / 8) * 8;
+            uint4 x = make_uint4(0, 0, 0, 0);
+            if (j0 + j < P.r) x = load8(F + (j0 + j) * P.F.sr + c0 + c, end - (c0 + c));
+            *reinterpret_cast<uint4 *>(dst + j * kFStride + c) = x;
+        }
+    } else if (P.mode == kFR) {
+        for (int v = gt; v < kNT * kChunk; v += 128) {
+            const int c = v / kNT, j = v % kNT * 8;
+            uint4 x = make_uint4(0, 0, 0, 0);
+            if (c0 + c < end) x = load8(F + (c0 + c) * P.F.sc + j0 + j, P.r - (j0 + j));
+            const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                dst[(j + e) * kFStride + c] = static_cast<uint16_t>(w[e >> 1] >> (16 * (e & 1)));
+        }
+    } else {
+        for (int v = gt; v < 8 * kNT * kChunk; v += 128) {
+            const int j = v / kChunk, c = v % kChunk;
+            dst[j * kFStride + c] = j0 + j < P.r && c0 + c < end
+                                        ? F[(c0 + c) * P.F.sc + (j0 + j) * P.F.sr]
+                                        : static_cast<uint16_t>(0);
+        }
+    }
+}
+
+template <typename T, int kNT, bool kDrop>
+__global__ void __launch_bounds__(kTileThreads, 2)
+    project_tiles_kernel(const __grid_constant__ ProjectParams P) {
+    extern __shared__ __align__(16) uint8_t smem[];
+    float *sum = reinterpret_cast<float *>(smem);                          // [128][8*kNT]
+    uint16_t *sF = reinterpret_cast<uint16_t *>(sum + kTileRows * 8 * kNT);  // [2][8*kNT][stride]
+    __shared__ unsigned least[2][8];
+    __shared__ int sidx[kTileRows];
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int g = lane >> 2, tq = lane & 3;
+    const int group = warp >> 2, gt = threadIdx.x & 127;
+    const uint32_t crank = cluster_rank(), csize = cluster_size();
+    const int64_t row0 = int64_t(blockIdx.x / csize) * kTileRows;
+    const int64_t j0 = int64_t(blockIdx.y) * 8 * kNT;
+    const int64_t begin = int64_t(crank) * P.slice;
+    const int64_t end = min(P.cols, begin + P.slice);
+    const uint64_t key = kDrop ? dropout_key(P.drop) : 0;
+
+    if (threadIdx.x < kTileRows) {
+        const int64_t t = row0 + threadIdx.x;
+        sidx[threadIdx.x] = t < P.rows ? P.index.at(t) : -1;
+    }
+    for (int e = threadIdx.x; e < kTileRows * 8 * kNT; e += kTileThreads) sum[e] = 0.0f;
+    __syncthreads();
+
+    const int wrow = (warp & 3) * 32;  // this warp's 32 rows; the thread's are wrow + g + 8*i
+    int idx[4];
+    const uint16_t *M[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        idx[i] = sidx[wrow + g + 8 * i];
+        M[i] = static_cast<const uint16_t *>(P.M) + (row0 + wrow + g + 8 * i) * P.ld;
+    }
+    const int my = sidx[threadIdx.x & 127];
+    int cur = -1, turn = 0;
+    while (true) {
+        // the next adapter in increasing order
+        const unsigned cand = my > cur ? static_cast<unsigned>(my) : 0x7FFFFFFFu;
+        const unsigned m = __reduce_min_sync(0xFFFFFFFFu, cand);
+        if (lane == 0) least[turn][warp] = m;
+        __syncthreads();
+        unsigned next = least[turn][0];
+#pragma unroll
+        for (int w = 1; w < 4; ++w) next = min(next, least[turn][w]);
+        turn ^= 1;
+        if (next == 0x7FFFFFFFu) break;
+        cur = static_cast<int>(next);
+        const bool any = __any_sync(0xFFFFFFFFu, idx[0] == cur || idx[1] == cur || idx[2] == cur ||
+                                                     idx[3] == cur);
+        float acc[2][kNT][4];
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int n = 0; n < kNT; ++n)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) acc[i][n][e] = 0.0f;
+
+        uint16_t *dst = sF + group * 8 * kNT * kFStride;
+        for (int64_t c0 = begin; c0 < end; c0 += kGroups * kChunk) {
+            const int64_t cg = c0 + group * kChunk;  // the same trip count for both groups
+            uint4 x[kChunk / 32][4];
+            if (any) {
+#pragma unroll
+                for (int s = 0; s < kChunk / 32; ++s)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const int64_t c = cg + 32 * s + 8 * tq;
+                        x[s][i] = idx[i] == cur ? load8(M[i] + c, end - c) : make_uint4(0, 0, 0, 0);
+                    }
+            }
+            __syncthreads();  // the previous step's F has been read
+            stage_factor<kNT>(P, cur, cg, end, j0, dst, gt);
+            __syncthreads();
+            if (!any) continue;
+#pragma unroll
+            for (int s = 0; s < kChunk / 32; ++s) {
+                if (kDrop) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        x[s][i] = masked(x[s][i], P.drop, key,
+                                         static_cast<uint32_t>(row0 + wrow + g + 8 * i),
+                                         static_cast<uint32_t>((cg + 32 * s + 8 * tq) >> 3));
+                }
+#pragma unroll
+                for (int n = 0; n < kNT; ++n) {
+                    const uint4 f = *reinterpret_cast<const uint4 *>(
+                        dst + (8 * n + g) * kFStride + 32 * s + 8 * tq);
+                    // the order of the inner dimension is free: a thread's 8 consecutive
+                    // elements fill the slots of two k16 steps, in M and F alike
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        const uint4 &a = x[s][2 * i], &b = x[s][2 * i + 1];
+                        mma16816<T>(acc[i][n], a.x, b.x, a.y, b.y, f.x, f.y);
+                        mma16816<T>(acc[i][n], a.z, b.z, a.w, b.w, f.z, f.w);
+                    }
+                }
+            }
+        }
+        // rows of this adapter keep its sums: first one group's, then the other adds its own
+        for (int turn_g = 0; turn_g < kGroups; ++turn_g) {
+            __syncthreads();
+            if (group == turn_g && any) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (idx[i] == cur) {
+                        float *dst_row = sum + (wrow + g + 8 * i) * 8 * kNT + 2 * tq;
+#pragma unroll
+                        for (int n = 0; n < kNT; ++n) {
+                            dst_row[8 * n] += acc[i >> 1][n][2 * (i & 1)];
+                            dst_row[8 * n + 1] += acc[i >> 1][n][2 * (i & 1) + 1];
+                        }
+                    }
+            }
+        }
+    }
+    // the cluster's slices, added in rank order; each CTA finishes a share of the rows
+    cluster_sync_all();
+    const int share = kTileRows / static_cast<int>(csize);
+    for (int e = threadIdx.x; e < share * 8 * kNT; e += kTileThreads) {
+        const int lr = static_cast<int>(crank) * share + e / (8 * kNT), j = e % (8 * kNT);
+        const int64_t t = row0 + lr;
+        if (t >= P.rows || j0 + j >= P.r) continue;
+        float v = 0.0f;
+        for (uint32_t q = 0; q < csize; ++q) v += load_remote(sum + lr * 8 * kNT + j, q);
+        const int i = sidx[lr];
+        P.P[t * P.r + j0 + j] = i < 0 ? 0.0f : v * (P.alpha * (P.scale ? P.scale[i] : 1.0f));
+    }
+    cluster_sync_all();  // nobody leaves while its sums are being read
+}
+
+// ---------------------------------------------------------------------------------------
+// few rows: a cluster per row
+// ---------------------------------------------------------------------------------------
+constexpr int kRowThreads = 128;
+constexpr int kRowChunk = 256;  // inner elements a warp takes per step: 8 per lane
+constexpr int kMaxRankRows = 256;
+
+template <typename T>
+__device__ __forceinline__ void unpack8(uint4 v, float (&f)[8]) {
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+            f[2 * e] = __uint_as_float(w[e] << 16);
+            f[2 * e + 1] = __uint_as_float(w[e] & 0xFFFF0000u);
+        } else {
+            const float2 h = __half22float2(*reinterpret_cast<const __half2 *>(&w[e]));
+            f[2 * e] = h.x;
+            f[2 * e + 1] = h.y;
+        }
+    }
+}
+
+template <typename T, bool kDrop>
+__global__ void __launch_bounds__(kRowThreads)
+    project_rows_kernel(const __grid_constant__ ProjectParams P) {
+    __shared__ float part[kRowThreads / 32][kMaxRankRows];
+    __shared__ float sum[kMaxRankRows];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t crank = cluster_rank(), csize = cluster_size();
+    const int64_t t = blockIdx.x / csize;
+    const int i = P.index.at(t);
+    const int64_t begin = int64_t(crank) * P.slice, end = min(P.cols, begin + P.slice);
+    const int r = static_cast<int>(P.r);
+    for (int e = threadIdx.x; e < (kRowThreads / 32) * kMaxRankRows; e += kRowThreads)
+        (&part[0][0])[e] = 0.0f;
+    __syncthreads();
+    if (i >= 0) {
+        const uint16_t *M = static_cast<const uint16_t *>(P.M) + t * P.ld;
+        const uint16_t *F = static_cast<const uint16_t *>(P.F.p) + i * P.F.ss;
+        const uint64_t key = kDrop ? dropout_key(P.drop) : 0;
+        // each warp takes every fourth chunk of 256 inner elements, 8 per lane
+        for (int64_t c0 = begin + warp * kRowChunk; c0 < end; c0 += 4 * kRowChunk) {
+            const int64_t c = c0 + 8 * lane;
+            uint4 xv = load8(M + c, end - c);
+            if (kDrop)
+                xv = masked(xv, P.drop, key, static_cast<uint32_t>(t), static_cast<uint32_t>(c >> 3));
+            float x[8];
+            unpack8<T>(xv, x);
+            if (P.mode == kFR) {
+                for (int jb = 0; jb < r; jb += 8) {
+                    uint4 fv[8];
+                    float acc[8];
+#pragma unroll
+                    for (int e = 0; e < 8; ++e)
+                        fv[e] = c + e < end ? load8(F + (c + e) * P.F.sc + jb, r - jb)
+                                            : make_uint4(0, 0, 0, 0);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) acc[e] = 0.0f;
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        float f[8];
+                        unpack8<T>(fv[e], f);
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) acc[j] += x[e] * f[j];
+                    }
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        float v = acc[j];
+#pragma unroll
+                        for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xFFFFFFFFu, v, o);
+                        if (lane == 0 && jb + j < r) part[warp][jb + j] += v;
+                    }
+                }
+            } else {
+#pragma unroll 4
+                for (int j = 0; j < r; ++j) {
+                    float f[8];
+                    if (P.mode == kFC) {
+                        unpack8<T>(load8(F + j * P.F.sr + c, end - c), f);
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 8; ++e)
+                            f[e] = c + e < end ? to_float(*reinterpret_cast<const T *>(
+                                                     F + (c + e) * P.F.sc + j * P.F.sr))
+                                               : 0.0f;
+                    }
+                    float v = 0.0f;
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) v += x[e] * f[e];
+#pragma unroll
+                    for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xFFFFFFFFu, v, o);
+                    if (lane == 0) part[warp][j] += v;
+                }
+            }
+        }
+    }
+    __syncthreads();
+    for (int j = threadIdx.x; j < r; j += kRowThreads)
+        sum[j] = (part[0][j] + part[1][j]) + (part[2][j] + part[3][j]);
+    cluster_sync_all();
+    if (crank == 0)
+        for (int j = threadIdx.x; j < r; j += kRowThreads) {
+            float v = 0.0f;
+            for (uint32_t q = 0; q < csize; ++q) v += load_remote(sum + j, q);
+            P.P[t * P.r + j] = i < 0 ? 0.0f : v * (P.alpha * (P.scale ? P.scale[i] : 1.0f));
+        }
+    cluster_sync_all();
+}
+
+int factor_mode(const Factor16 &F) {
+    const bool base = (reinterpret_cast<uintptr_t>(F.p) & 15) == 0 && F.ss % 8 == 0;
+    if (base && F.sc == 1 && F.sr % 8 == 0) return kFC;
+    if (base && F.sr == 1 && F.sc % 8 == 0) return kFR;
+    return kFScalar;
+}
+
+template <typename K>
+cudaError_t launch_cluster(K kernel, int parts, dim3 grid, int threads, size_t smem,
+                           const ProjectParams &P, cudaStream_t stream) {
+    if (smem > 48 * 1024) {
+        // a repeated setting is cheap and keeps no state per device
+        cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                             static_cast<int>(smem));
+        if (e != cudaSuccess) return e;
+    }
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = parts;
+    attr.val.clusterDim.y = 1;
+    attr.val.clusterDim.z = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kernel, P);
+}
+
+template <typename T, int kNT>
+cudaError_t tiles(const ProjectParams &P, int parts, dim3 grid, cudaStream_t stream) {
+    if constexpr (kNT < 8)
+        if (P.drop.cut)
+            return launch_cluster(project_tiles_kernel<T, kNT, true>, parts, grid, kTileThreads,
+                                  tile_smem<kNT>(), P, stream);
+    return launch_cluster(project_tiles_kernel<T, kNT, false>, parts, grid, kTileThreads,
+                          tile_smem<kNT>(), P, stream);
+}
+
+template <typename T>
+cudaError_t project(ProjectParams P, int num_sms, cudaStream_t stream) {
+    int parts = 1;
+    if (P.rows <= kProjectRowsLimit) {
+        // slices of 1024 (256 for each warp) until 8 CTAs share a row
+        while (parts < 8 && P.cols > 1024 * parts) ++parts;
+        P.slice = ((P.cols + parts - 1) / parts + kRowChunk - 1) / kRowChunk * kRowChunk;
+        const dim3 grid(static_cast<unsigned>(parts * P.rows));
+        return P.drop.cut ? launch_cluster(project_rows_kernel<T, true>, parts, grid, kRowThreads,
+                                           0, P, stream)
+                          : launch_cluster(project_rows_kernel<T, false>, parts, grid, kRowThreads,
+                                           0, P, stream);
+    }
+    const int64_t tile_count = (P.rows + kTileRows - 1) / kTileRows;
+    // (with a mask the widest block would spill registers)
+    const int nt = P.r <= 8 ? 1 : P.r <= 16 ? 2 : P.r <= 32 || P.drop.cut ? 4 : 8;
+    const int64_t blocks = (P.r + 8 * nt - 1) / (8 * nt);
+    // 1, 2, 4 or 8 CTAs share a tile's inner dimension, until two per SM have work
+    constexpr int kStep = kGroups * kChunk;
+    while (parts < 8 && tile_count * blocks * parts < 2 * num_sms && P.cols >= 2 * parts * kStep)
+        parts *= 2;
+    P.slice = ((P.cols + parts - 1) / parts + kStep - 1) / kStep * kStep;
+    const dim3 grid(static_cast<unsigned>(parts * tile_count), static_cast<unsigned>(blocks));
+    switch (nt) {
+        case 1: return tiles<T, 1>(P, parts, grid, stream);
+        case 2: return tiles<T, 2>(P, parts, grid, stream);
+        case 4: return tiles<T, 4>(P, parts, grid, stream);
+        default: return tiles<T, 8>(P, parts, grid, stream);
+    }
+}
+
+}  // namespace
+
+cudaError_t lr_project(bool half, const Matrix16 &M, int64_t rows, int64_t cols, const Factor16 &F,
+                       int64_t r, const RowIndex &index, const float *scale, float alpha,
+                       const Dropout &drop, float *Pout, int num_sms, cudaStream_t stream) {
+    ProjectParams P{M.p,  M.s0, rows, cols, F,    r, index, scale, alpha,
+                    drop, Pout, 0,    factor_mode(F)};
+    return half ? project<__half>(P, num_sms, stream) : project<__nv_bfloat16>(P, num_sms, stream);
+}
+
+}  // namespace ti
