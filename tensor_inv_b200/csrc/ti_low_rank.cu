@@ -39,27 +39,6 @@ __global__ void pack_kernel(Matrix16 src, int64_t rows, int64_t cols, uint16_t *
     }
 }
 
-// out[s][c][j] = sum over the rows t of adapter s of m(t, c) M[t][c] V[t][j].
-template <typename T>
-__global__ void wgrad_kernel(Matrix16 M, int64_t rows, int64_t cols, const float *V, int64_t r,
-                             RowIndex index, Dropout drop, T *out, int64_t ss, int64_t sc,
-                             int64_t sr) {
-    const int64_t e = blockIdx.x * int64_t(blockDim.x) + threadIdx.x;
-    if (e >= index.s * cols * r) return;
-    const int64_t j = e % r, c = e / r % cols, s = e / (r * cols);
-    const uint64_t key = drop.cut ? dropout_key(drop) : 0;
-    float acc = 0.0f;
-    for (int64_t t = 0; t < rows; ++t) {
-        if (index.at(t) != s) continue;
-        if (drop.cut && !dropout_kept(dropout_bits(drop, key, static_cast<uint32_t>(t),
-                                                   static_cast<uint32_t>(c >> 3)),
-                                      static_cast<int>(c & 7), drop.cut))
-            continue;
-        acc += to_float(static_cast<const T *>(M.p)[t * M.s0 + c * M.s1]) * V[t * r + j];
-    }
-    out[s * ss + c * sc + j * sr] = from_float<T>(acc);
-}
-
 constexpr int64_t kMaxRank = 256;
 
 size_t align256(size_t x) { return (x + 255) & ~size_t(255); }
@@ -78,8 +57,6 @@ int check_op(const ti_low_rank_t *op) {
 Dropout device_spec(const ti_dropout_spec_t &d) {
     return Dropout{static_cast<uint32_t>(d.cut), d.seed, d.seed_ptr, d.offset};
 }
-
-unsigned blocks_for(int64_t n, int per) { return static_cast<unsigned>((n + per - 1) / per); }
 
 int status(cudaError_t e) { return e == cudaSuccess ? TI_OK : TI_ERR_CUDA; }
 
@@ -170,6 +147,10 @@ int backward(const ti_low_rank_t &op, const Gradient &g, Arena &arena, int sms, 
     const Matrix16 dY = readable(Matrix16{g.dY, g.sdy0, g.sdy1}, op.t, op.n, arena, sms, st);
     const Matrix16 X = readable(Matrix16{op.x, op.sx0, op.sx1}, op.t, op.k, arena, sms, st);
     const Matrix16 Wt = readable_w(Matrix16{op.w, op.sw1, op.sw0}, op.n, op.k, arena, sms, st);
+    const WgradPlan plan = lr_wgrad_plan(op.t, op.r, op.s, op.k, op.n, index.p != nullptr);
+    void *lists = arena.take(plan.list_bytes);
+    float *part_a = plan.part_a ? static_cast<float *>(arena.take(plan.part_a)) : nullptr;
+    float *part_b = plan.part_b ? static_cast<float *>(arena.take(plan.part_b)) : nullptr;
     if (!arena.base) return TI_OK;
     cudaError_t e = cudaSuccess;
     const bool half = op.dtype == TI_TYPE_F16;
@@ -187,15 +168,11 @@ int backward(const ti_low_rank_t &op, const Gradient &g, Arena &arena, int sms, 
                                 g.lddx, err, st);
         if (e != cudaSuccess) return status(e);
     }
-    if (g.dA && op.k)
-        wgrad_kernel<T><<<blocks_for(op.s * op.k * op.r, 256), 256, 0, st>>>(
-            X, op.t, op.k, dP, op.r, index, drop, static_cast<T *>(g.dA), g.sda[0], g.sda[1],
-            g.sda[2]);
-    if (g.dB && op.n)
-        wgrad_kernel<T><<<blocks_for(op.s * op.n * op.r, 256), 256, 0, st>>>(
-            dY, op.t, op.n, g.P, op.r, index, Dropout{}, static_cast<T *>(g.dB), g.sdb[0],
-            g.sdb[2], g.sdb[1]);
-    return status(cudaGetLastError());
+    return status(lr_wgrad(
+        half,
+        WgradOperand{X, op.k, dP, drop, part_a, g.dA, g.sda[0], g.sda[1], g.sda[2]},
+        WgradOperand{dY, op.n, g.P, Dropout{}, part_b, g.dB, g.sdb[0], g.sdb[2], g.sdb[1]}, op.t,
+        op.r, index, plan, lists, sms, st));
 }
 
 int run_forward(const ti_low_rank_t &op, void *Y, int64_t ldy, float *P, Arena &arena, int sms,

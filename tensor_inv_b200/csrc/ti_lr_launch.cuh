@@ -32,4 +32,26 @@ cudaError_t lr_expand_pairs(bool half, const Matrix16 &M, int64_t rows, int64_t 
                             int64_t r, const RowIndex &index, const Dropout &drop, void *out,
                             int64_t ldo, int *err, cudaStream_t stream);
 
+// The gradients of the adapters (ti_lr_wgrad.cu).
+struct WgradPlan {
+    int64_t chunk, chunks;
+    size_t list_bytes, part_a, part_b;  // workspace
+};
+WgradPlan lr_wgrad_plan(int64_t rows, int64_t r, int64_t s, int64_t cols_a, int64_t cols_b,
+                        bool indexed);
+
+// out[s][c][j] = sum over adapter s's rows of m(t, c) M[t][c] V[t][j]; out null: not computed
+struct WgradOperand {
+    Matrix16 M;  // unit s1, copyable
+    int64_t cols;
+    const float *V;
+    Dropout drop;
+    float *part;
+    void *out;
+    int64_t ss, sc, sr;
+};
+cudaError_t lr_wgrad(bool half, const WgradOperand &a, const WgradOperand &b, int64_t rows,
+                     int64_t r, const RowIndex &index, const WgradPlan &plan, void *lists,
+                     int num_sms, cudaStream_t stream);
+
 }  // namespace ti

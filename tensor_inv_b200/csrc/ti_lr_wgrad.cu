@@ -1,0 +1,380 @@
+// ti_lr_wgrad.cu -- the gradients of the adapters: sums over each adapter's rows.
+//
+//   dA[s][c][j] = sum_{t: index[t] = s} m(t, c) X[t][c] dP[t][j]
+//   dB[s][j][c] = sum_{t: index[t] = s} dY[t][c] P[t][j]
+//
+// Both are out[s] = M^T V with a wide 16-bit M (rows x cols) and a thin float32 V (rows x r); both
+// run in one launch.  M's bytes bound them: each element is read once and meets r values of V.
+// V keeps its 32 bits by entering mma.sync (tf32) in two parts, its upper 11 bits and the rest, while
+// M's 16-bit values are exact in tf32; the legacy tensor path is enough for a product this thin.
+// (An infinity in M meets both parts, so its column comes out infinite or NaN.)
+//
+//   lists  one CTA per adapter writes the positions of its rows, in order, so that an adapter's rows
+//          are consecutive; no atomics, so the sums have one order.
+//   wgrad  a CTA takes a chunk of that order and 512 columns (64 per warp).  A thread reads 16
+//          bytes of a row -- 8 columns that are the same fragment position of 8 MMAs -- so M goes
+//          from memory to registers with the dropout mask applied on the way.  Where a chunk
+//          crosses from one adapter to the next it writes its sums to another slot: chunk + adapter
+//          numbers the (chunk, adapter) pairs that occur without gaps in either direction.
+//   join   adds an adapter's slots in order and rounds once.  One chunk needs no join.
+#include <type_traits>
+
+#include "ti_common.cuh"
+#include "ti_lr_launch.cuh"
+
+namespace ti {
+namespace {
+
+constexpr int kThreads = 256, kWarpCols = 64, kCtaCols = 8 * kWarpCols;
+constexpr int kStage = 64;  // rows of V in shared memory at a time
+
+struct Side {
+    const void *M;
+    int64_t ld, cols;
+    const float *V;
+    Dropout drop;
+    float *part;      // [slot][r][round8(cols)], or null: one chunk, straight to out
+    void *out;
+    int64_t ss, sc, sr;
+    int blocks;       // column blocks of this side; 0: not computed
+};
+
+struct WgradParams {
+    Side side[2];
+    int64_t rows, r, s;
+    const int32_t *order;   // row numbers grouped by adapter, or null: all rows, adapter 0
+    const int32_t *start;   // [s + 1] first position of each adapter, or null
+    int64_t chunk;
+};
+
+__device__ __forceinline__ uint4 load8(const uint16_t *p, int64_t n) {
+    if (n >= 8) return __ldg(reinterpret_cast<const uint4 *>(p));
+    uint32_t w[4] = {0, 0, 0, 0};
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+        if (e < n) w[e >> 1] |= static_cast<uint32_t>(p[e]) << (16 * (e & 1));
+    return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+template <typename T>
+__device__ __forceinline__ float half_of(uint32_t w, int hi) {
+    if constexpr (std::is_same<T, __nv_bfloat16>::value)
+        return __uint_as_float(hi ? w & 0xFFFF0000u : w << 16);
+    else
+        return __half2float(__ushort_as_half(static_cast<unsigned short>(hi ? w >> 16 : w)));
+}
+
+__device__ __forceinline__ void mma_tf32(float (&d)[4], const float (&a)[4], float b0, float b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
+        "{%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(__float_as_uint(a[0])), "r"(__float_as_uint(a[1])), "r"(__float_as_uint(a[2])),
+          "r"(__float_as_uint(a[3])), "r"(__float_as_uint(b0)), "r"(__float_as_uint(b1)));
+}
+
+// order[] and start[]: rows grouped by adapter, ascending within one.  CTA s compacts the rows of
+// adapter s behind those of smaller adapters, which it counts in the same pass.
+__global__ void __launch_bounds__(1024) lists_kernel(RowIndex index, int64_t rows, int32_t *order,
+                                                     int32_t *start) {
+    __shared__ int64_t below_sum;
+    __shared__ int warp_n[32], warp_below[32];
+    const int s = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    // first pass: how many rows belong to smaller adapters
+    int below = 0;
+    for (int64_t t = threadIdx.x; t < rows; t += 1024) {
+        const int i = index.at(t);
+        below += i >= 0 && i < s;
+    }
+    below = __reduce_add_sync(0xFFFFFFFFu, below);
+    if (lane == 0) warp_below[warp] = below;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        int64_t n = 0;
+        for (int w = 0; w < 32; ++w) n += warp_below[w];
+        below_sum = n;
+        start[s] = static_cast<int32_t>(n);
+    }
+    __syncthreads();
+    // second pass: its own rows, 1024 at a time
+    int64_t at = below_sum;
+    for (int64_t t0 = 0; t0 < rows; t0 += 1024) {
+        const int64_t t = t0 + threadIdx.x;
+        const bool own = t < rows && index.at(t) == s;
+        const unsigned ballot = __ballot_sync(0xFFFFFFFFu, own);
+        if (lane == 0) warp_n[warp] = __popc(ballot);
+        __syncthreads();
+        int before = 0, all = 0;
+        for (int w = 0; w < 32; ++w) {
+            before += w < warp ? warp_n[w] : 0;
+            all += warp_n[w];
+        }
+        if (own) order[at + before + __popc(ballot & ((1u << lane) - 1))] = static_cast<int32_t>(t);
+        at += all;
+        __syncthreads();
+    }
+    if (s == gridDim.x - 1 && threadIdx.x == 0) start[s + 1] = static_cast<int32_t>(at);
+}
+
+// Accumulators of one warp: 16*kNJ ranks x 64 columns.  In MMA i, column n of the instruction is
+// column 8n + i of the warp's 64, so a thread's two columns of a row are 16tq + i and 16tq + 8 + i.
+template <typename T, int kNJ>
+__device__ __forceinline__ void store_sums(const WgradParams &P, const Side &S,
+                                           const float (&acc)[kNJ][8][4], int64_t slot, int64_t s,
+                                           int64_t c0, int64_t j0, int g, int tq) {
+    const int64_t ldc = (S.cols + 7) / 8 * 8;
+#pragma unroll
+    for (int nj = 0; nj < kNJ; ++nj)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {  // rank g or g + 8
+            const int64_t j = j0 + 16 * nj + g + 8 * h;
+            if (j >= P.r) continue;
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {  // columns 16tq + 8k ..
+                const int64_t c = c0 + 16 * tq + 8 * k;
+                if (c >= S.cols) continue;
+                if (S.part) {
+                    float4 *dst = reinterpret_cast<float4 *>(S.part + (slot * P.r + j) * ldc + c);
+                    dst[0] = make_float4(acc[nj][0][2 * h + k], acc[nj][1][2 * h + k],
+                                         acc[nj][2][2 * h + k], acc[nj][3][2 * h + k]);
+                    dst[1] = make_float4(acc[nj][4][2 * h + k], acc[nj][5][2 * h + k],
+                                         acc[nj][6][2 * h + k], acc[nj][7][2 * h + k]);
+                } else {
+                    T *dst = static_cast<T *>(S.out) + s * S.ss + j * S.sr;
+#pragma unroll
+                    for (int i = 0; i < 8; ++i)
+                        if (c + i < S.cols)
+                            dst[(c + i) * S.sc] = from_float<T>(acc[nj][i][2 * h + k]);
+                }
+            }
+        }
+}
+
+template <typename T, int kNJ>
+__global__ void __launch_bounds__(kThreads, 2) wgrad_kernel(const __grid_constant__ WgradParams P) {
+    constexpr int kVStride = 16 * kNJ + 8;  // floats: the 4 x 8 fragment reads hit all 32 banks
+    __shared__ float vhi[kStage][kVStride], vlo[kStage][kVStride];
+    __shared__ int32_t srow[kStage];
+    const int which = blockIdx.x < static_cast<unsigned>(P.side[0].blocks) ? 0 : 1;
+    const Side &S = P.side[which];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, tq = lane & 3;
+    const int64_t c0 =
+        int64_t(blockIdx.x - (which ? P.side[0].blocks : 0)) * kCtaCols + warp * kWarpCols;
+    const int64_t j0 = int64_t(blockIdx.z) * 16 * kNJ;
+    const int64_t total = P.start ? P.start[P.s] : P.rows;
+    const bool direct = S.part == nullptr;
+    int64_t pos = int64_t(blockIdx.y) * P.chunk;
+    const int64_t stop = min(total, pos + P.chunk);
+    const uint64_t key = S.drop.cut ? dropout_key(S.drop) : 0;
+    const uint32_t cut2 = S.drop.cut * 0x10001u;
+
+    // the first adapter whose rows reach past pos (from the first one, where every adapter's
+    // gradient is written here)
+    int64_t s = 0;
+    if (P.start && !direct) {
+        int64_t lo = 0, hi = P.s;
+        while (lo < hi) {
+            const int64_t mid = (lo + hi) / 2;
+            if (P.start[mid + 1] > pos) hi = mid;
+            else lo = mid + 1;
+        }
+        s = lo;
+    }
+    const int64_t col = c0 + 8 * g;
+    const uint16_t *M = static_cast<const uint16_t *>(S.M);
+    for (; s < P.s && (direct || pos < stop); ++s) {
+        const int64_t seg_end = P.start ? min(stop, int64_t(P.start[s + 1])) : stop;
+        float acc[kNJ][8][4];
+#pragma unroll
+        for (int nj = 0; nj < kNJ; ++nj)
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) acc[nj][i][e] = 0.0f;
+
+        for (int64_t b = pos; b < seg_end; b += kStage) {
+            const int n = static_cast<int>(min(int64_t(kStage), seg_end - b));
+            __syncthreads();  // the previous stage has been read
+            if (threadIdx.x < kStage)
+                srow[threadIdx.x] = static_cast<int>(threadIdx.x) >= n ? -1
+                                    : P.order ? P.order[b + threadIdx.x]
+                                              : static_cast<int32_t>(b + threadIdx.x);
+            __syncthreads();
+            for (int e = threadIdx.x; e < kStage * 16 * kNJ; e += kThreads) {
+                const int q = e / (16 * kNJ), j = e % (16 * kNJ);
+                const int t = srow[q];
+                const float v = t >= 0 && j0 + j < P.r ? S.V[int64_t(t) * P.r + j0 + j] : 0.0f;
+                // infinities and NaN stay whole in the upper part
+                const uint32_t bits = __float_as_uint(v);
+                const bool odd = (bits & 0x7F800000u) == 0x7F800000u;
+                const float hi = odd ? v : __uint_as_float(bits & 0xFFFFE000u);
+                vhi[q][j] = hi;
+                vlo[q][j] = odd ? 0.0f : v - hi;
+            }
+            __syncthreads();
+            if (c0 >= S.cols) continue;
+            // rows q + 4*h + tq of a step of 16; the next step's rows are read ahead
+            uint4 x[4];
+            auto fetch = [&](int q, uint4(&v)[4]) {
+#pragma unroll
+                for (int h = 0; h < 4; ++h) {
+                    const int t = srow[q + 4 * h + tq];
+                    v[h] = t >= 0 ? load8(M + t * S.ld + col, S.cols - col) : make_uint4(0, 0, 0, 0);
+                }
+            };
+            fetch(0, x);
+#pragma unroll 1
+            for (int q = 0; q < n; q += 16) {
+                uint4 next[4];
+                if (q + 16 < n) fetch(q + 16, next);
+                if (S.drop.cut) {
+#pragma unroll
+                    for (int h = 0; h < 4; ++h) {
+                        const uint4 bits =
+                            dropout_bits(S.drop, key, static_cast<uint32_t>(srow[q + 4 * h + tq]),
+                                         static_cast<uint32_t>(col >> 3));
+                        const bool none = S.drop.cut > 65535u;  // everything is dropped
+                        x[h].x = none ? 0 : x[h].x & __vcmpgeu2(bits.x, cut2);
+                        x[h].y = none ? 0 : x[h].y & __vcmpgeu2(bits.y, cut2);
+                        x[h].z = none ? 0 : x[h].z & __vcmpgeu2(bits.z, cut2);
+                        x[h].w = none ? 0 : x[h].w & __vcmpgeu2(bits.w, cut2);
+                    }
+                }
+#pragma unroll
+                for (int k = 0; k < 2; ++k) {  // two steps of 8 rows
+                    const int q0 = q + 8 * k + tq;
+                    const uint32_t m0[4] = {x[2 * k].x, x[2 * k].y, x[2 * k].z, x[2 * k].w};
+                    const uint32_t m1[4] = {x[2 * k + 1].x, x[2 * k + 1].y, x[2 * k + 1].z,
+                                            x[2 * k + 1].w};
+#pragma unroll
+                    for (int nj = 0; nj < kNJ; ++nj) {
+                        const int j = 16 * nj + g;
+                        const float ahi[4] = {vhi[q0][j], vhi[q0][j + 8], vhi[q0 + 4][j],
+                                              vhi[q0 + 4][j + 8]};
+                        const float alo[4] = {vlo[q0][j], vlo[q0][j + 8], vlo[q0 + 4][j],
+                                              vlo[q0 + 4][j + 8]};
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) {
+                            const float b0 = half_of<T>(m0[i >> 1], i & 1);
+                            const float b1 = half_of<T>(m1[i >> 1], i & 1);
+                            mma_tf32(acc[nj][i], ahi, b0, b1);
+                            mma_tf32(acc[nj][i], alo, b0, b1);
+                        }
+                    }
+                }
+#pragma unroll
+                for (int h = 0; h < 4; ++h) x[h] = next[h];
+            }
+        }
+        if (seg_end > pos || direct)
+            store_sums<T, kNJ>(P, S, acc, int64_t(blockIdx.y) + s, s, c0, j0, g, tq);
+        pos = max(pos, seg_end);
+    }
+}
+
+// out[s][c][j] = the sum of adapter s's slots, in order.
+template <typename T>
+__global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ WgradParams P, int which) {
+    const Side &S = P.side[which];
+    const int64_t ldc = (S.cols + 7) / 8 * 8;
+    const int64_t total = P.start ? P.start[P.s] : P.rows;
+    const int64_t quads = (S.cols + 3) / 4;
+    for (int64_t u = blockIdx.x * int64_t(blockDim.x) + threadIdx.x; u < P.s * P.r * quads;
+         u += int64_t(gridDim.x) * blockDim.x) {
+        const int64_t c = u % quads * 4, j = u / quads % P.r, s = u / (quads * P.r);
+        const int64_t first = P.start ? P.start[s] : 0;
+        const int64_t end = P.start ? P.start[s + 1] : s == 0 ? total : 0;
+        float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        if (end > first)
+            for (int64_t k = first / P.chunk; k <= (end - 1) / P.chunk; ++k) {
+                const float4 a =
+                    *reinterpret_cast<const float4 *>(S.part + ((k + s) * P.r + j) * ldc + c);
+                v.x += a.x;
+                v.y += a.y;
+                v.z += a.z;
+                v.w += a.w;
+            }
+        T *dst = static_cast<T *>(S.out) + s * S.ss + j * S.sr;
+        const float w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (c + e < S.cols) dst[(c + e) * S.sc] = from_float<T>(w[e]);
+    }
+}
+
+}  // namespace
+
+// Chunks of rows: one wave of two CTAs per SM, so that the partial sums, which are written and
+// read once for each chunk, stay few.
+WgradPlan lr_wgrad_plan(int64_t rows, int64_t r, int64_t s, int64_t cols_a, int64_t cols_b,
+                        bool indexed) {
+    constexpr int64_t kCtas = 2 * 148;  // fixed: the workspace is sized without a device
+    WgradPlan p{};
+    const int64_t blocks = ((cols_a + kCtaCols - 1) / kCtaCols + (cols_b + kCtaCols - 1) / kCtaCols) *
+                           (r <= 16 ? 1 : (r + 31) / 32);
+    int64_t chunks = blocks ? kCtas / blocks : 1;
+    const int64_t most = (rows + kStage - 1) / kStage;
+    if (chunks > most) chunks = most;
+    if (chunks < 1) chunks = 1;
+    p.chunk = (rows + chunks - 1) / chunks;
+    p.chunk = (p.chunk + 15) / 16 * 16;
+    if (p.chunk == 0) p.chunk = 16;
+    p.chunks = rows ? (rows + p.chunk - 1) / p.chunk : 1;
+    const int64_t slots = p.chunks + s - 1;
+    p.list_bytes = indexed ? sizeof(int32_t) * static_cast<size_t>(rows + s + 1) : 0;
+    if (p.chunks > 1) {
+        p.part_a = sizeof(float) * static_cast<size_t>(slots * r * ((cols_a + 7) / 8 * 8));
+        p.part_b = sizeof(float) * static_cast<size_t>(slots * r * ((cols_b + 7) / 8 * 8));
+    }
+    return p;
+}
+
+template <typename T>
+static cudaError_t wgrad(const WgradParams &P, const WgradPlan &plan, int num_sms,
+                         cudaStream_t stream) {
+    const int blocks = P.side[0].blocks + P.side[1].blocks;
+    if (blocks == 0) return cudaSuccess;
+    const int nj = P.r <= 16 ? 1 : 2;
+    const dim3 grid(static_cast<unsigned>(blocks), static_cast<unsigned>(plan.chunks),
+                    static_cast<unsigned>((P.r + 16 * nj - 1) / (16 * nj)));
+    if (nj == 1)
+        wgrad_kernel<T, 1><<<grid, kThreads, 0, stream>>>(P);
+    else
+        wgrad_kernel<T, 2><<<grid, kThreads, 0, stream>>>(P);
+    for (int w = 0; w < 2; ++w)
+        if (P.side[w].part) {
+            const int64_t work = P.s * P.r * ((P.side[w].cols + 3) / 4);
+            const int64_t want = (work + 255) / 256, most = int64_t(num_sms) * 8;
+            join_kernel<T><<<static_cast<unsigned>(want < most ? want : most), 256, 0, stream>>>(P, w);
+        }
+    return cudaGetLastError();
+}
+
+cudaError_t lr_wgrad(bool half, const WgradOperand &a, const WgradOperand &b, int64_t rows,
+                     int64_t r, const RowIndex &index, const WgradPlan &plan, void *lists,
+                     int num_sms, cudaStream_t stream) {
+    WgradParams P{};
+    P.rows = rows;
+    P.r = r;
+    P.s = index.s;
+    P.chunk = plan.chunk;
+    const WgradOperand *ops[2] = {&a, &b};
+    for (int w = 0; w < 2; ++w) {
+        const WgradOperand &o = *ops[w];
+        const int blocks = o.out ? static_cast<int>((o.cols + kCtaCols - 1) / kCtaCols) : 0;
+        P.side[w] = Side{o.M.p, o.M.s0, o.cols, o.V, o.drop, blocks ? o.part : nullptr, o.out,
+                         o.ss,  o.sc,   o.sr,   blocks};
+    }
+    if (P.side[0].blocks + P.side[1].blocks == 0) return cudaSuccess;
+    if (index.p) {
+        int32_t *start = static_cast<int32_t *>(lists);
+        int32_t *order = start + index.s + 1;
+        lists_kernel<<<static_cast<unsigned>(index.s), 1024, 0, stream>>>(index, rows, order, start);
+        P.order = order;
+        P.start = start;
+    }
+    return half ? wgrad<__half>(P, plan, num_sms, stream)
+                : wgrad<__nv_bfloat16>(P, plan, num_sms, stream);
+}
+
+}  // namespace ti
