@@ -1,6 +1,9 @@
 // ti_dropout.cu -- Y = dropout(X) with a mask made from a counter-based generator.
 //
 // Memory bound: each element is read once and written once, the mask exists in registers only.
+// One thread takes the 8 columns of one generator block at a time -- 16, 32 or 64 bytes of a row,
+// in 16-byte copies where both matrices allow them -- and two blocks are in flight per thread, so
+// that the loads of one hide behind the ten rounds of the other.
 #include "tensor_inv_crt.h"
 #include "ti_common.cuh"
 #include "ti_low_rank.cuh"
@@ -11,34 +14,91 @@ int device_context(int *num_sms, int **err);
 
 namespace {
 
+constexpr int kThreads = 256, kUnroll = 2;
+
 template <typename T>
-__device__ __forceinline__ T scaled(T v, uint32_t cut) {
-    return from_float<T>(to_float(v) * dropout_scale(cut));
+__device__ __forceinline__ T scaled(T v, double, float scale) {
+    return from_float<T>(to_float(v) * scale);
 }
 template <>
-__device__ __forceinline__ double scaled<double>(double v, uint32_t cut) {
-    return v * (65536.0 / (65536.0 - cut));
+__device__ __forceinline__ double scaled<double>(double v, double scale, float) {
+    return v * scale;
 }
 
-// One thread per block of 8 columns.
 template <typename T>
-__global__ void dropout_kernel(const T *X, int64_t sx0, int64_t sx1, T *Y, int64_t ldy,
-                               int64_t rows, int64_t cols, Dropout drop) {
+struct alignas(16) Block {
+    T v[8];
+};
+
+template <typename T, bool kVec>
+__device__ __forceinline__ void load(Block<T> &x, const T *p, int64_t s1, int64_t n) {
+    if (kVec && n >= 8) {
+        constexpr int kWords = sizeof(x) / 16;
+#pragma unroll
+        for (int w = 0; w < kWords; ++w)
+            reinterpret_cast<uint4 *>(&x)[w] = __ldcs(reinterpret_cast<const uint4 *>(p) + w);
+    } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+            if (j < n) x.v[j] = p[j * s1];
+    }
+}
+
+template <typename T, bool kVec>
+__device__ __forceinline__ void store(const Block<T> &x, T *p, int64_t n) {
+    if (kVec && n >= 8) {
+        constexpr int kWords = sizeof(x) / 16;
+#pragma unroll
+        for (int w = 0; w < kWords; ++w)
+            reinterpret_cast<uint4 *>(p)[w] = reinterpret_cast<const uint4 *>(&x)[w];
+    } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+            if (j < n) p[j] = x.v[j];
+    }
+}
+
+template <typename T, bool kVec>
+__global__ void __launch_bounds__(kThreads)
+    dropout_kernel(const T *X, int64_t sx0, int64_t sx1, T *Y, int64_t ldy, int64_t rows,
+                   int64_t cols, Dropout drop) {
     const int64_t blocks = (cols + 7) >> 3;
     const uint64_t key = dropout_key(drop);
-    for (int64_t u = blockIdx.x * int64_t(blockDim.x) + threadIdx.x; u < rows * blocks;
-         u += int64_t(gridDim.x) * blockDim.x) {
-        const int64_t i = u / blocks, b = u % blocks;
-        const uint4 bits =
-            dropout_bits(drop, key, static_cast<uint32_t>(i), static_cast<uint32_t>(b));
-        for (int j = 0; j < 8; ++j) {
-            const int64_t c = 8 * b + j;
-            if (c >= cols) break;
-            T y = T(0.0f);
-            // cut = 0 copies the bits: a product with 1 would make a NaN canonical
-            if (dropout_kept(bits, j, drop.cut))
-                y = drop.cut ? scaled(X[i * sx0 + c * sx1], drop.cut) : X[i * sx0 + c * sx1];
-            Y[i * ldy + c] = y;
+    const double scale64 = drop.cut > 65535u ? 0.0 : 65536.0 / (65536.0 - drop.cut);
+    const float scale32 = dropout_scale(drop.cut);
+    // unit (i, b): row i, columns 8b ..; a step of the whole grid is (step_i, step_b)
+    const int64_t step = int64_t(gridDim.x) * kThreads;
+    const int64_t step_i = step / blocks, step_b = step % blocks;
+    const int64_t first = blockIdx.x * int64_t(kThreads) + threadIdx.x;
+    int64_t i = first / blocks, b = first % blocks;
+    while (i < rows) {
+        Block<T> x[kUnroll];
+        int64_t ui[kUnroll], ub[kUnroll];
+#pragma unroll
+        for (int u = 0; u < kUnroll; ++u) {
+            ui[u] = i;
+            ub[u] = b;
+            if (i < rows) load<T, kVec>(x[u], X + i * sx0 + 8 * b * sx1, sx1, cols - 8 * b);
+            i += step_i;
+            b += step_b;
+            if (b >= blocks) {
+                b -= blocks;
+                ++i;
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < kUnroll; ++u) {
+            if (ui[u] >= rows) break;
+            if (drop.cut) {  // cut = 0 copies the bits: a product with 1 would change a NaN's
+                const uint4 bits = dropout_bits(drop, key, static_cast<uint32_t>(ui[u]),
+                                                static_cast<uint32_t>(ub[u]));
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+                    x[u].v[j] = dropout_kept(bits, j, drop.cut)
+                                    ? scaled<T>(x[u].v[j], scale64, scale32)
+                                    : T(0.0f);
+            }
+            store<T, kVec>(x[u], Y + ui[u] * ldy + 8 * ub[u], cols - 8 * ub[u]);
         }
     }
 }
@@ -46,10 +106,18 @@ __global__ void dropout_kernel(const T *X, int64_t sx0, int64_t sx1, T *Y, int64
 template <typename T>
 cudaError_t launch(const void *X, int64_t sx0, int64_t sx1, void *Y, int64_t ldy, int64_t rows,
                    int64_t cols, const Dropout &drop, int sms, cudaStream_t st) {
+    constexpr int64_t kPer16 = 16 / sizeof(T);
+    const bool vec = sx1 == 1 && ((reinterpret_cast<uintptr_t>(X) | reinterpret_cast<uintptr_t>(Y)) & 15) == 0 &&
+                     (rows == 1 || (sx0 % kPer16 == 0 && ldy % kPer16 == 0));
     const int64_t units = rows * ((cols + 7) / 8);
-    const int64_t want = (units + 255) / 256, most = int64_t(sms) * 8;
-    dropout_kernel<T><<<static_cast<unsigned>(want < most ? want : most), 256, 0, st>>>(
-        static_cast<const T *>(X), sx0, sx1, static_cast<T *>(Y), ldy, rows, cols, drop);
+    const int64_t want = (units + kThreads - 1) / kThreads, most = int64_t(sms) * 8;
+    const unsigned grid = static_cast<unsigned>(want < most ? want : most);
+    const T *x = static_cast<const T *>(X);
+    T *y = static_cast<T *>(Y);
+    if (vec)
+        dropout_kernel<T, true><<<grid, kThreads, 0, st>>>(x, sx0, sx1, y, ldy, rows, cols, drop);
+    else
+        dropout_kernel<T, false><<<grid, kThreads, 0, st>>>(x, sx0, sx1, y, ldy, rows, cols, drop);
     return cudaGetLastError();
 }
 
