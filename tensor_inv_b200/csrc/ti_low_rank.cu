@@ -117,7 +117,17 @@ cudaError_t clear(void *out, int64_t ldo, int64_t rows, int64_t cols, cudaStream
     return cudaMemset2DAsync(out, 2 * ldo, 0, 2 * cols, rows, st);
 }
 
-template <typename T>
+cudaError_t expand(bool half, const Matrix16 &M, int64_t rows, int64_t inner, const Matrix16 &W,
+                   int64_t cols, const float *P, const Factor16 &F, int64_t r,
+                   const RowIndex &index, const Dropout &drop, void *out, int64_t ldo, int sms,
+                   int *err, cudaStream_t st) {
+    if (!inner) return clear(out, ldo, rows, cols, st);
+    if (rows <= kExpandRowsLimit)
+        return lr_expand_rows(half, M, rows, inner, W, cols, P, F, r, index, drop, out, ldo, sms,
+                              err, st);
+    return lr_expand_pairs(half, M, rows, inner, W, cols, P, F, r, index, drop, out, ldo, err, st);
+}
+
 int forward(const ti_low_rank_t &op, void *Y, int64_t ldy, float *P, Arena &arena, int sms,
             int *err, cudaStream_t st) {
     const RowIndex index{op.index, op.index_bytes == 8, op.s};
@@ -132,13 +142,11 @@ int forward(const ti_low_rank_t &op, void *Y, int64_t ldy, float *P, Arena &aren
                                      Factor16{op.a, op.sa0, op.sa1, op.sa2}, op.r, index, op.scale,
                                      op.alpha * dropout_scale(drop.cut), drop, P, sms, st);
     if (e != cudaSuccess || !op.n) return status(e);
-    if (!op.k) return status(clear(Y, ldy, op.t, op.n, st));
-    return status(lr_expand_pairs(half, X, op.t, op.k, W, op.n, P,
-                                  Factor16{op.b, op.sb0, op.sb2, op.sb1}, op.r, index, Dropout{}, Y,
-                                  ldy, err, st));
+    return status(expand(half, X, op.t, op.k, W, op.n, P,
+                         Factor16{op.b, op.sb0, op.sb2, op.sb1}, op.r, index, Dropout{}, Y, ldy,
+                         sms, err, st));
 }
 
-template <typename T>
 int backward(const ti_low_rank_t &op, const Gradient &g, Arena &arena, int sms, int *err,
              cudaStream_t st) {
     const RowIndex index{op.index, op.index_bytes == 8, op.s};
@@ -160,12 +168,8 @@ int backward(const ti_low_rank_t &op, const Gradient &g, Arena &arena, int sms, 
         if (e != cudaSuccess) return status(e);
     }
     if (g.dX && op.t && op.k) {
-        if (!op.n)
-            e = clear(g.dX, g.lddx, op.t, op.k, st);
-        else
-            e = lr_expand_pairs(half, dY, op.t, op.n, Wt, op.k, dP,
-                                Factor16{op.a, op.sa0, op.sa1, op.sa2}, op.r, index, drop, g.dX,
-                                g.lddx, err, st);
+        e = expand(half, dY, op.t, op.n, Wt, op.k, dP, Factor16{op.a, op.sa0, op.sa1, op.sa2},
+                   op.r, index, drop, g.dX, g.lddx, sms, err, st);
         if (e != cudaSuccess) return status(e);
     }
     return status(lr_wgrad(
@@ -173,18 +177,6 @@ int backward(const ti_low_rank_t &op, const Gradient &g, Arena &arena, int sms, 
         WgradOperand{X, op.k, dP, drop, part_a, g.dA, g.sda[0], g.sda[1], g.sda[2]},
         WgradOperand{dY, op.n, g.P, Dropout{}, part_b, g.dB, g.sdb[0], g.sdb[2], g.sdb[1]}, op.t,
         op.r, index, plan, lists, sms, st));
-}
-
-int run_forward(const ti_low_rank_t &op, void *Y, int64_t ldy, float *P, Arena &arena, int sms,
-                int *err, cudaStream_t st) {
-    return op.dtype == TI_TYPE_F16 ? forward<__half>(op, Y, ldy, P, arena, sms, err, st)
-                                   : forward<__nv_bfloat16>(op, Y, ldy, P, arena, sms, err, st);
-}
-
-int run_backward(const ti_low_rank_t &op, const Gradient &g, Arena &arena, int sms, int *err,
-                 cudaStream_t st) {
-    return op.dtype == TI_TYPE_F16 ? backward<__half>(op, g, arena, sms, err, st)
-                                   : backward<__nv_bfloat16>(op, g, arena, sms, err, st);
 }
 
 bool bad_workspace(const void *ws, size_t have, size_t need) {
@@ -202,7 +194,7 @@ int ti_low_rank_workspace_size(const ti_low_rank_t *op, size_t *bytes) {
     const int rc = check_op(op);
     if (rc != TI_OK || !bytes) return rc != TI_OK ? rc : TI_ERR_INVALID_ARGUMENT;
     Arena count{nullptr, 0};
-    run_forward(*op, nullptr, 0, nullptr, count, 0, nullptr, nullptr);
+    forward(*op, nullptr, 0, nullptr, count, 0, nullptr, nullptr);
     *bytes = count.used;
     return TI_OK;
 }
@@ -216,7 +208,7 @@ int ti_low_rank_backward_workspace_size(const ti_low_rank_t *op, const void *dY,
     g.dY = dY;
     g.sdy0 = sdy0;
     g.sdy1 = sdy1;
-    run_backward(*op, g, count, 0, nullptr, nullptr);
+    backward(*op, g, count, 0, nullptr, nullptr);
     *bytes = count.used;
     return TI_OK;
 }
@@ -234,7 +226,7 @@ int ti_low_rank_matmul(const ti_low_rank_t *op, void *Y, int64_t ldy, float *P, 
         return TI_ERR_INVALID_ARGUMENT;
     if (bad_workspace(workspace, workspace_bytes, need)) return TI_ERR_WORKSPACE;
     Arena arena{static_cast<uint8_t *>(workspace), 0};
-    return run_forward(*op, Y, ldy, P, arena, sms, err, static_cast<cudaStream_t>(stream));
+    return forward(*op, Y, ldy, P, arena, sms, err, static_cast<cudaStream_t>(stream));
 }
 
 int ti_low_rank_backward(const ti_low_rank_t *op, const void *dY, int64_t sdy0, int64_t sdy1,
@@ -256,7 +248,7 @@ int ti_low_rank_backward(const ti_low_rank_t *op, const void *dY, int64_t sdy0, 
     // a call without rows may come without a workspace: there is nothing to pack then
     alignas(256) static uint8_t none[256];
     Arena arena{workspace ? static_cast<uint8_t *>(workspace) : none, 0};
-    return run_backward(*op, g, arena, sms, err, static_cast<cudaStream_t>(stream));
+    return backward(*op, g, arena, sms, err, static_cast<cudaStream_t>(stream));
 }
 
 }  // extern "C"

@@ -32,6 +32,15 @@ cudaError_t lr_expand_pairs(bool half, const Matrix16 &M, int64_t rows, int64_t 
                             int64_t r, const RowIndex &index, const Dropout &drop, void *out,
                             int64_t ldo, int *err, cudaStream_t stream);
 
+// The same for few rows (ti_lr_rows.cu).
+cudaError_t lr_expand_rows(bool half, const Matrix16 &M, int64_t rows, int64_t inner,
+                           const Matrix16 &W, int64_t cols, const float *P, const Factor16 &F,
+                           int64_t r, const RowIndex &index, const Dropout &drop, void *out,
+                           int64_t ldo, int num_sms, int *err, cudaStream_t stream);
+
+// Up to this many rows, expand streams W past the rows; above it, CTA pairs take 256-row tiles.
+constexpr int64_t kExpandRowsLimit = 256;
+
 // The gradients of the adapters (ti_lr_wgrad.cu).
 struct WgradPlan {
     int64_t chunk, chunks;

@@ -149,6 +149,7 @@ __global__ void __launch_bounds__(kTileThreads, 2)
     uint16_t *sF = reinterpret_cast<uint16_t *>(sum + kTileRows * 8 * kNT);  // [2][8*kNT][stride]
     __shared__ unsigned least[2][8];
     __shared__ int sidx[kTileRows];
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int g = lane >> 2, tq = lane & 3;
@@ -300,6 +301,8 @@ __global__ void __launch_bounds__(kRowThreads)
     project_rows_kernel(const __grid_constant__ ProjectParams P) {
     __shared__ float part[kRowThreads / 32][kMaxRankRows];
     __shared__ float sum[kMaxRankRows];
+    // the kernel that reads P may start its own copies now; it waits for this grid before P
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t crank = cluster_rank(), csize = cluster_size();
     const int64_t t = blockIdx.x / csize;
