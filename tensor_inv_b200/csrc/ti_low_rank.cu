@@ -117,15 +117,20 @@ cudaError_t clear(void *out, int64_t ldo, int64_t rows, int64_t cols, cudaStream
     return cudaMemset2DAsync(out, 2 * ldo, 0, 2 * cols, rows, st);
 }
 
-cudaError_t expand(bool half, const Matrix16 &M, int64_t rows, int64_t inner, const Matrix16 &W,
-                   int64_t cols, const float *P, const Factor16 &F, int64_t r,
-                   const RowIndex &index, const Dropout &drop, void *out, int64_t ldo, int sms,
-                   int *err, cudaStream_t st) {
-    if (!inner) return clear(out, ldo, rows, cols, st);
-    if (rows <= kExpandRowsLimit)
-        return lr_expand_rows(half, M, rows, inner, W, cols, P, F, r, index, drop, out, ldo, sms,
-                              err, st);
-    return lr_expand_pairs(half, M, rows, inner, W, cols, P, F, r, index, drop, out, ldo, err, st);
+// The projection, then the expansion that reads it; for very few rows one kernel does both.
+// `want_p`: the projection is needed beyond the expansion.
+cudaError_t project_expand(bool half, const ProjectOperands &p, const ExpandOperands *x, bool want_p,
+                           int sms, int *err, cudaStream_t st) {
+    if (x && x->inner && x->rows <= kFuseRows) {
+        ExpandOperands o = *x;
+        if (!want_p) o.P = nullptr;
+        return lr_expand_rows(half, o, &p, sms, err, st);
+    }
+    const cudaError_t e = lr_project(half, p, sms, st);
+    if (e != cudaSuccess || !x) return e;
+    if (!x->inner) return clear(x->out, x->ldo, x->rows, x->cols, st);
+    return x->rows <= kExpandRowsLimit ? lr_expand_rows(half, *x, nullptr, sms, err, st)
+                                       : lr_expand_pairs(half, *x, err, st);
 }
 
 int forward(const ti_low_rank_t &op, void *Y, int64_t ldy, float *P, Arena &arena, int sms,
@@ -137,14 +142,15 @@ int forward(const ti_low_rank_t &op, void *Y, int64_t ldy, float *P, Arena &aren
     const Matrix16 X = readable(Matrix16{op.x, op.sx0, op.sx1}, op.t, op.k, arena, sms, st);
     const Matrix16 W = readable_w(Matrix16{op.w, op.sw0, op.sw1}, op.k, op.n, arena, sms, st);
     if (!arena.base) return TI_OK;
-    const bool half = op.dtype == TI_TYPE_F16;
-    const cudaError_t e = lr_project(half, X, op.t, op.k,
-                                     Factor16{op.a, op.sa0, op.sa1, op.sa2}, op.r, index, op.scale,
-                                     op.alpha * dropout_scale(drop.cut), drop, P, sms, st);
-    if (e != cudaSuccess || !op.n) return status(e);
-    return status(expand(half, X, op.t, op.k, W, op.n, P,
-                         Factor16{op.b, op.sb0, op.sb2, op.sb1}, op.r, index, Dropout{}, Y, ldy,
-                         sms, err, st));
+    const ProjectOperands p{X,     op.t,     op.k,
+                            Factor16{op.a, op.sa0, op.sa1, op.sa2},
+                            op.r,  index,    op.scale,
+                            op.alpha * dropout_scale(drop.cut),
+                            drop,  P};
+    const ExpandOperands x{X,    op.t,  op.k,      W,  op.n, P, Factor16{op.b, op.sb0, op.sb2, op.sb1},
+                           op.r, index, Dropout{}, Y,  ldy};
+    return status(project_expand(op.dtype == TI_TYPE_F16, p, op.n ? &x : nullptr, P != own, sms, err,
+                                 st));
 }
 
 int backward(const ti_low_rank_t &op, const Gradient &g, Arena &arena, int sms, int *err,
@@ -160,16 +166,17 @@ int backward(const ti_low_rank_t &op, const Gradient &g, Arena &arena, int sms, 
     float *part_a = plan.part_a ? static_cast<float *>(arena.take(plan.part_a)) : nullptr;
     float *part_b = plan.part_b ? static_cast<float *>(arena.take(plan.part_b)) : nullptr;
     if (!arena.base) return TI_OK;
-    cudaError_t e = cudaSuccess;
     const bool half = op.dtype == TI_TYPE_F16;
     if ((g.dX || g.dA) && op.t) {
-        e = lr_project(half, dY, op.t, op.n, Factor16{op.b, op.sb0, op.sb2, op.sb1}, op.r, index,
-                       op.scale, op.alpha * dropout_scale(drop.cut), Dropout{}, dP, sms, st);
-        if (e != cudaSuccess) return status(e);
-    }
-    if (g.dX && op.t && op.k) {
-        e = expand(half, dY, op.t, op.n, Wt, op.k, dP, Factor16{op.a, op.sa0, op.sa1, op.sa2},
-                   op.r, index, drop, g.dX, g.lddx, sms, err, st);
+        const ProjectOperands p{dY,    op.t,     op.n,
+                                Factor16{op.b, op.sb0, op.sb2, op.sb1},
+                                op.r,  index,    op.scale,
+                                op.alpha * dropout_scale(drop.cut),
+                                Dropout{}, dP};
+        const ExpandOperands x{dY,   op.t,  op.n, Wt,   op.k, dP, Factor16{op.a, op.sa0, op.sa1, op.sa2},
+                               op.r, index, drop, g.dX, g.lddx};
+        const cudaError_t e =
+            project_expand(half, p, g.dX && op.k ? &x : nullptr, g.dA != nullptr, sms, err, st);
         if (e != cudaSuccess) return status(e);
     }
     return status(lr_wgrad(

@@ -102,30 +102,6 @@ __device__ __forceinline__ void umma_tf32_pair(uint32_t d, uint64_t a, uint64_t 
         : "memory");
 }
 
-__device__ __forceinline__ bool try_wait_cluster(uint32_t bar, uint32_t parity) {
-    uint32_t ok;
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
-        "selp.u32 %0, 1, 0, p;\n\t}"
-        : "=r"(ok)
-        : "r"(bar), "r"(parity)
-        : "memory");
-    return ok != 0;
-}
-
-// mbar_wait for a barrier that the other CTA's threads arrive on after writing shared memory.
-__device__ __forceinline__ bool mbar_wait_cluster(uint64_t *bar, uint32_t parity,
-                                                  volatile int *abort) {
-    const uint32_t a = smem_u32(bar);
-    if (try_wait_cluster(a, parity)) return true;
-    const unsigned long long t0 = globaltimer_ns();
-    while (!try_wait_cluster(a, parity)) {
-        if (*abort || globaltimer_ns() - t0 > kWaitTimeoutNs) return false;
-    }
-    return true;
-}
-
 __device__ __forceinline__ void loader_sync() {
     asm volatile("bar.sync 1, %0;" ::"n"(kLoaders) : "memory");
 }
@@ -624,38 +600,36 @@ cudaError_t launch(const CUtensorMap &tmM, const CUtensorMap &tmW, const Params 
 }
 
 template <typename T>
-cudaError_t expand(const Matrix16 &M, int64_t rows, int64_t inner, const Matrix16 &W, int64_t cols,
-                   const float *Pj, const Factor16 &F, int64_t r, const RowIndex &index,
-                   const Dropout &drop, void *out, int64_t ldo, int *err, cudaStream_t stream) {
-    const int bn = drop.cut ? 128 : 256;
+cudaError_t expand(const ExpandOperands &o, int *err, cudaStream_t stream) {
+    const int bn = o.drop.cut ? 128 : 256;
     Params P;
     std::memset(&P, 0, sizeof(P));
-    P.rows = rows;
-    P.cols = cols;
-    P.num_kb = static_cast<int>((inner + kBK - 1) / kBK);
-    P.tiles_m = static_cast<int>((rows + kBM - 1) / kBM);
-    P.tiles_n = static_cast<int>((cols + bn - 1) / bn);
+    P.rows = o.rows;
+    P.cols = o.cols;
+    P.num_kb = static_cast<int>((o.inner + kBK - 1) / kBK);
+    P.tiles_m = static_cast<int>((o.rows + kBM - 1) / kBM);
+    P.tiles_n = static_cast<int>((o.cols + bn - 1) / bn);
     P.total = int64_t(P.tiles_m) * P.tiles_n;
-    P.w_nmajor = W.s0 != 1;
+    P.w_nmajor = o.W.s0 != 1;
     const int type = std::is_same<T, __half>::value ? 0 : 1;
     P.idesc16 = idesc(type, bn, P.w_nmajor);
     P.idesc32 = idesc(2, bn, false);
-    P.P = Pj;
-    P.r = r;
-    P.F = F;
-    P.index = index;
-    P.drop = drop;
-    P.out = out;
-    P.ldo = ldo;
-    P.vec = ldo % 8 == 0 && (reinterpret_cast<uintptr_t>(out) & 15) == 0;
+    P.P = o.P;
+    P.r = o.r;
+    P.F = o.F;
+    P.index = o.index;
+    P.drop = o.drop;
+    P.out = o.out;
+    P.ldo = o.ldo;
+    P.vec = o.ldo % 8 == 0 && (reinterpret_cast<uintptr_t>(o.out) & 15) == 0;
     P.err = err;
     CUtensorMap tmM, tmW;
-    if (!make_map16(&tmM, M.p, inner, rows, M.s0, kBK, kHalf)) return cudaErrorInvalidValue;
-    if (P.w_nmajor ? !make_map16(&tmW, W.p, cols, inner, W.s0, 64, kBK)
-                   : !make_map16(&tmW, W.p, inner, cols, W.s1, kBK, bn / 2))
+    if (!make_map16(&tmM, o.M.p, o.inner, o.rows, o.M.s0, kBK, kHalf)) return cudaErrorInvalidValue;
+    if (P.w_nmajor ? !make_map16(&tmW, o.W.p, o.cols, o.inner, o.W.s0, 64, kBK)
+                   : !make_map16(&tmW, o.W.p, o.inner, o.cols, o.W.s1, kBK, bn / 2))
         return cudaErrorInvalidValue;
-    return drop.cut ? launch<T, 128, true>(tmM, tmW, P, stream)
-                    : launch<T, 256, false>(tmM, tmW, P, stream);
+    return o.drop.cut ? launch<T, 128, true>(tmM, tmW, P, stream)
+                      : launch<T, 256, false>(tmM, tmW, P, stream);
 }
 
 }  // namespace
@@ -673,13 +647,8 @@ bool make_map16(CUtensorMap *map, const void *base, int64_t inner, int64_t outer
                CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-cudaError_t lr_expand_pairs(bool half, const Matrix16 &M, int64_t rows, int64_t inner,
-                            const Matrix16 &W, int64_t cols, const float *P, const Factor16 &F,
-                            int64_t r, const RowIndex &index, const Dropout &drop, void *out,
-                            int64_t ldo, int *err, cudaStream_t stream) {
-    return half ? expand<__half>(M, rows, inner, W, cols, P, F, r, index, drop, out, ldo, err, stream)
-                : expand<__nv_bfloat16>(M, rows, inner, W, cols, P, F, r, index, drop, out, ldo, err,
-                                        stream);
+cudaError_t lr_expand_pairs(bool half, const ExpandOperands &o, int *err, cudaStream_t stream) {
+    return half ? expand<__half>(o, err, stream) : expand<__nv_bfloat16>(o, err, stream);
 }
 
 }  // namespace ti

@@ -21,25 +21,44 @@ inline bool copyable(const void *p, int64_t rows, int64_t ld, int64_t s_inner, i
 // Up to this many rows, project runs a cluster per row, above it tiles of 128 rows.
 constexpr int64_t kProjectRowsLimit = 256;
 
-// P = f (m M) F (ti_lr_project.cu): M with unit s1 and copyable.
-cudaError_t lr_project(bool half, const Matrix16 &M, int64_t rows, int64_t cols, const Factor16 &F,
-                       int64_t r, const RowIndex &index, const float *scale, float alpha,
-                       const Dropout &drop, float *P, int num_sms, cudaStream_t stream);
+// P = f (m M) F: the rows' projections, F a factor along M's inner dimension.
+struct ProjectOperands {
+    Matrix16 M;  // unit s1, copyable
+    int64_t rows, cols;
+    Factor16 F;
+    int64_t r;
+    RowIndex index;
+    const float *scale;
+    float alpha;
+    Dropout drop;
+    float *P;
+};
+cudaError_t lr_project(bool half, const ProjectOperands &o, int num_sms, cudaStream_t stream);
 
-// out = M W + P F (ti_lr_gemm.cu): M with unit s1, W with one unit stride, both copyable.
-cudaError_t lr_expand_pairs(bool half, const Matrix16 &M, int64_t rows, int64_t inner,
-                            const Matrix16 &W, int64_t cols, const float *P, const Factor16 &F,
-                            int64_t r, const RowIndex &index, const Dropout &drop, void *out,
-                            int64_t ldo, int *err, cudaStream_t stream);
-
-// The same for few rows (ti_lr_rows.cu).
-cudaError_t lr_expand_rows(bool half, const Matrix16 &M, int64_t rows, int64_t inner,
-                           const Matrix16 &W, int64_t cols, const float *P, const Factor16 &F,
-                           int64_t r, const RowIndex &index, const Dropout &drop, void *out,
-                           int64_t ldo, int num_sms, int *err, cudaStream_t stream);
+// out = M W + m (P F), F a factor along out's columns.
+struct ExpandOperands {
+    Matrix16 M;  // unit s1, copyable
+    int64_t rows, inner;
+    Matrix16 W;  // one unit stride, copyable
+    int64_t cols;
+    float *P;
+    Factor16 F;
+    int64_t r;
+    RowIndex index;
+    Dropout drop;
+    void *out;
+    int64_t ldo;
+};
+// 256-row tiles on CTA pairs (ti_lr_gemm.cu)
+cudaError_t lr_expand_pairs(bool half, const ExpandOperands &o, int *err, cudaStream_t stream);
+// W streamed past a few rows (ti_lr_rows.cu).  With `fuse` (rows <= kFuseRows) it makes the
+// projection too and o.P is written where it is not null.
+cudaError_t lr_expand_rows(bool half, const ExpandOperands &o, const ProjectOperands *fuse,
+                           int num_sms, int *err, cudaStream_t stream);
 
 // Up to this many rows, expand streams W past the rows; above it, CTA pairs take 256-row tiles.
 constexpr int64_t kExpandRowsLimit = 256;
+constexpr int kFuseRows = 4;
 
 // The gradients of the adapters (ti_lr_wgrad.cu).
 struct WgradPlan {

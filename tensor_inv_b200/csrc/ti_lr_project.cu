@@ -12,9 +12,7 @@
 //          and every row keeps the result of its own.
 //   rows:  one row per cluster, plain multiply-adds: for few rows each with an adapter of its own
 //          F's bytes bound it, and no product is shared between rows.
-#include <type_traits>
-
-#include "ti_common.cuh"
+#include "ti_lr_dot.cuh"
 #include "ti_lr_launch.cuh"
 
 namespace ti {
@@ -33,32 +31,6 @@ struct ProjectParams {
     int64_t slice;  // inner elements per CTA, a multiple of 128 (tiles) or 256 (rows)
     int mode;       // how F is read: kFC vectors along c, kFR vectors along j, kFScalar
 };
-
-enum { kFScalar = 0, kFC = 1, kFR = 2 };
-
-__device__ __forceinline__ uint32_t keep2(uint32_t x, uint32_t bits, uint32_t cut2) {
-    return x & __vcmpgeu2(bits, cut2);  // halves whose 16 bits are below the cut become 0
-}
-
-// 8 elements of a row with the mask applied; cut = 65536 (everything dropped) has no 16-bit form.
-__device__ __forceinline__ uint4 masked(uint4 v, const Dropout &d, uint64_t key, uint32_t row,
-                                        uint32_t block) {
-    if (d.cut > 65535u) return make_uint4(0, 0, 0, 0);
-    const uint4 b = dropout_bits(d, key, row, block);
-    const uint32_t cut2 = d.cut * 0x10001u;
-    return make_uint4(keep2(v.x, b.x, cut2), keep2(v.y, b.y, cut2), keep2(v.z, b.z, cut2),
-                      keep2(v.w, b.w, cut2));
-}
-
-// 8 consecutive elements at `p`, of which the first n exist (n <= 0: none)
-__device__ __forceinline__ uint4 load8(const uint16_t *p, int64_t n) {
-    if (n >= 8) return __ldg(reinterpret_cast<const uint4 *>(p));
-    uint32_t w[4] = {0, 0, 0, 0};
-#pragma unroll
-    for (int e = 0; e < 8; ++e)
-        if (e < n) w[e >> 1] |= static_cast<uint32_t>(p[e]) << (16 * (e & 1));
-    return make_uint4(w[0], w[1], w[2], w[3]);
-}
 
 template <typename T>
 __device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2,
@@ -82,22 +54,6 @@ __device__ __forceinline__ void mma16816<__half>(float (&d)[4], uint32_t a0, uin
         "{%8,%9}, {%0,%1,%2,%3};"
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-}
-
-// A float in the shared memory of CTA `rank` of the cluster, at this CTA's address `p`.
-__device__ __forceinline__ float load_remote(const float *p, uint32_t rank) {
-    float v;
-    asm volatile("ld.shared::cluster.f32 %0, [%1];"
-                 : "=f"(v)
-                 : "r"(map_to_rank(smem_u32(p), rank))
-                 : "memory");
-    return v;
-}
-
-__device__ __forceinline__ uint32_t cluster_size() {
-    uint32_t n;
-    asm volatile("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(n));
-    return n;
 }
 
 constexpr int kTileRows = 128, kTileThreads = 256, kGroups = 2;  // two groups share the slice
@@ -276,30 +232,14 @@ __global__ void __launch_bounds__(kTileThreads, 2)
 // ---------------------------------------------------------------------------------------
 // few rows: a cluster per row
 // ---------------------------------------------------------------------------------------
-constexpr int kRowThreads = 128;
-constexpr int kRowChunk = 256;  // inner elements a warp takes per step: 8 per lane
+constexpr int kRowThreads = 256;
 constexpr int kMaxRankRows = 256;
-
-template <typename T>
-__device__ __forceinline__ void unpack8(uint4 v, float (&f)[8]) {
-    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-        if constexpr (std::is_same<T, __nv_bfloat16>::value) {
-            f[2 * e] = __uint_as_float(w[e] << 16);
-            f[2 * e + 1] = __uint_as_float(w[e] & 0xFFFF0000u);
-        } else {
-            const float2 h = __half22float2(*reinterpret_cast<const __half2 *>(&w[e]));
-            f[2 * e] = h.x;
-            f[2 * e + 1] = h.y;
-        }
-    }
-}
 
 template <typename T, bool kDrop>
 __global__ void __launch_bounds__(kRowThreads)
     project_rows_kernel(const __grid_constant__ ProjectParams P) {
-    __shared__ float part[kRowThreads / 32][kMaxRankRows];
+    constexpr int kWarps = kRowThreads / 32;
+    __shared__ float part[kWarps][kMaxRankRows];
     __shared__ float sum[kMaxRankRows];
     // the kernel that reads P may start its own copies now; it waits for this grid before P
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
@@ -309,72 +249,19 @@ __global__ void __launch_bounds__(kRowThreads)
     const int i = P.index.at(t);
     const int64_t begin = int64_t(crank) * P.slice, end = min(P.cols, begin + P.slice);
     const int r = static_cast<int>(P.r);
-    for (int e = threadIdx.x; e < (kRowThreads / 32) * kMaxRankRows; e += kRowThreads)
-        (&part[0][0])[e] = 0.0f;
+    if (i >= 0)
+        dot_slice<T, kDrop, kWarps>(
+            static_cast<const uint16_t *>(P.M) + t * P.ld,
+            static_cast<const uint16_t *>(P.F.p) + i * P.F.ss, P.F.sc, P.F.sr, P.mode, r, begin,
+            end, P.drop, kDrop ? dropout_key(P.drop) : 0, static_cast<uint32_t>(t), warp, lane,
+            &part[0][0], kMaxRankRows);
     __syncthreads();
-    if (i >= 0) {
-        const uint16_t *M = static_cast<const uint16_t *>(P.M) + t * P.ld;
-        const uint16_t *F = static_cast<const uint16_t *>(P.F.p) + i * P.F.ss;
-        const uint64_t key = kDrop ? dropout_key(P.drop) : 0;
-        // each warp takes every fourth chunk of 256 inner elements, 8 per lane
-        for (int64_t c0 = begin + warp * kRowChunk; c0 < end; c0 += 4 * kRowChunk) {
-            const int64_t c = c0 + 8 * lane;
-            uint4 xv = load8(M + c, end - c);
-            if (kDrop)
-                xv = masked(xv, P.drop, key, static_cast<uint32_t>(t), static_cast<uint32_t>(c >> 3));
-            float x[8];
-            unpack8<T>(xv, x);
-            if (P.mode == kFR) {
-                for (int jb = 0; jb < r; jb += 8) {
-                    uint4 fv[8];
-                    float acc[8];
-#pragma unroll
-                    for (int e = 0; e < 8; ++e)
-                        fv[e] = c + e < end ? load8(F + (c + e) * P.F.sc + jb, r - jb)
-                                            : make_uint4(0, 0, 0, 0);
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) acc[e] = 0.0f;
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) {
-                        float f[8];
-                        unpack8<T>(fv[e], f);
-#pragma unroll
-                        for (int j = 0; j < 8; ++j) acc[j] += x[e] * f[j];
-                    }
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) {
-                        float v = acc[j];
-#pragma unroll
-                        for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xFFFFFFFFu, v, o);
-                        if (lane == 0 && jb + j < r) part[warp][jb + j] += v;
-                    }
-                }
-            } else {
-#pragma unroll 4
-                for (int j = 0; j < r; ++j) {
-                    float f[8];
-                    if (P.mode == kFC) {
-                        unpack8<T>(load8(F + j * P.F.sr + c, end - c), f);
-                    } else {
-#pragma unroll
-                        for (int e = 0; e < 8; ++e)
-                            f[e] = c + e < end ? to_float(*reinterpret_cast<const T *>(
-                                                     F + (c + e) * P.F.sc + j * P.F.sr))
-                                               : 0.0f;
-                    }
-                    float v = 0.0f;
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) v += x[e] * f[e];
-#pragma unroll
-                    for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xFFFFFFFFu, v, o);
-                    if (lane == 0) part[warp][j] += v;
-                }
-            }
-        }
+    for (int j = threadIdx.x; j < r; j += kRowThreads) {
+        float v = 0.0f;
+        if (i >= 0)
+            for (int w = 0; w < kWarps; ++w) v += part[w][j];
+        sum[j] = v;
     }
-    __syncthreads();
-    for (int j = threadIdx.x; j < r; j += kRowThreads)
-        sum[j] = (part[0][j] + part[1][j]) + (part[2][j] + part[3][j]);
     cluster_sync_all();
     if (crank == 0)
         for (int j = threadIdx.x; j < r; j += kRowThreads) {
@@ -383,13 +270,6 @@ __global__ void __launch_bounds__(kRowThreads)
             P.P[t * P.r + j] = i < 0 ? 0.0f : v * (P.alpha * (P.scale ? P.scale[i] : 1.0f));
         }
     cluster_sync_all();
-}
-
-int factor_mode(const Factor16 &F) {
-    const bool base = (reinterpret_cast<uintptr_t>(F.p) & 15) == 0 && F.ss % 8 == 0;
-    if (base && F.sc == 1 && F.sr % 8 == 0) return kFC;
-    if (base && F.sr == 1 && F.sc % 8 == 0) return kFR;
-    return kFScalar;
 }
 
 template <typename K>
@@ -430,9 +310,9 @@ template <typename T>
 cudaError_t project(ProjectParams P, int num_sms, cudaStream_t stream) {
     int parts = 1;
     if (P.rows <= kProjectRowsLimit) {
-        // slices of 1024 (256 for each warp) until 8 CTAs share a row
+        // slices of 1024 (8 elements for each of 128 lanes) until 8 CTAs share a row
         while (parts < 8 && P.cols > 1024 * parts) ++parts;
-        P.slice = ((P.cols + parts - 1) / parts + kRowChunk - 1) / kRowChunk * kRowChunk;
+        P.slice = ((P.cols + parts - 1) / parts + 255) / 256 * 256;
         const dim3 grid(static_cast<unsigned>(parts * P.rows));
         return P.drop.cut ? launch_cluster(project_rows_kernel<T, true>, parts, grid, kRowThreads,
                                            0, P, stream)
@@ -459,11 +339,9 @@ cudaError_t project(ProjectParams P, int num_sms, cudaStream_t stream) {
 
 }  // namespace
 
-cudaError_t lr_project(bool half, const Matrix16 &M, int64_t rows, int64_t cols, const Factor16 &F,
-                       int64_t r, const RowIndex &index, const float *scale, float alpha,
-                       const Dropout &drop, float *Pout, int num_sms, cudaStream_t stream) {
-    ProjectParams P{M.p,  M.s0, rows, cols, F,    r, index, scale, alpha,
-                    drop, Pout, 0,    factor_mode(F)};
+cudaError_t lr_project(bool half, const ProjectOperands &o, int num_sms, cudaStream_t stream) {
+    const ProjectParams P{o.M.p,   o.M.s0,  o.rows, o.cols, o.F, o.r,
+                          o.index, o.scale, o.alpha, o.drop, o.P, 0, factor_mode(o.F)};
     return half ? project<__half>(P, num_sms, stream) : project<__nv_bfloat16>(P, num_sms, stream);
 }
 

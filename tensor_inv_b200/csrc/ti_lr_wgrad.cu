@@ -17,9 +17,7 @@
 //          crosses from one adapter to the next it writes its sums to another slot: chunk + adapter
 //          numbers the (chunk, adapter) pairs that occur without gaps in either direction.
 //   join   adds an adapter's slots in order and rounds once.  One chunk needs no join.
-#include <type_traits>
-
-#include "ti_common.cuh"
+#include "ti_lr_dot.cuh"
 #include "ti_lr_launch.cuh"
 
 namespace ti {
@@ -46,15 +44,6 @@ struct WgradParams {
     const int32_t *start;   // [s + 1] first position of each adapter, or null
     int64_t chunk;
 };
-
-__device__ __forceinline__ uint4 load8(const uint16_t *p, int64_t n) {
-    if (n >= 8) return __ldg(reinterpret_cast<const uint4 *>(p));
-    uint32_t w[4] = {0, 0, 0, 0};
-#pragma unroll
-    for (int e = 0; e < 8; ++e)
-        if (e < n) w[e >> 1] |= static_cast<uint32_t>(p[e]) << (16 * (e & 1));
-    return make_uint4(w[0], w[1], w[2], w[3]);
-}
 
 template <typename T>
 __device__ __forceinline__ float half_of(uint32_t w, int hi) {
@@ -166,7 +155,6 @@ __global__ void __launch_bounds__(kThreads, 2) wgrad_kernel(const __grid_constan
     int64_t pos = int64_t(blockIdx.y) * P.chunk;
     const int64_t stop = min(total, pos + P.chunk);
     const uint64_t key = S.drop.cut ? dropout_key(S.drop) : 0;
-    const uint32_t cut2 = S.drop.cut * 0x10001u;
 
     // the first adapter whose rows reach past pos (from the first one, where every adapter's
     // gradient is written here)
@@ -230,14 +218,9 @@ __global__ void __launch_bounds__(kThreads, 2) wgrad_kernel(const __grid_constan
                 if (S.drop.cut) {
 #pragma unroll
                     for (int h = 0; h < 4; ++h) {
-                        const uint4 bits =
-                            dropout_bits(S.drop, key, static_cast<uint32_t>(srow[q + 4 * h + tq]),
-                                         static_cast<uint32_t>(col >> 3));
-                        const bool none = S.drop.cut > 65535u;  // everything is dropped
-                        x[h].x = none ? 0 : x[h].x & __vcmpgeu2(bits.x, cut2);
-                        x[h].y = none ? 0 : x[h].y & __vcmpgeu2(bits.y, cut2);
-                        x[h].z = none ? 0 : x[h].z & __vcmpgeu2(bits.z, cut2);
-                        x[h].w = none ? 0 : x[h].w & __vcmpgeu2(bits.w, cut2);
+                        x[h] = masked(x[h], S.drop, key,
+                                      static_cast<uint32_t>(srow[q + 4 * h + tq]),
+                                      static_cast<uint32_t>(col >> 3));
                     }
                 }
 #pragma unroll
