@@ -117,19 +117,13 @@ cudaError_t clear(void *out, int64_t ldo, int64_t rows, int64_t cols, cudaStream
     return cudaMemset2DAsync(out, 2 * ldo, 0, 2 * cols, rows, st);
 }
 
-// The projection, then the expansion that reads it; for very few rows one kernel does both.
-// `want_p`: the projection is needed beyond the expansion.
-cudaError_t project_expand(bool half, const ProjectOperands &p, const ExpandOperands *x, bool want_p,
-                           int sms, int *err, cudaStream_t st) {
-    if (x && x->inner && x->rows <= kFuseRows) {
-        ExpandOperands o = *x;
-        if (!want_p) o.P = nullptr;
-        return lr_expand_rows(half, o, &p, sms, err, st);
-    }
+// The projection, then the expansion that reads it.
+cudaError_t project_expand(bool half, const ProjectOperands &p, const ExpandOperands *x, int sms,
+                           int *err, cudaStream_t st) {
     const cudaError_t e = lr_project(half, p, sms, st);
     if (e != cudaSuccess || !x) return e;
     if (!x->inner) return clear(x->out, x->ldo, x->rows, x->cols, st);
-    return x->rows <= kExpandRowsLimit ? lr_expand_rows(half, *x, nullptr, sms, err, st)
+    return x->rows <= kExpandRowsLimit ? lr_expand_rows(half, *x, sms, err, st)
                                        : lr_expand_pairs(half, *x, err, st);
 }
 
@@ -149,8 +143,7 @@ int forward(const ti_low_rank_t &op, void *Y, int64_t ldy, float *P, Arena &aren
                             drop,  P};
     const ExpandOperands x{X,    op.t,  op.k,      W,  op.n, P, Factor16{op.b, op.sb0, op.sb2, op.sb1},
                            op.r, index, Dropout{}, Y,  ldy};
-    return status(project_expand(op.dtype == TI_TYPE_F16, p, op.n ? &x : nullptr, P != own, sms, err,
-                                 st));
+    return status(project_expand(op.dtype == TI_TYPE_F16, p, op.n ? &x : nullptr, sms, err, st));
 }
 
 int backward(const ti_low_rank_t &op, const Gradient &g, Arena &arena, int sms, int *err,
@@ -176,7 +169,7 @@ int backward(const ti_low_rank_t &op, const Gradient &g, Arena &arena, int sms, 
         const ExpandOperands x{dY,   op.t,  op.n, Wt,   op.k, dP, Factor16{op.a, op.sa0, op.sa1, op.sa2},
                                op.r, index, drop, g.dX, g.lddx};
         const cudaError_t e =
-            project_expand(half, p, g.dX && op.k ? &x : nullptr, g.dA != nullptr, sms, err, st);
+            project_expand(half, p, g.dX && op.k ? &x : nullptr, sms, err, st);
         if (e != cudaSuccess) return status(e);
     }
     return status(lr_wgrad(

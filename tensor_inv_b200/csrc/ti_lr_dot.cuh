@@ -1,5 +1,4 @@
-// ti_lr_dot.cuh -- one row times its adapter's factor over a slice of the inner dimension, by
-// a group of warps; 16-bit loads shared by the kernels of the low-rank products.
+// ti_lr_dot.cuh -- loads and small pieces shared by the kernels of the low-rank products.
 #pragma once
 
 #include <type_traits>
@@ -78,67 +77,6 @@ __device__ __forceinline__ uint32_t cluster_size() {
     uint32_t n;
     asm volatile("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(n));
     return n;
-}
-
-// part[w][j] (w < kWarps) such that its sum over w is sum_{c in [begin, end)} m(t, c) x[c] F[c][j].
-// Called by kWarps whole warps; begin is a multiple of 8.  The caller synchronises afterwards.
-//   vectors along c:    a warp takes a rank at a time, its lanes 8 elements of c each
-//   vectors along rank: a warp takes a part of the slice, its lanes one element of c each
-template <typename T, bool kDrop, int kWarps>
-__device__ __forceinline__ void dot_slice(const uint16_t *x, const uint16_t *F, int64_t sc,
-                                          int64_t sr, int mode, int r, int64_t begin, int64_t end,
-                                          const Dropout &drop, uint64_t key, uint32_t row,
-                                          int warp, int lane, float *part, int part_stride) {
-    if (mode == kFR) {
-        const int64_t share = ((end - begin + kWarps - 1) / kWarps + 7) / 8 * 8;
-        const int64_t lo = begin + warp * share, hi = min(end, lo + share);
-        for (int jb = 0; jb < r; jb += 8) {
-            float acc[8];
-#pragma unroll
-            for (int j = 0; j < 8; ++j) acc[j] = 0.0f;
-#pragma unroll 8
-            for (int64_t c = lo + lane; c < hi; c += 32) {
-                float f[8];
-                unpack8<T>(load8(F + c * sc + jb, r - jb), f);
-                float v = to_float(*reinterpret_cast<const T *>(x + c));
-                if (kDrop)
-                    if (!dropout_kept(dropout_bits(drop, key, row, static_cast<uint32_t>(c >> 3)),
-                                      static_cast<int>(c & 7), drop.cut))
-                        v = 0.0f;
-#pragma unroll
-                for (int j = 0; j < 8; ++j) acc[j] += v * f[j];
-            }
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const float v = warp_sum(acc[j]);
-                if (lane == 0 && jb + j < r) part[warp * part_stride + jb + j] = v;
-            }
-        }
-        return;
-    }
-    for (int j = warp; j < r; j += kWarps) {
-        float acc = 0.0f;
-#pragma unroll 4
-        for (int64_t c = begin + 8 * lane; c < end; c += 256) {
-            uint4 xv = load8(x + c, end - c);
-            if (kDrop) xv = masked(xv, drop, key, row, static_cast<uint32_t>(c >> 3));
-            float v[8], f[8];
-            unpack8<T>(xv, v);
-            if (mode == kFC) {
-                unpack8<T>(load8(F + j * sr + c, end - c), f);
-            } else {
-#pragma unroll
-                for (int e = 0; e < 8; ++e)
-                    f[e] = c + e < end
-                               ? to_float(*reinterpret_cast<const T *>(F + (c + e) * sc + j * sr))
-                               : 0.0f;
-            }
-#pragma unroll
-            for (int e = 0; e < 8; ++e) acc += v[e] * f[e];
-        }
-        acc = warp_sum(acc);
-        if (lane < kWarps) part[lane * part_stride + j] = lane == 0 ? acc : 0.0f;
-    }
 }
 
 }  // namespace ti

@@ -51,14 +51,13 @@ struct ExpandOperands {
 };
 // 256-row tiles on CTA pairs (ti_lr_gemm.cu)
 cudaError_t lr_expand_pairs(bool half, const ExpandOperands &o, int *err, cudaStream_t stream);
-// W streamed past a few rows (ti_lr_rows.cu).  With `fuse` (rows <= kFuseRows) it makes the
-// projection too and o.P is written where it is not null.
-cudaError_t lr_expand_rows(bool half, const ExpandOperands &o, const ProjectOperands *fuse,
-                           int num_sms, int *err, cudaStream_t stream);
+// W streamed past a few rows (ti_lr_rows.cu); launched directly behind the projection that makes
+// o.P, whose other operands it reads before that has finished.
+cudaError_t lr_expand_rows(bool half, const ExpandOperands &o, int num_sms, int *err,
+                           cudaStream_t stream);
 
 // Up to this many rows, expand streams W past the rows; above it, CTA pairs take 256-row tiles.
 constexpr int64_t kExpandRowsLimit = 256;
-constexpr int kFuseRows = 4;
 
 // The gradients of the adapters (ti_lr_wgrad.cu).
 struct WgradPlan {

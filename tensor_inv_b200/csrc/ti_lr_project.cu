@@ -232,16 +232,119 @@ __global__ void __launch_bounds__(kTileThreads, 2)
 // ---------------------------------------------------------------------------------------
 // few rows: a cluster per row
 // ---------------------------------------------------------------------------------------
-constexpr int kRowThreads = 256;
+constexpr int kRowThreads = 256, kRowWarps = kRowThreads / 32;
 constexpr int kMaxRankRows = 256;
 
+// part[w][j] such that its sum over the warps w is sum_{c in [begin, end)} m(t, c) x[c] F[c][j].
+// begin is a multiple of 8; the caller synchronises afterwards.  All reads of a step are issued
+// before the first is used: a step covers 1024 elements and 16 ranks, the whole of a usual slice.
+//   vectors along c, or element by element: a warp takes two ranks, its lanes 8 elements each
+//   vectors along the rank: a warp takes an eighth of the slice, its lanes one element each
 template <typename T, bool kDrop>
-__global__ void __launch_bounds__(kRowThreads)
+__device__ __forceinline__ void dot_slice(const ProjectParams &P, const uint16_t *x,
+                                          const uint16_t *F, int64_t begin, int64_t end,
+                                          uint64_t key, uint32_t row, int warp, int lane,
+                                          float (*part)[kMaxRankRows]) {
+    const int r = static_cast<int>(P.r);
+    if (P.mode == kFR) {
+        const int64_t share = (end - begin + 8 * kRowWarps - 1) / (8 * kRowWarps) * 8;
+        const int64_t lo = begin + warp * share, hi = min(end, lo + share);
+        for (int jb = 0; jb < r; jb += 16) {
+            float acc[16];
+#pragma unroll
+            for (int j = 0; j < 16; ++j) acc[j] = 0.0f;
+            for (int64_t c0 = lo + lane; c0 - lane < hi; c0 += 128) {
+                uint4 f[4][2];
+                float v[4];
+#pragma unroll
+                for (int s = 0; s < 4; ++s) {
+                    const int64_t c = c0 + 32 * s;
+                    const bool in = c < hi;
+                    v[s] = in ? to_float(*reinterpret_cast<const T *>(x + c)) : 0.0f;
+#pragma unroll
+                    for (int h = 0; h < 2; ++h)
+                        f[s][h] = load8(F + (in ? c : lo) * P.F.sc + jb + 8 * h,
+                                        in ? r - jb - 8 * h : 0);
+                }
+#pragma unroll
+                for (int s = 0; s < 4; ++s) {
+                    const int64_t c = c0 + 32 * s;
+                    if (kDrop && c < hi)
+                        if (!dropout_kept(dropout_bits(P.drop, key, row, static_cast<uint32_t>(c >> 3)),
+                                          static_cast<int>(c & 7), P.drop.cut))
+                            v[s] = 0.0f;
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        float w[8];
+                        unpack8<T>(f[s][h], w);
+                        // an element past the end is skipped, not multiplied by zero
+                        if (c < hi)
+#pragma unroll
+                            for (int j = 0; j < 8; ++j) acc[8 * h + j] += v[s] * w[j];
+                    }
+                }
+            }
+#pragma unroll
+            for (int j = 0; j < 16; ++j) {
+                const float v = warp_sum(acc[j]);
+                if (lane == 0 && jb + j < r) part[warp][jb + j] = v;
+            }
+        }
+        return;
+    }
+    for (int jb = 0; jb < r; jb += 2 * kRowWarps) {
+        const int j[2] = {jb + warp, jb + warp + kRowWarps};
+        float acc[2] = {0.0f, 0.0f};
+        for (int64_t c0 = begin + 8 * lane; c0 - 8 * lane < end; c0 += 1024) {
+            uint4 xv[4], f[2][4];
+#pragma unroll
+            for (int s = 0; s < 4; ++s) {
+                const int64_t c = c0 + 256 * s, n = end - c;
+                xv[s] = load8(x + c, n);
+#pragma unroll
+                for (int k = 0; k < 2; ++k) {
+                    if (P.mode == kFC) {
+                        f[k][s] = load8(F + j[k] * P.F.sr + c, j[k] < r ? n : 0);
+                    } else {
+                        uint32_t w[4] = {0, 0, 0, 0};
+#pragma unroll
+                        for (int e = 0; e < 8; ++e)
+                            if (j[k] < r && e < n)
+                                w[e >> 1] |= static_cast<uint32_t>(
+                                                 __ldg(F + (c + e) * P.F.sc + j[k] * P.F.sr))
+                                             << (16 * (e & 1));
+                        f[k][s] = make_uint4(w[0], w[1], w[2], w[3]);
+                    }
+                }
+            }
+#pragma unroll
+            for (int s = 0; s < 4; ++s) {
+                const int64_t c = c0 + 256 * s;
+                if (kDrop) xv[s] = masked(xv[s], P.drop, key, row, static_cast<uint32_t>(c >> 3));
+                float v[8], w[8];
+                unpack8<T>(xv[s], v);
+#pragma unroll
+                for (int k = 0; k < 2; ++k) {
+                    unpack8<T>(f[k][s], w);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) acc[k] += v[e] * w[e];
+                }
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            const float v = warp_sum(acc[k]);
+            if (j[k] < r && lane < kRowWarps) part[lane][j[k]] = lane == 0 ? v : 0.0f;
+        }
+    }
+}
+
+template <typename T, bool kDrop>
+__global__ void __launch_bounds__(kRowThreads, 3)
     project_rows_kernel(const __grid_constant__ ProjectParams P) {
-    constexpr int kWarps = kRowThreads / 32;
-    __shared__ float part[kWarps][kMaxRankRows];
+    __shared__ float part[kRowWarps][kMaxRankRows];
     __shared__ float sum[kMaxRankRows];
-    // the kernel that reads P may start its own copies now; it waits for this grid before P
+    // the kernel that reads P may start its own reads now; it waits for this grid before P
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t crank = cluster_rank(), csize = cluster_size();
@@ -250,16 +353,15 @@ __global__ void __launch_bounds__(kRowThreads)
     const int64_t begin = int64_t(crank) * P.slice, end = min(P.cols, begin + P.slice);
     const int r = static_cast<int>(P.r);
     if (i >= 0)
-        dot_slice<T, kDrop, kWarps>(
-            static_cast<const uint16_t *>(P.M) + t * P.ld,
-            static_cast<const uint16_t *>(P.F.p) + i * P.F.ss, P.F.sc, P.F.sr, P.mode, r, begin,
-            end, P.drop, kDrop ? dropout_key(P.drop) : 0, static_cast<uint32_t>(t), warp, lane,
-            &part[0][0], kMaxRankRows);
+        dot_slice<T, kDrop>(P, static_cast<const uint16_t *>(P.M) + t * P.ld,
+                            static_cast<const uint16_t *>(P.F.p) + i * P.F.ss, begin, end,
+                            kDrop ? dropout_key(P.drop) : 0, static_cast<uint32_t>(t), warp, lane,
+                            part);
     __syncthreads();
     for (int j = threadIdx.x; j < r; j += kRowThreads) {
         float v = 0.0f;
         if (i >= 0)
-            for (int w = 0; w < kWarps; ++w) v += part[w][j];
+            for (int w = 0; w < kRowWarps; ++w) v += part[w][j];
         sum[j] = v;
     }
     cluster_sync_all();
@@ -275,12 +377,14 @@ __global__ void __launch_bounds__(kRowThreads)
 template <typename K>
 cudaError_t launch_cluster(K kernel, int parts, dim3 grid, int threads, size_t smem,
                            const ProjectParams &P, cudaStream_t stream) {
-    if (smem > 48 * 1024) {
-        // a repeated setting is cheap and keeps no state per device
-        cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                             static_cast<int>(smem));
-        if (e != cudaSuccess) return e;
-    }
+    // (Repeated settings are cheap and keep no state per device.)  An SM whose shared memory is
+    // carved out small would have to drain before the expanding kernel's CTAs fit beside this one.
+    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout,
+                                         cudaSharedmemCarveoutMaxShared);
+    if (e == cudaSuccess && smem > 48 * 1024)
+        e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                 static_cast<int>(smem));
+    if (e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = grid;
     cfg.blockDim = dim3(threads);

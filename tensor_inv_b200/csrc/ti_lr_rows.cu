@@ -3,20 +3,20 @@
 // With few rows every element of W is read once and meets a handful of rows, so the kernel is a
 // stream of W: its columns stand on the 128-row side of the MMA (D[c][t] = sum_k W[k][c] M[t][k]),
 // the rows fill the narrow side (16 to 128 of them), and the inner dimension is split over a
-// cluster so that about every SM streams a share.  The partial tiles meet in distributed shared
-// memory: each CTA adds the cluster's parts of some rows, in rank order, and stores them.
+// cluster so that about every SM streams a share.  Rows are served by the cluster's CTAs in turn: a
+// CTA sends its part of a row into the serving CTA's shared memory, which adds the parts in rank
+// order and stores the row.
 //
 // The low-rank term is a few multiply-adds per output and runs on the plain cores while the copies
-// of W are in flight: each CTA of the cluster takes every C-th row, thread c holds column c, and
-// the row's P meets its adapter's F in float32.  It reads only the adapters that rows ask for, each
-// once per row, and nothing of one row's adapter can reach another row.
+// of W are in flight: thread c of the serving CTA holds column c, and the row's P meets its
+// adapter's F in float32.  It reads only the adapters that rows ask for, each once per row, and
+// nothing of one row's adapter can reach another row.
 //
-// For up to kFuseRows rows the projection is made here as well: each CTA of a cluster takes its
-// share of the inner dimension, and the one that serves a row adds the shares.  Every column tile
-// repeats that work, but for so few rows it is small against W and hides behind its copies, and
-// one launch is left of two.  Otherwise the projection runs before, and this kernel may start
-// before it has finished (programmatic launch): copies of M and W, which the projection only
-// reads, begin at once, and P is waited for where it is needed.
+// The kernel starts while the projection still runs (programmatic launch): W, M, the indices and F,
+// which the projection only reads or does not touch, are asked for at once, and P is waited for
+// where it is needed.  A stream of W fills the memory system's queues, and a read behind them
+// takes several microseconds; so all but the first copies wait until the first rows of F, the one
+// dependent chain of reads here, have been asked for.
 //
 // Roles: warp 0 copies, warp 1 TMEM and MMA issue, warps 2..9 low-rank term and epilogue (two
 // groups of 128 threads, one thread per column, that share the rows).
@@ -33,19 +33,22 @@ namespace {
 constexpr int kCols = 128, kBK = 64;
 constexpr int kLowWarps = 8, kLowThreads = 32 * kLowWarps;
 constexpr int kThreads = 64 + kLowThreads;
-constexpr int kMaxRank = 256;
 constexpr int kWBytes = kCols * kBK * 2;  // 16 KB
+constexpr int kEarly = 2;                 // copies that do not wait for the reads of F
+constexpr int kBatch = 4;                 // rows of a group whose reads of F overlap
 
-template <int kNT, bool kFused>
+template <int kNT>
 struct Shape {
     static constexpr int kMBytes = kNT * kBK * 2;
     static constexpr int kStageBytes = kWBytes + kMBytes;
-    static constexpr int kPartBytes = kNT * kCols * 4;
-    // the projection's sums by warp and in all, for the rows of the fused form
-    static constexpr int kFuseBytes = kFused ? kFuseRows * kMaxRank * 4 * (kLowWarps + 2) : 0;
-    static constexpr int kStages = kFused ? 8 : kNT <= 32 ? 9 : kNT == 64 ? 7 : 4;
-    static constexpr size_t kSmem = size_t(kStages) * kStageBytes + kPartBytes + kFuseBytes + 1024 +
-                                    512 + sizeof(int) * kNT;
+    // Parts: [sending CTA][rows served][128], for up to 8 CTAs.  The low-rank term is one more
+    // sender, so that nothing is read back to be added to; at 128 rows there is no room for that,
+    // and the serving CTA adds its own part to it.
+    static constexpr bool kLowApart = kNT < 128;
+    static constexpr int kPartBytes = (kLowApart ? 2 * kNT : kNT + 8) * kCols * 4;
+    static constexpr int kStages = kNT <= 32 ? 8 : kNT == 64 ? 6 : 4;
+    static constexpr size_t kSmem =
+        size_t(kStages) * kStageBytes + kPartBytes + 1024 + 256 + sizeof(int) * kNT;
     static constexpr uint32_t kTmemCols = kNT < 32 ? 32 : kNT;
 };
 
@@ -55,18 +58,10 @@ struct Params {
     int row_tiles;
     int w_nmajor;
     uint32_t idesc;
-    float *P;              // the projection; fused: written if not null
-    int64_t r;
+    const float *P;
+    int r;
     Factor16 F;
-    int fmode, pvec;       // F in vectors along the rank (kFR); P's rows in vectors of 4
-    // fused form: the projection's own operands
-    const void *M;
-    int64_t ldm, inner;
-    Factor16 G;
-    int gmode;
-    const float *scale;
-    float alpha;
-    Dropout gdrop;
+    int fvec, pvec;        // F in vectors of 8 along the rank; P's rows in vectors of 4
     RowIndex index;
     Dropout drop;
     void *out;
@@ -100,127 +95,125 @@ __device__ __forceinline__ void drain_wait(const Params &P, uint64_t *bar, uint3
     }
 }
 
+// Writes a float into the shared memory of CTA `rank`, at this CTA's address `p`.
+__device__ __forceinline__ void store_remote(float *p, uint32_t rank, float v) {
+    asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(map_to_rank(smem_u32(p), rank)), "f"(v));
+}
+
 __device__ __forceinline__ void low_sync() {
     asm volatile("bar.sync 1, %0;" ::"n"(kLowThreads) : "memory");
 }
 
-// sum_j p[u][j] F[i[u]][c][j] for up to four rows at once (their loads overlap); rows without an
-// adapter, or a column past the end, give 0.
+// 16 bytes, in program order with the barriers around it.
+__device__ __forceinline__ uint4 load_ordered(const void *p) {
+    uint4 v;
+    asm volatile("ld.global.nc.v4.u32 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+                 : "l"(p)
+                 : "memory");
+    return v;
+}
+
+// F[i][c][j0 .. j0+16) of kBatch rows' adapters, as 16-bit values; zeros where there are none.
 template <typename T>
-__device__ __forceinline__ void low_rank(const Params &P, const float *const (&p)[4],
-                                         const int (&i)[4], int64_t c, float (&acc)[4]) {
-    const T *f[4];
+__device__ __forceinline__ void load_factors(const Params &P, const int (&i)[kBatch], int64_t c,
+                                             int j0, uint4 (&f)[kBatch][2]) {
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
-        acc[u] = 0.0f;
-        f[u] = static_cast<const T *>(P.F.p) + max(i[u], 0) * P.F.ss + c * P.F.sc;
-    }
-    if (c >= P.cols) return;
-    const int r = static_cast<int>(P.r);
-#pragma unroll 2
-    for (int j0 = 0; j0 < r; j0 += 8) {
-        const bool whole = j0 + 8 <= r;
-        uint4 x[4];
-        float v[4][8], w[4][8];
+    for (int u = 0; u < kBatch; ++u) {
+        const uint16_t *src = static_cast<const uint16_t *>(P.F.p) + max(i[u], 0) * P.F.ss +
+                              c * P.F.sc + j0 * P.F.sr;
 #pragma unroll
-        for (int u = 0; u < 4; ++u) {
-            if (P.fmode == kFR) {
-                x[u] = make_uint4(0, 0, 0, 0);
-                if (i[u] >= 0)
-                    x[u] = load8(reinterpret_cast<const uint16_t *>(f[u] + j0), r - j0);
-            } else {
+        for (int h = 0; h < 2; ++h) {
+            const int n = i[u] >= 0 && c < P.cols ? P.r - j0 - 8 * h : 0;
+            f[u][h] = make_uint4(0, 0, 0, 0);
+            if (P.fvec && n >= 8) {
+                f[u][h] = load_ordered(src + 8 * h);
+            } else if (n > 0) {
+                uint32_t w[4] = {0, 0, 0, 0};
 #pragma unroll
                 for (int e = 0; e < 8; ++e)
-                    v[u][e] = i[u] >= 0 && j0 + e < r ? to_float(f[u][(j0 + e) * P.F.sr]) : 0.0f;
+                    if (e < n)
+                        w[e >> 1] |= static_cast<uint32_t>(__ldg(src + (8 * h + e) * P.F.sr))
+                                     << (16 * (e & 1));
+                f[u][h] = make_uint4(w[0], w[1], w[2], w[3]);
             }
-            if (P.pvec && whole) {
-                const float4 a = *reinterpret_cast<const float4 *>(p[u] + j0);
-                const float4 b = *reinterpret_cast<const float4 *>(p[u] + j0 + 4);
-                w[u][0] = a.x, w[u][1] = a.y, w[u][2] = a.z, w[u][3] = a.w;
-                w[u][4] = b.x, w[u][5] = b.y, w[u][6] = b.z, w[u][7] = b.w;
-            } else {
-#pragma unroll
-                for (int e = 0; e < 8; ++e) w[u][e] = j0 + e < r ? p[u][j0 + e] : 0.0f;
-            }
-        }
-#pragma unroll
-        for (int u = 0; u < 4; ++u) {
-            if (i[u] < 0) continue;
-            if (P.fmode == kFR) unpack8<T>(x[u], v[u]);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) acc[u] += w[u][e] * v[u][e];
         }
     }
 }
 
-template <typename T, int kNT, bool kDrop, bool kFused>
-__global__ void __launch_bounds__(kThreads, 1)
+// (Registers are held to what lets a CTA start beside two CTAs of the projection.)
+template <typename T, int kNT, bool kDrop>
+__global__ void __launch_bounds__(kThreads, 2)
     lr_rows_kernel(const __grid_constant__ CUtensorMap tmM, const __grid_constant__ CUtensorMap tmW,
                    const __grid_constant__ Params P) {
-    using S = Shape<kNT, kFused>;
+    using S = Shape<kNT>;
     extern __shared__ uint8_t smem_raw[];
     uint8_t *smem = reinterpret_cast<uint8_t *>(
         (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     uint8_t *sW = smem;
     uint8_t *sM = sW + S::kStages * kWBytes;
-    float *part = reinterpret_cast<float *>(sM + S::kStages * S::kMBytes);  // [kNT][128]
-    float *fuse = part + kNT * kCols;                // [kLowWarps][kFuseRows][kMaxRank]
-    float *slice_sum = fuse + kLowWarps * kFuseRows * kMaxRank;  // [kFuseRows][kMaxRank]
-    float *projection = slice_sum + kFuseRows * kMaxRank;        // [kFuseRows][kMaxRank]
-    uint64_t *full = reinterpret_cast<uint64_t *>(fuse + S::kFuseBytes / 4);
+    float *part = reinterpret_cast<float *>(sM + S::kStages * S::kMBytes);
+    uint64_t *full = reinterpret_cast<uint64_t *>(part + S::kPartBytes / 4);
     uint64_t *empty = full + S::kStages;
     uint64_t *tfull = empty + S::kStages;
     uint64_t *drain = tfull + 1;
-    uint64_t *sums = drain + 1;  // fused: every CTA's slice of the projection is in place
-    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(sums + 1);
+    uint64_t *asked = drain + 1;  // the first reads of F are on their way
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(asked + 1);
     volatile int *abort = reinterpret_cast<volatile int *>(tmem_slot + 1);
     int *sidx = const_cast<int *>(abort) + 1;  // [kNT] adapters of the tile's rows
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const uint32_t rank = cluster_rank(), csize = cluster_size();
+    const int rank = static_cast<int>(cluster_rank()), csize = static_cast<int>(cluster_size());
     const int64_t tile = blockIdx.x / csize;
     // neighbouring clusters share W's columns, so a second row tile finds them in L2
     const int64_t row0 = tile % P.row_tiles * kNT, col0 = tile / P.row_tiles * kCols;
-    const int kb0 = static_cast<int>(rank) * P.per_rank;
+    const int kb0 = rank * P.per_rank;
     const int steps = max(0, min(P.num_kb, kb0 + P.per_rank) - kb0);
+    const int here = static_cast<int>(min(int64_t(kNT), P.rows - row0));
+    // row t of the tile is the k-th that CTA t % csize serves, k = t / csize; there the parts lie
+    // [sending CTA][k][column]
+    const int part_rows = (kNT + csize - 1) / csize;
 
     if (threadIdx.x == 0) {
+        prefetch_tensormap(&tmW);
+        prefetch_tensormap(&tmM);
         for (int s = 0; s < S::kStages; ++s) {
             mbar_init(&full[s], 1);
             mbar_init(&empty[s], 1);
         }
         mbar_init(tfull, 1);
         mbar_init(drain, 1);
-        mbar_init(sums, csize);
+        mbar_init(asked, kLowWarps);
         *abort = 0;
         fence_barrier_init();
-        prefetch_tensormap(&tmM);
-        prefetch_tensormap(&tmW);
     }
+    // a row's adapter is asked for now and awaited behind the barrier
+    int adapter = -1;
+    if (warp >= 2 && static_cast<int>(threadIdx.x) - 64 < here)
+        adapter = P.index.at(row0 + threadIdx.x - 64);
     if (warp == 1) {
         tmem_alloc(tmem_slot, S::kTmemCols);
         tmem_relinquish();
     }
     tc_fence_before();
     __syncthreads();
-    if (kFused) cluster_sync_all();  // every `sums` is ready for the other CTAs' arrivals
     tc_fence_after();
     const uint32_t tmem_base = *tmem_slot;
+    cluster_arrive();  // awaited before anything is written to another CTA: it must have started
 
     if (warp == 0) {
         if (lane == 0) {
             // ---------------- copies ----------------
-            int stage = 0;
-            uint32_t phase = 0, issued_mask = 0, issued_phase = 0;
-            bool ok = true;
-            for (int k = 0; k < steps; ++k) {
-                if (!mbar_wait(&empty[stage], phase ^ 1, abort)) {
+            int stage = 0, issued = 0;
+            uint32_t phase = 0;
+            for (; issued < steps; ++issued) {
+                if ((issued == kEarly && !mbar_wait(asked, 0, abort)) ||
+                    !mbar_wait(&empty[stage], phase ^ 1, abort)) {
                     raise(P, abort, kErrTimeoutProducer);
-                    ok = false;
                     break;
                 }
                 mbar_arrive_expect_tx(&full[stage], S::kStageBytes);
-                const int k0 = (kb0 + k) * kBK;
+                const int k0 = (kb0 + issued) * kBK;
                 uint8_t *w = sW + stage * kWBytes;
                 if (P.w_nmajor) {
                     tma_load_2d(w, &tmW, &full[stage], static_cast<int>(col0), k0);
@@ -229,17 +222,17 @@ __global__ void __launch_bounds__(kThreads, 1)
                     tma_load_2d(w, &tmW, &full[stage], k0, static_cast<int>(col0));
                 }
                 tma_load_2d(sM + stage * S::kMBytes, &tmM, &full[stage], k0, static_cast<int>(row0));
-                issued_mask |= 1u << stage;
-                issued_phase = (issued_phase & ~(1u << stage)) | (phase << stage);
                 if (++stage == S::kStages) {
                     stage = 0;
                     phase ^= 1;
                 }
             }
-            if (!ok)
-                for (int s = 0; s < S::kStages; ++s)
-                    if ((issued_mask >> s) & 1) drain_wait(P, &full[s], (issued_phase >> s) & 1);
+            if (issued < steps)  // gave up: every copy lands before the CTA may exit
+                for (int k = max(0, issued - S::kStages); k < issued; ++k)
+                    drain_wait(P, &full[k % S::kStages], static_cast<uint32_t>(k / S::kStages) & 1);
         }
+        __syncwarp();
+        cluster_wait();
     } else if (warp == 1) {
         if (lane == 0) {
             // ---------------- MMA issuer ----------------
@@ -276,103 +269,87 @@ __global__ void __launch_bounds__(kThreads, 1)
                 drain_wait(P, drain, 0);
             }
         }
+        __syncwarp();
+        cluster_wait();
     } else {
         // ---------------- low-rank term, then this CTA's part of the tile ----------------
         const int q = warp & 3, lc = q * 32 + lane;  // TMEM lane = column of the tile
         const int group = (warp - 2) >> 2, lt = threadIdx.x - 64;
         const int64_t col = col0 + lc;
-        const int here = static_cast<int>(min(int64_t(kNT), P.rows - row0));
-        const int c4 = static_cast<int>(csize);
-        for (int t = lt; t < here; t += kLowThreads) sidx[t] = P.index.at(row0 + t);
-        for (int t = group; t < here; t += 2)
-            if (t % c4 != static_cast<int>(rank)) part[t * kCols + lc] = 0.0f;
-        low_sync();
-        // this group's rows: rank + c4 * (group + 2 * n); their adapters' factors come into L2
-        const int first = static_cast<int>(rank) + c4 * group;
-        if (P.fmode == kFR && col < P.cols)
-            for (int t = first; t < here; t += 2 * c4) {
-                const int i = sidx[t];
-                if (i < 0) continue;
-                const T *f = static_cast<const T *>(P.F.p) + i * P.F.ss + col * P.F.sc;
-                for (int j = 0; j < P.r; j += 16)
-                    asm volatile("prefetch.global.L2 [%0];" ::"l"(f + j));
-            }
-        if constexpr (kFused) {
-            const int64_t begin = int64_t(kb0) * kBK;
-            const int64_t end = min(P.inner, begin + int64_t(steps) * kBK);
-            const uint64_t gkey = P.gdrop.cut ? dropout_key(P.gdrop) : 0;
-            const int r = static_cast<int>(P.r);
-            for (int t = 0; t < here; ++t) {
-                const int i = sidx[t];
-                if (i < 0) continue;
-                const uint16_t *x = static_cast<const uint16_t *>(P.M) + (row0 + t) * P.ldm;
-                const uint16_t *g = static_cast<const uint16_t *>(P.G.p) + i * P.G.ss;
-                float *dst = fuse + t * kMaxRank;
-                if (P.gdrop.cut)
-                    dot_slice<T, true, kLowWarps>(x, g, P.G.sc, P.G.sr, P.gmode, r, begin, end,
-                                                  P.gdrop, gkey, static_cast<uint32_t>(row0 + t),
-                                                  warp - 2, lane, dst, kFuseRows * kMaxRank);
-                else
-                    dot_slice<T, false, kLowWarps>(x, g, P.G.sc, P.G.sr, P.gmode, r, begin, end,
-                                                   P.gdrop, 0, 0, warp - 2, lane, dst,
-                                                   kFuseRows * kMaxRank);
-            }
-            low_sync();
-            for (int e = lt; e < here * r; e += kLowThreads) {
-                const int t = e / r, j = e % r;
-                float v = 0.0f;
-                if (sidx[t] >= 0)
-                    for (int w = 0; w < kLowWarps; ++w)
-                        v += fuse[(w * kFuseRows + t) * kMaxRank + j];
-                slice_sum[t * kMaxRank + j] = v;
-            }
-            low_sync();
-            // tell every CTA of the cluster, then add the slices of the rows served here
-            if (lt < c4) mbar_arrive_remote(map_to_rank(smem_u32(sums), lt));
-            bool ok = mbar_wait_cluster(sums, 0, abort);
-            if (!ok) raise(P, abort, kErrTimeoutEpilogue);
-            for (int e = lt; ok && e < here * r; e += kLowThreads) {
-                const int t = e / r, j = e % r;
-                if (t % c4 != static_cast<int>(rank)) continue;
-                const int i = sidx[t];
-                float v = 0.0f;
-                if (i >= 0) {
-                    for (int k = 0; k < c4; ++k) v += load_remote(slice_sum + t * kMaxRank + j, k);
-                    v *= P.alpha * (P.scale ? P.scale[i] : 1.0f);
-                }
-                projection[t * kMaxRank + j] = v;
-                if (P.P && col0 == 0) P.P[(row0 + t) * P.r + j] = v;
-            }
-            low_sync();
-        } else {
-            asm volatile("griddepcontrol.wait;" ::: "memory");  // the projection is complete
-        }
+        float *send = part + rank * part_rows * kCols + lc;
+        float *low = S::kLowApart ? part + csize * part_rows * kCols + lc : send;
         const uint64_t key = kDrop ? dropout_key(P.drop) : 0;
-        for (int t0 = first; t0 < here; t0 += 8 * c4) {
-            const float *p[4];
-            int i[4];
-            float acc[4];
+        if (lt < kNT) sidx[lt] = adapter;
+        low_sync();
+        // the served rows k = group, group + 2, ..., kBatch of them at a time
+        bool waited = false;
+        for (int k0 = group; rank + csize * k0 < here || !waited; k0 += 2 * kBatch) {
+            int i[kBatch];
+            float acc[kBatch];
 #pragma unroll
-            for (int u = 0; u < 4; ++u) {
-                const int t = t0 + 2 * c4 * u;
+            for (int u = 0; u < kBatch; ++u) {
+                const int t = rank + csize * (k0 + 2 * u);
                 i[u] = t < here ? sidx[t] : -1;
-                const int tc = t < here ? t : t0;
-                p[u] = kFused ? projection + tc * kMaxRank : P.P + (row0 + tc) * P.r;
+                acc[u] = 0.0f;
             }
-            low_rank<T>(P, p, i, col, acc);
+#pragma unroll 1
+            for (int j0 = 0; j0 < P.r; j0 += 16) {
+                uint4 f[kBatch][2];
+                load_factors<T>(P, i, col, j0, f);
+                if (!waited) {
+                    waited = true;
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(asked);
+                    // the factors of later rows come as far as L2
+                    if (P.fvec && col < P.cols)
+                        for (int k = k0 + 2 * kBatch; rank + csize * k < here; k += 2) {
+                            const int later = sidx[rank + csize * k];
+                            if (later >= 0)
+                                asm volatile("prefetch.global.L2 [%0];" ::"l"(
+                                    static_cast<const uint16_t *>(P.F.p) + later * P.F.ss +
+                                    col * P.F.sc));
+                        }
+                    asm volatile("griddepcontrol.wait;" ::: "memory");  // the projection is complete
+                }
 #pragma unroll
-            for (int u = 0; u < 4; ++u) {
-                const int t = t0 + 2 * c4 * u;
+                for (int u = 0; u < kBatch; ++u) {
+                    if (i[u] < 0) continue;
+                    const float *p = P.P + (row0 + rank + csize * (k0 + 2 * u)) * P.r + j0;
+                    float v[16];
+                    unpack8<T>(f[u][0], *reinterpret_cast<float(*)[8]>(&v[0]));
+                    unpack8<T>(f[u][1], *reinterpret_cast<float(*)[8]>(&v[8]));
+#pragma unroll
+                    for (int e = 0; e < 16; e += 4) {
+                        if (P.pvec) {  // r is a multiple of 4
+                            if (j0 + e < P.r) {
+                                const float4 w = *reinterpret_cast<const float4 *>(p + e);
+                                acc[u] += w.x * v[e];
+                                acc[u] += w.y * v[e + 1];
+                                acc[u] += w.z * v[e + 2];
+                                acc[u] += w.w * v[e + 3];
+                            }
+                        } else {
+#pragma unroll
+                            for (int d = 0; d < 4; ++d)
+                                if (j0 + e + d < P.r) acc[u] += p[e + d] * v[e + d];
+                        }
+                    }
+                }
+            }
+#pragma unroll
+            for (int u = 0; u < kBatch; ++u) {
+                const int t = rank + csize * (k0 + 2 * u);
                 if (t >= here) break;
                 if (kDrop && i[u] >= 0) {
                     const uint4 bits = dropout_bits(P.drop, key, static_cast<uint32_t>(row0 + t),
                                                     static_cast<uint32_t>(col >> 3));
                     if (!dropout_kept(bits, static_cast<int>(col & 7), P.drop.cut)) acc[u] = 0.0f;
                 }
-                part[t * kCols + lc] = acc[u];
+                low[(k0 + 2 * u) * kCols] = acc[u];
             }
         }
-        low_sync();  // the low-rank parts of both groups are in place
+        cluster_wait();
+        if (!S::kLowApart) low_sync();  // both groups' low-rank terms are in place
         bool ok = true;
         if (!mbar_wait(tfull, 0, abort)) {
             raise(P, abort, kErrTimeoutEpilogue);
@@ -380,15 +357,28 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         __syncwarp();
         tc_fence_after();
-        if (__all_sync(0xFFFFFFFFu, ok) && steps > 0) {
+        if (__all_sync(0xFFFFFFFFu, ok)) {
             const uint32_t tbase = tmem_base + (static_cast<uint32_t>(q * 32) << 16);
             for (int c = 32 * group; c < here; c += 64) {  // the groups take 32 rows in turn
                 uint32_t v[32];
                 tmem_ld_32x32b_x32(tbase + c, v);
                 tmem_wait_ld();
+                int to = c % csize, k = c / csize;  // row c + e: served by CTA `to`, its k-th
 #pragma unroll
-                for (int e = 0; e < 32; ++e)
-                    if (c + e < here) part[(c + e) * kCols + lc] += __uint_as_float(v[e]);
+                for (int e = 0; e < 32; ++e) {
+                    // a CTA without steps has nothing in TMEM
+                    const float x = steps > 0 ? __uint_as_float(v[e]) : 0.0f;
+                    if (c + e < here) {
+                        if (to == rank)
+                            send[k * kCols] = S::kLowApart ? x : send[k * kCols] + x;
+                        else
+                            store_remote(send + k * kCols, to, x);
+                    }
+                    if (++to == csize) {
+                        to = 0;
+                        ++k;
+                    }
+                }
             }
         }
     }
@@ -398,27 +388,29 @@ __global__ void __launch_bounds__(kThreads, 1)
         tc_fence_after();
         tmem_dealloc(tmem_base, S::kTmemCols);
     }
-    cluster_sync_all();  // every CTA's part is written
+    cluster_sync_all();  // every part has arrived; no remote access follows
     if (warp >= 2) {
         const int lc = (threadIdx.x - 64) % kCols, group = (threadIdx.x - 64) / kCols;
         const int64_t col = col0 + lc;
-        const int here = static_cast<int>(min(int64_t(kNT), P.rows - row0));
         T *out = static_cast<T *>(P.out);
         if (col < P.cols)
-            for (int t = static_cast<int>(rank + csize * group); t < here; t += 2 * csize) {
+#pragma unroll 4
+            for (int k = group; rank + csize * k < here; k += 2) {
+                const float *src = part + k * kCols + lc;
                 float v = 0.0f;
-                for (uint32_t k = 0; k < csize; ++k) v += load_remote(part + t * kCols + lc, k);
-                out[(row0 + t) * P.ldo + col] = from_float<T>(v);
+#pragma unroll
+                for (int c = 0; c < 9; ++c)
+                    if (c < csize + S::kLowApart) v += src[c * part_rows * kCols];
+                out[(row0 + rank + csize * k) * P.ldo + col] = from_float<T>(v);
             }
     }
-    cluster_sync_all();  // nobody leaves while its part is being read
 }
 
-template <typename T, int kNT, bool kDrop, bool kFused>
+template <typename T, int kNT, bool kDrop>
 cudaError_t launch(const CUtensorMap &tmM, const CUtensorMap &tmW, const Params &P, int64_t tiles,
                    int ranks, cudaStream_t stream) {
-    using S = Shape<kNT, kFused>;
-    auto kernel = lr_rows_kernel<T, kNT, kDrop, kFused>;
+    using S = Shape<kNT>;
+    auto kernel = lr_rows_kernel<T, kNT, kDrop>;
     constexpr int kMaxDev = 64;
     static std::atomic<int> configured[kMaxDev];
     int dev = 0;
@@ -444,13 +436,12 @@ cudaError_t launch(const CUtensorMap &tmM, const CUtensorMap &tmW, const Params 
     attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = kFused ? 1 : 2;  // the fused form reads what earlier work wrote at once
+    cfg.numAttrs = 2;
     return cudaLaunchKernelEx(&cfg, kernel, tmM, tmW, P);
 }
 
 template <typename T, int kNT>
-cudaError_t expand(const ExpandOperands &o, const ProjectOperands *fuse, int num_sms, int *err,
-                   cudaStream_t stream) {
+cudaError_t expand(const ExpandOperands &o, int num_sms, int *err, cudaStream_t stream) {
     Params P;
     std::memset(&P, 0, sizeof(P));
     P.rows = o.rows;
@@ -468,9 +459,9 @@ cudaError_t expand(const ExpandOperands &o, const ProjectOperands *fuse, int num
               (P.w_nmajor ? 1u << 15 : 0u) | (static_cast<uint32_t>(kNT >> 3) << 17) |
               (static_cast<uint32_t>(kCols >> 4) << 24);
     P.P = o.P;
-    P.r = o.r;
+    P.r = static_cast<int>(o.r);
     P.F = o.F;
-    P.fmode = factor_mode(o.F) == kFR ? kFR : kFScalar;
+    P.fvec = factor_mode(o.F) == kFR;
     P.pvec = o.r % 4 == 0 && (reinterpret_cast<uintptr_t>(o.P) & 15) == 0;
     P.index = o.index;
     P.drop = o.drop;
@@ -482,38 +473,24 @@ cudaError_t expand(const ExpandOperands &o, const ProjectOperands *fuse, int num
     if (P.w_nmajor ? !make_map16(&tmW, o.W.p, o.cols, o.inner, o.W.s0, 64, kBK)
                    : !make_map16(&tmW, o.W.p, o.inner, o.cols, o.W.s1, kBK, kCols))
         return cudaErrorInvalidValue;
-    if constexpr (kNT == 16)
-        if (fuse) {
-            P.M = o.M.p;
-            P.ldm = o.M.s0;
-            P.inner = o.inner;
-            P.G = fuse->F;
-            P.gmode = factor_mode(fuse->F);
-            P.scale = fuse->scale;
-            P.alpha = fuse->alpha;
-            P.gdrop = fuse->drop;
-            return o.drop.cut ? launch<T, kNT, true, true>(tmM, tmW, P, tiles, ranks, stream)
-                              : launch<T, kNT, false, true>(tmM, tmW, P, tiles, ranks, stream);
-        }
-    return o.drop.cut ? launch<T, kNT, true, false>(tmM, tmW, P, tiles, ranks, stream)
-                      : launch<T, kNT, false, false>(tmM, tmW, P, tiles, ranks, stream);
+    return o.drop.cut ? launch<T, kNT, true>(tmM, tmW, P, tiles, ranks, stream)
+                      : launch<T, kNT, false>(tmM, tmW, P, tiles, ranks, stream);
 }
 
 template <typename T>
-cudaError_t by_rows(const ExpandOperands &o, const ProjectOperands *fuse, int num_sms, int *err,
-                    cudaStream_t stream) {
-    return o.rows <= 16   ? expand<T, 16>(o, fuse, num_sms, err, stream)
-           : o.rows <= 32 ? expand<T, 32>(o, fuse, num_sms, err, stream)
-           : o.rows <= 64 ? expand<T, 64>(o, fuse, num_sms, err, stream)
-                          : expand<T, 128>(o, fuse, num_sms, err, stream);
+cudaError_t by_rows(const ExpandOperands &o, int num_sms, int *err, cudaStream_t stream) {
+    return o.rows <= 16   ? expand<T, 16>(o, num_sms, err, stream)
+           : o.rows <= 32 ? expand<T, 32>(o, num_sms, err, stream)
+           : o.rows <= 64 ? expand<T, 64>(o, num_sms, err, stream)
+                          : expand<T, 128>(o, num_sms, err, stream);
 }
 
 }  // namespace
 
-cudaError_t lr_expand_rows(bool half, const ExpandOperands &o, const ProjectOperands *fuse,
-                           int num_sms, int *err, cudaStream_t stream) {
-    return half ? by_rows<__half>(o, fuse, num_sms, err, stream)
-                : by_rows<__nv_bfloat16>(o, fuse, num_sms, err, stream);
+cudaError_t lr_expand_rows(bool half, const ExpandOperands &o, int num_sms, int *err,
+                           cudaStream_t stream) {
+    return half ? by_rows<__half>(o, num_sms, err, stream)
+                : by_rows<__nv_bfloat16>(o, num_sms, err, stream);
 }
 
 }  // namespace ti
