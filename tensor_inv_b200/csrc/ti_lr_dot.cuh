@@ -63,14 +63,9 @@ __device__ __forceinline__ float warp_sum(float v) {
     return v;
 }
 
-// A float in the shared memory of CTA `rank` of the cluster, at this CTA's address `p`.
-__device__ __forceinline__ float load_remote(const float *p, uint32_t rank) {
-    float v;
-    asm volatile("ld.shared::cluster.f32 %0, [%1];"
-                 : "=f"(v)
-                 : "r"(map_to_rank(smem_u32(p), rank))
-                 : "memory");
-    return v;
+// Writes a float into the shared memory of CTA `rank`, at this CTA's address `p`.
+__device__ __forceinline__ void store_remote(float *p, uint32_t rank, float v) {
+    asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(map_to_rank(smem_u32(p), rank)), "f"(v));
 }
 
 __device__ __forceinline__ uint32_t cluster_size() {

@@ -7,9 +7,10 @@
 // enough -- what counts is that M goes from memory to registers once, with the mask applied on the
 // way, and never through shared memory.  Two kernels:
 //   tiles: 128 rows x a slice of the inner dimension per CTA; a cluster of up to 8 CTAs shares the
-//          rows and adds its slices through distributed shared memory.  A tile walks the distinct
-//          adapters of its rows (one, for the runs of rows that prompts and training steps have)
-//          and every row keeps the result of its own.
+//          rows and adds its slices through distributed shared memory.  Every warp walks the distinct
+//          adapters of its own 32 rows (one, for the runs of rows that prompts and training steps
+//          have), reads their factor in fragment order straight from the caches and waits for
+//          nobody; a row keeps the result of its own adapter.
 //   rows:  one row per cluster, plain multiply-adds: for few rows each with an adapter of its own
 //          F's bytes bound it, and no product is shared between rows.
 #include "ti_lr_dot.cuh"
@@ -56,98 +57,121 @@ __device__ __forceinline__ void mma16816<__half>(float (&d)[4], uint32_t a0, uin
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
+__device__ __forceinline__ void store_cluster(uint32_t addr, float v) {
+    asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(addr), "f"(v));
+}
+
 constexpr int kTileRows = 128, kTileThreads = 256, kGroups = 2;  // two groups share the slice
-constexpr int kChunk = 64;             // inner elements per group and step
-constexpr int kFStride = kChunk + 32;  // F's rows in shared memory: 16-byte reads hit all banks
+constexpr int kChunk = 64;  // inner elements per warp and step
 
 template <int kNT>
 constexpr size_t tile_smem() {
-    return sizeof(uint16_t) * kGroups * 8 * kNT * kFStride + sizeof(float) * kTileRows * 8 * kNT;
+    return sizeof(float) * kGroups * kTileRows * 8 * kNT;
 }
 
-// Copies F[cur][c0 .. c0+64)[j0 .. j0+8*kNT) to shared memory as rows of one j (128 threads).
+// kNT 16-bit elements in one load (kNT = 1, 2 or 4).
 template <int kNT>
-__device__ __forceinline__ void stage_factor(const ProjectParams &P, int cur, int64_t c0,
-                                             int64_t end, int64_t j0, uint16_t *dst, int gt) {
-    const uint16_t *F = static_cast<const uint16_t *>(P.F.p) + cur * P.F.ss;
-    if (P.mode == kFC) {
-        for (int v = gt; v < 8 * kNT * (kChunk / 8); v += 128) {
-            const int j = v / (kChunk / 8), c = v % (kChunk / 8) * 8;
-            uint4 x = make_uint4(0, 0, 0, 0);
-            if (j0 + j < P.r) x = load8(F + (j0 + j) * P.F.sr + c0 + c, end - (c0 + c));
-            *reinterpret_cast<uint4 *>(dst + j * kFStride + c) = x;
-        }
-    } else if (P.mode == kFR) {
-        for (int v = gt; v < kNT * kChunk; v += 128) {
-            const int c = v / kNT, j = v % kNT * 8;
-            uint4 x = make_uint4(0, 0, 0, 0);
-            if (c0 + c < end) x = load8(F + (c0 + c) * P.F.sc + j0 + j, P.r - (j0 + j));
-            const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+__device__ __forceinline__ uint2 load_few(const uint16_t *p) {
+    if constexpr (kNT == 4) return __ldg(reinterpret_cast<const uint2 *>(p));
+    if constexpr (kNT == 2) return make_uint2(__ldg(reinterpret_cast<const uint32_t *>(p)), 0);
+    return make_uint2(__ldg(p), 0);
+}
+
+// F's fragments for 32 inner elements: f[n] holds, for column tile n, the thread's elements
+// c .. c + 7 of its column, in pairs.  Where F's vectors run along the rank (kFR), a thread reads
+// kNT consecutive ranks of each element, so the columns of the tiles interleave: column `g` of
+// tile n is rank kNT * g + n, else 8 * n + g.  kWhole: no element lies past the end (c + 8 <= end;
+// for kFR, r is a multiple of kNT); the general form handles every edge and every stride.
+template <int kNT, int kMode, bool kWhole>
+__device__ __forceinline__ void load_fragments(const ProjectParams &P, const uint16_t *F, int64_t c,
+                                               int64_t end, int64_t j0, int g, uint4 (&f)[kNT]) {
+    const int r = static_cast<int>(P.r);
+    if constexpr (kMode == kFR) {
+        const int j = static_cast<int>(j0) + kNT * g;
+        uint2 v[8];
 #pragma unroll
-            for (int e = 0; e < 8; ++e)
-                dst[(j + e) * kFStride + c] = static_cast<uint16_t>(w[e >> 1] >> (16 * (e & 1)));
+        for (int e = 0; e < 8; ++e) {
+            v[e] = make_uint2(0, 0);
+            const uint16_t *src = F + (c + e) * P.F.sc + j;
+            if (kWhole) {
+                if (j < r) v[e] = load_few<kNT>(src);
+            } else if (c + e < end) {
+#pragma unroll
+                for (int n = 0; n < kNT; ++n)
+                    if (j + n < r)
+                        (n < 2 ? v[e].x : v[e].y) |= static_cast<uint32_t>(__ldg(src + n))
+                                                     << (16 * (n & 1));
+            }
+        }
+#pragma unroll
+        for (int n = 0; n < kNT; ++n) {
+            const uint32_t sel = n & 1 ? 0x7632u : 0x5410u;  // upper or lower halves of two words
+            auto word = [&](int e) { return n < 2 ? v[e].x : v[e].y; };
+            f[n] = make_uint4(__byte_perm(word(0), word(1), sel), __byte_perm(word(2), word(3), sel),
+                              __byte_perm(word(4), word(5), sel), __byte_perm(word(6), word(7), sel));
         }
     } else {
-        for (int v = gt; v < 8 * kNT * kChunk; v += 128) {
-            const int j = v / kChunk, c = v % kChunk;
-            dst[j * kFStride + c] = j0 + j < P.r && c0 + c < end
-                                        ? F[(c0 + c) * P.F.sc + (j0 + j) * P.F.sr]
-                                        : static_cast<uint16_t>(0);
+#pragma unroll
+        for (int n = 0; n < kNT; ++n) {
+            const int j = static_cast<int>(j0) + 8 * n + g;
+            f[n] = make_uint4(0, 0, 0, 0);
+            if (kWhole) {
+                if (j < r) f[n] = __ldg(reinterpret_cast<const uint4 *>(F + j * P.F.sr + c));
+            } else if (j < r) {
+                uint32_t w[4] = {0, 0, 0, 0};
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                    if (c + e < end)
+                        w[e >> 1] |= static_cast<uint32_t>(__ldg(F + (c + e) * P.F.sc + j * P.F.sr))
+                                     << (16 * (e & 1));
+                f[n] = make_uint4(w[0], w[1], w[2], w[3]);
+            }
         }
     }
 }
 
-template <typename T, int kNT, bool kDrop>
+template <typename T, int kNT, bool kDrop, int kMode>
 __global__ void __launch_bounds__(kTileThreads, 2)
     project_tiles_kernel(const __grid_constant__ ProjectParams P) {
     extern __shared__ __align__(16) uint8_t smem[];
-    float *sum = reinterpret_cast<float *>(smem);                          // [128][8*kNT]
-    uint16_t *sF = reinterpret_cast<uint16_t *>(sum + kTileRows * 8 * kNT);  // [2][8*kNT][stride]
-    __shared__ unsigned least[2][8];
+    // what this CTA finishes: [sending CTA and group][row of its share][8*kNT]
+    float *sum = reinterpret_cast<float *>(smem);
     __shared__ int sidx[kTileRows];
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    cluster_arrive();  // awaited before anything is written to another CTA: it must have started
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int g = lane >> 2, tq = lane & 3;
-    const int group = warp >> 2, gt = threadIdx.x & 127;
+    const int group = warp >> 2;
     const uint32_t crank = cluster_rank(), csize = cluster_size();
+    const int share = kTileRows / static_cast<int>(csize);  // rows that each CTA finishes
     const int64_t row0 = int64_t(blockIdx.x / csize) * kTileRows;
     const int64_t j0 = int64_t(blockIdx.y) * 8 * kNT;
     const int64_t begin = int64_t(crank) * P.slice;
     const int64_t end = min(P.cols, begin + P.slice);
     const uint64_t key = kDrop ? dropout_key(P.drop) : 0;
 
-    if (threadIdx.x < kTileRows) {
-        const int64_t t = row0 + threadIdx.x;
-        sidx[threadIdx.x] = t < P.rows ? P.index.at(t) : -1;
-    }
-    for (int e = threadIdx.x; e < kTileRows * 8 * kNT; e += kTileThreads) sum[e] = 0.0f;
-    __syncthreads();
-
     const int wrow = (warp & 3) * 32;  // this warp's 32 rows; the thread's are wrow + g + 8*i
+    const int64_t mine = row0 + wrow + lane;
+    const int my = mine < P.rows ? P.index.at(mine) : -1;
+    if (group == 0) sidx[wrow + lane] = my;
     int idx[4];
     const uint16_t *M[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        idx[i] = sidx[wrow + g + 8 * i];
+        idx[i] = __shfl_sync(0xFFFFFFFFu, my, g + 8 * i);
         M[i] = static_cast<const uint16_t *>(P.M) + (row0 + wrow + g + 8 * i) * P.ld;
     }
-    const int my = sidx[threadIdx.x & 127];
-    int cur = -1, turn = 0;
+    // F's vectors can be read whole (a factor in neither vector order runs as kFC, by elements)
+    const bool vectors = P.mode == kMode && (kMode == kFC || P.r % kNT == 0);
+    int cur = -1;
+    bool started = false;
     while (true) {
-        // the next adapter in increasing order
-        const unsigned cand = my > cur ? static_cast<unsigned>(my) : 0x7FFFFFFFu;
-        const unsigned m = __reduce_min_sync(0xFFFFFFFFu, cand);
-        if (lane == 0) least[turn][warp] = m;
-        __syncthreads();
-        unsigned next = least[turn][0];
-#pragma unroll
-        for (int w = 1; w < 4; ++w) next = min(next, least[turn][w]);
-        turn ^= 1;
+        // the next adapter of the warp's rows in increasing order
+        const unsigned next = __reduce_min_sync(
+            0xFFFFFFFFu, my > cur ? static_cast<unsigned>(my) : 0x7FFFFFFFu);
         if (next == 0x7FFFFFFFu) break;
         cur = static_cast<int>(next);
-        const bool any = __any_sync(0xFFFFFFFFu, idx[0] == cur || idx[1] == cur || idx[2] == cur ||
-                                                     idx[3] == cur);
+        const uint16_t *F = static_cast<const uint16_t *>(P.F.p) + cur * P.F.ss;
         float acc[2][kNT][4];
 #pragma unroll
         for (int i = 0; i < 2; ++i)
@@ -156,23 +180,23 @@ __global__ void __launch_bounds__(kTileThreads, 2)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) acc[i][n][e] = 0.0f;
 
-        uint16_t *dst = sF + group * 8 * kNT * kFStride;
-        for (int64_t c0 = begin; c0 < end; c0 += kGroups * kChunk) {
-            const int64_t cg = c0 + group * kChunk;  // the same trip count for both groups
-            uint4 x[kChunk / 32][4];
-            if (any) {
+        auto step = [&](int64_t c0, auto whole) {
+            constexpr bool kWhole = decltype(whole)::value;
+            uint4 x[kChunk / 32][4], f[kChunk / 32][kNT];
 #pragma unroll
-                for (int s = 0; s < kChunk / 32; ++s)
+            for (int s = 0; s < kChunk / 32; ++s) {
+                const int64_t c = c0 + 32 * s + 8 * tq;
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const int64_t c = cg + 32 * s + 8 * tq;
-                        x[s][i] = idx[i] == cur ? load8(M[i] + c, end - c) : make_uint4(0, 0, 0, 0);
-                    }
+                for (int i = 0; i < 4; ++i) {
+                    x[s][i] = make_uint4(0, 0, 0, 0);
+                    if (idx[i] == cur)
+                        x[s][i] = kWhole ? __ldg(reinterpret_cast<const uint4 *>(M[i] + c))
+                                         : load8(M[i] + c, end - c);
+                }
             }
-            __syncthreads();  // the previous step's F has been read
-            stage_factor<kNT>(P, cur, cg, end, j0, dst, gt);
-            __syncthreads();
-            if (!any) continue;
+#pragma unroll
+            for (int s = 0; s < kChunk / 32; ++s)
+                load_fragments<kNT, kMode, kWhole>(P, F, c0 + 32 * s + 8 * tq, end, j0, g, f[s]);
 #pragma unroll
             for (int s = 0; s < kChunk / 32; ++s) {
                 if (kDrop) {
@@ -180,53 +204,65 @@ __global__ void __launch_bounds__(kTileThreads, 2)
                     for (int i = 0; i < 4; ++i)
                         x[s][i] = masked(x[s][i], P.drop, key,
                                          static_cast<uint32_t>(row0 + wrow + g + 8 * i),
-                                         static_cast<uint32_t>((cg + 32 * s + 8 * tq) >> 3));
+                                         static_cast<uint32_t>((c0 + 32 * s + 8 * tq) >> 3));
                 }
 #pragma unroll
                 for (int n = 0; n < kNT; ++n) {
-                    const uint4 f = *reinterpret_cast<const uint4 *>(
-                        dst + (8 * n + g) * kFStride + 32 * s + 8 * tq);
                     // the order of the inner dimension is free: a thread's 8 consecutive
                     // elements fill the slots of two k16 steps, in M and F alike
 #pragma unroll
                     for (int i = 0; i < 2; ++i) {
                         const uint4 &a = x[s][2 * i], &b = x[s][2 * i + 1];
-                        mma16816<T>(acc[i][n], a.x, b.x, a.y, b.y, f.x, f.y);
-                        mma16816<T>(acc[i][n], a.z, b.z, a.w, b.w, f.z, f.w);
+                        mma16816<T>(acc[i][n], a.x, b.x, a.y, b.y, f[s][n].x, f[s][n].y);
+                        mma16816<T>(acc[i][n], a.z, b.z, a.w, b.w, f[s][n].z, f[s][n].w);
                     }
                 }
             }
+        };
+        int64_t c0 = begin + group * kChunk;
+        if (vectors)
+#pragma unroll 1
+            for (; c0 + kChunk <= end; c0 += kGroups * kChunk) step(c0, std::true_type{});
+#pragma unroll 1
+        for (; c0 < end; c0 += kGroups * kChunk) step(c0, std::false_type{});
+        // rows of this adapter keep its sums
+        if (!started) {
+            started = true;
+            cluster_wait();
         }
-        // rows of this adapter keep its sums: first one group's, then the other adds its own
-        for (int turn_g = 0; turn_g < kGroups; ++turn_g) {
-            __syncthreads();
-            if (group == turn_g && any) {
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    if (idx[i] == cur) {
-                        float *dst_row = sum + (wrow + g + 8 * i) * 8 * kNT + 2 * tq;
+        for (int i = 0; i < 4; ++i)
+            if (idx[i] == cur) {
+                const int lr = wrow + g + 8 * i;
+                float *dst = sum + ((crank * kGroups + group) * share + lr % share) * 8 * kNT;
+                const uint32_t to = map_to_rank(smem_u32(dst), lr / share);
 #pragma unroll
-                        for (int n = 0; n < kNT; ++n) {
-                            dst_row[8 * n] += acc[i >> 1][n][2 * (i & 1)];
-                            dst_row[8 * n + 1] += acc[i >> 1][n][2 * (i & 1) + 1];
-                        }
+                for (int n = 0; n < kNT; ++n)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        const int col = 2 * tq + e;
+                        store_cluster(to + 4 * (kMode == kFR ? kNT * col + n : 8 * n + col),
+                                      acc[i >> 1][n][2 * (i & 1) + e]);
                     }
             }
-        }
     }
-    // the cluster's slices, added in rank order; each CTA finishes a share of the rows
-    cluster_sync_all();
-    const int share = kTileRows / static_cast<int>(csize);
+    if (!started) cluster_wait();
+    // the kernel that reads P may prepare itself now; it waits for this grid before P
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    cluster_sync_all();  // every sum has arrived; no remote access follows
+    // the cluster's slices, added in order
     for (int e = threadIdx.x; e < share * 8 * kNT; e += kTileThreads) {
         const int lr = static_cast<int>(crank) * share + e / (8 * kNT), j = e % (8 * kNT);
         const int64_t t = row0 + lr;
         if (t >= P.rows || j0 + j >= P.r) continue;
-        float v = 0.0f;
-        for (uint32_t q = 0; q < csize; ++q) v += load_remote(sum + lr * 8 * kNT + j, q);
         const int i = sidx[lr];
-        P.P[t * P.r + j0 + j] = i < 0 ? 0.0f : v * (P.alpha * (P.scale ? P.scale[i] : 1.0f));
+        float v = 0.0f;
+        if (i >= 0) {
+            for (uint32_t q = 0; q < kGroups * csize; ++q) v += sum[q * share * 8 * kNT + e];
+            v *= P.alpha * (P.scale ? P.scale[i] : 1.0f);
+        }
+        P.P[t * P.r + j0 + j] = v;
     }
-    cluster_sync_all();  // nobody leaves while its sums are being read
 }
 
 // ---------------------------------------------------------------------------------------
@@ -343,7 +379,8 @@ template <typename T, bool kDrop>
 __global__ void __launch_bounds__(kRowThreads, 3)
     project_rows_kernel(const __grid_constant__ ProjectParams P) {
     __shared__ float part[kRowWarps][kMaxRankRows];
-    __shared__ float sum[kMaxRankRows];
+    __shared__ float sum[8][kMaxRankRows];  // in CTA 0: every CTA's slice
+    cluster_arrive();  // awaited before anything is written to another CTA: it must have started
     // the kernel that reads P may start its own reads now; it waits for this grid before P
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -357,21 +394,21 @@ __global__ void __launch_bounds__(kRowThreads, 3)
                             static_cast<const uint16_t *>(P.F.p) + i * P.F.ss, begin, end,
                             kDrop ? dropout_key(P.drop) : 0, static_cast<uint32_t>(t), warp, lane,
                             part);
+    cluster_wait();
     __syncthreads();
     for (int j = threadIdx.x; j < r; j += kRowThreads) {
         float v = 0.0f;
         if (i >= 0)
             for (int w = 0; w < kRowWarps; ++w) v += part[w][j];
-        sum[j] = v;
+        store_remote(&sum[crank][j], 0, v);
     }
     cluster_sync_all();
     if (crank == 0)
         for (int j = threadIdx.x; j < r; j += kRowThreads) {
             float v = 0.0f;
-            for (uint32_t q = 0; q < csize; ++q) v += load_remote(sum + j, q);
+            for (uint32_t q = 0; q < csize; ++q) v += sum[q][j];
             P.P[t * P.r + j] = i < 0 ? 0.0f : v * (P.alpha * (P.scale ? P.scale[i] : 1.0f));
         }
-    cluster_sync_all();
 }
 
 template <typename K>
@@ -402,12 +439,16 @@ cudaError_t launch_cluster(K kernel, int parts, dim3 grid, int threads, size_t s
 
 template <typename T, int kNT>
 cudaError_t tiles(const ProjectParams &P, int parts, dim3 grid, cudaStream_t stream) {
-    if constexpr (kNT < 8)
-        if (P.drop.cut)
-            return launch_cluster(project_tiles_kernel<T, kNT, true>, parts, grid, kTileThreads,
-                                  tile_smem<kNT>(), P, stream);
-    return launch_cluster(project_tiles_kernel<T, kNT, false>, parts, grid, kTileThreads,
-                          tile_smem<kNT>(), P, stream);
+    const size_t smem = tile_smem<kNT>();
+    if (P.mode == kFR)
+        return P.drop.cut ? launch_cluster(project_tiles_kernel<T, kNT, true, kFR>, parts, grid,
+                                           kTileThreads, smem, P, stream)
+                          : launch_cluster(project_tiles_kernel<T, kNT, false, kFR>, parts, grid,
+                                           kTileThreads, smem, P, stream);
+    return P.drop.cut ? launch_cluster(project_tiles_kernel<T, kNT, true, kFC>, parts, grid,
+                                       kTileThreads, smem, P, stream)
+                      : launch_cluster(project_tiles_kernel<T, kNT, false, kFC>, parts, grid,
+                                       kTileThreads, smem, P, stream);
 }
 
 template <typename T>
@@ -424,8 +465,8 @@ cudaError_t project(ProjectParams P, int num_sms, cudaStream_t stream) {
                                            0, P, stream);
     }
     const int64_t tile_count = (P.rows + kTileRows - 1) / kTileRows;
-    // (with a mask the widest block would spill registers)
-    const int nt = P.r <= 8 ? 1 : P.r <= 16 ? 2 : P.r <= 32 || P.drop.cut ? 4 : 8;
+    // 8, 16 or 32 ranks per CTA; more of them read M again, from L2
+    const int nt = P.r <= 8 ? 1 : P.r <= 16 ? 2 : 4;
     const int64_t blocks = (P.r + 8 * nt - 1) / (8 * nt);
     // 1, 2, 4 or 8 CTAs share a tile's inner dimension, until two per SM have work
     constexpr int kStep = kGroups * kChunk;
@@ -436,8 +477,7 @@ cudaError_t project(ProjectParams P, int num_sms, cudaStream_t stream) {
     switch (nt) {
         case 1: return tiles<T, 1>(P, parts, grid, stream);
         case 2: return tiles<T, 2>(P, parts, grid, stream);
-        case 4: return tiles<T, 4>(P, parts, grid, stream);
-        default: return tiles<T, 8>(P, parts, grid, stream);
+        default: return tiles<T, 4>(P, parts, grid, stream);
     }
 }
 

@@ -95,11 +95,6 @@ __device__ __forceinline__ void drain_wait(const Params &P, uint64_t *bar, uint3
     }
 }
 
-// Writes a float into the shared memory of CTA `rank`, at this CTA's address `p`.
-__device__ __forceinline__ void store_remote(float *p, uint32_t rank, float v) {
-    asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(map_to_rank(smem_u32(p), rank)), "f"(v));
-}
-
 __device__ __forceinline__ void low_sync() {
     asm volatile("bar.sync 1, %0;" ::"n"(kLowThreads) : "memory");
 }
