@@ -16,16 +16,17 @@ int device_context(int *num_sms, int **err);
 
 namespace {
 
-// dst[i][j] = src[i][j], rows of `ld` elements: operands that a copy engine cannot read (odd strides or
-// addresses) are copied once.  32 x 32 tiles through shared memory, so that both sides are
-// coalesced whichever stride of src is 1.
-__global__ void pack_kernel(Matrix16 src, int64_t rows, int64_t cols, uint16_t *dst, int64_t ld) {
+// dst[z][i][j] = src[z][i][j], rows of `ld` elements: operands that a copy engine cannot read (odd
+// strides or addresses) are copied once.  32 x 32 tiles through shared memory, so that both sides
+// are coalesced whichever stride of src is 1.
+__global__ void pack_kernel(Matrix16 src, int64_t batch, int64_t s_batch, int64_t rows, int64_t cols,
+                            uint16_t *dst, int64_t ld) {
     __shared__ uint16_t tile[32][33];
-    const uint16_t *s = static_cast<const uint16_t *>(src.p);
-    const int64_t tiles_c = (cols + 31) / 32, total = (rows + 31) / 32 * tiles_c;
+    const int64_t tiles_c = (cols + 31) / 32, tiles = (rows + 31) / 32 * tiles_c;
     const bool turned = src.s0 == 1 && src.s1 != 1;
-    for (int64_t u = blockIdx.x; u < total; u += gridDim.x) {
-        const int64_t r0 = u / tiles_c * 32, c0 = u % tiles_c * 32;
+    for (int64_t u = blockIdx.x; u < batch * tiles; u += gridDim.x) {
+        const int64_t z = u / tiles, r0 = u % tiles / tiles_c * 32, c0 = u % tiles_c * 32;
+        const uint16_t *s = static_cast<const uint16_t *>(src.p) + z * s_batch;
         for (int y = threadIdx.y; y < 32; y += 8) {
             const int64_t i = r0 + (turned ? threadIdx.x : y), j = c0 + (turned ? y : threadIdx.x);
             if (i < rows && j < cols)
@@ -34,7 +35,7 @@ __global__ void pack_kernel(Matrix16 src, int64_t rows, int64_t cols, uint16_t *
         __syncthreads();
         for (int y = threadIdx.y; y < 32; y += 8)
             if (r0 + y < rows && c0 + threadIdx.x < cols)
-                dst[(r0 + y) * ld + c0 + threadIdx.x] = tile[y][threadIdx.x];
+                dst[(z * rows + r0 + y) * ld + c0 + threadIdx.x] = tile[y][threadIdx.x];
         __syncthreads();
     }
 }
@@ -73,6 +74,14 @@ struct Arena {
     }
 };
 
+void pack(const Matrix16 &M, int64_t batch, int64_t s_batch, int64_t rows, int64_t cols, void *dst,
+          int64_t ld, int sms, cudaStream_t st) {
+    const int64_t tiles = batch * ((rows + 31) / 32) * ((cols + 31) / 32), most = int64_t(sms) * 8;
+    if (tiles)
+        pack_kernel<<<static_cast<unsigned>(tiles < most ? tiles : most), dim3(32, 8), 0, st>>>(
+            M, batch, s_batch, rows, cols, static_cast<uint16_t *>(dst), ld);
+}
+
 // The matrix as `rows` rows of contiguous elements that a copy engine can read: itself, or a
 // packed copy in the workspace (launched unless the arena only counts).
 Matrix16 readable(const Matrix16 &M, int64_t rows, int64_t cols, Arena &arena, int sms,
@@ -80,12 +89,19 @@ Matrix16 readable(const Matrix16 &M, int64_t rows, int64_t cols, Arena &arena, i
     const int64_t ld = round8(cols);
     if (copyable(M.p, rows, M.s0, M.s1, cols)) return Matrix16{M.p, rows <= 1 ? ld : M.s0, 1};
     void *dst = arena.take(sizeof(uint16_t) * static_cast<size_t>(rows * ld));
-    if (arena.base && rows && cols) {
-        const int64_t tiles = (rows + 31) / 32 * ((cols + 31) / 32), most = int64_t(sms) * 8;
-        pack_kernel<<<static_cast<unsigned>(tiles < most ? tiles : most), dim3(32, 8), 0, st>>>(
-            M, rows, cols, static_cast<uint16_t *>(dst), ld);
-    }
+    if (arena.base) pack(M, 1, 0, rows, cols, dst, ld, sms, st);
     return Matrix16{dst, ld, 1};
+}
+
+// A projecting factor (s adapters, cols x r) as it is, or, where the copy engine has to read it and
+// cannot, packed in rows of one rank.
+Factor16 readable_factor(const Factor16 &F, int64_t s, int64_t cols, int64_t r, int64_t rows,
+                         Arena &arena, int sms, cudaStream_t st) {
+    if (rows <= kProjectRowsLimit || factor_mode(F) != kFScalar) return F;
+    const int64_t ld = round8(cols), batch = F.ss == 0 ? 1 : s;
+    void *dst = arena.take(sizeof(uint16_t) * static_cast<size_t>(batch * r * ld));
+    if (arena.base) pack(Matrix16{F.p, F.sr, F.sc}, batch, F.ss, r, cols, dst, ld, sms, st);
+    return Factor16{dst, F.ss == 0 ? 0 : r * ld, 1, ld};
 }
 
 // W (inner x cols) with one unit stride, readable in that orientation.
@@ -120,7 +136,7 @@ cudaError_t clear(void *out, int64_t ldo, int64_t rows, int64_t cols, cudaStream
 // The projection, then the expansion that reads it.
 cudaError_t project_expand(bool half, const ProjectOperands &p, const ExpandOperands *x, int sms,
                            int *err, cudaStream_t st) {
-    const cudaError_t e = lr_project(half, p, sms, st);
+    const cudaError_t e = lr_project(half, p, sms, err, st);
     if (e != cudaSuccess || !x) return e;
     if (!x->inner) return clear(x->out, x->ldo, x->rows, x->cols, st);
     return x->rows <= kExpandRowsLimit ? lr_expand_rows(half, *x, sms, err, st)
@@ -135,9 +151,11 @@ int forward(const ti_low_rank_t &op, void *Y, int64_t ldy, float *P, Arena &aren
     if (!P) P = own;
     const Matrix16 X = readable(Matrix16{op.x, op.sx0, op.sx1}, op.t, op.k, arena, sms, st);
     const Matrix16 W = readable_w(Matrix16{op.w, op.sw0, op.sw1}, op.k, op.n, arena, sms, st);
+    const Factor16 A = readable_factor(Factor16{op.a, op.sa0, op.sa1, op.sa2}, op.s, op.k, op.r,
+                                       op.t, arena, sms, st);
     if (!arena.base) return TI_OK;
     const ProjectOperands p{X,     op.t,     op.k,
-                            Factor16{op.a, op.sa0, op.sa1, op.sa2},
+                            A,
                             op.r,  index,    op.scale,
                             op.alpha * dropout_scale(drop.cut),
                             drop,  P};
@@ -158,11 +176,13 @@ int backward(const ti_low_rank_t &op, const Gradient &g, Arena &arena, int sms, 
     void *lists = arena.take(plan.list_bytes);
     float *part_a = plan.part_a ? static_cast<float *>(arena.take(plan.part_a)) : nullptr;
     float *part_b = plan.part_b ? static_cast<float *>(arena.take(plan.part_b)) : nullptr;
+    const Factor16 Bt = readable_factor(Factor16{op.b, op.sb0, op.sb2, op.sb1}, op.s, op.n, op.r,
+                                        op.t, arena, sms, st);
     if (!arena.base) return TI_OK;
     const bool half = op.dtype == TI_TYPE_F16;
     if ((g.dX || g.dA) && op.t) {
         const ProjectOperands p{dY,    op.t,     op.n,
-                                Factor16{op.b, op.sb0, op.sb2, op.sb1},
+                                Bt,
                                 op.r,  index,    op.scale,
                                 op.alpha * dropout_scale(drop.cut),
                                 Dropout{}, dP};

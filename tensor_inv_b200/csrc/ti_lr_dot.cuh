@@ -8,16 +8,6 @@
 
 namespace ti {
 
-// How a factor is read: element by element, in 16-byte vectors along c, or along the rank.
-enum { kFScalar = 0, kFC = 1, kFR = 2 };
-
-__host__ inline int factor_mode(const Factor16 &F) {
-    const bool base = (reinterpret_cast<uintptr_t>(F.p) & 15) == 0 && F.ss % 8 == 0;
-    if (base && F.sc == 1 && F.sr % 8 == 0) return kFC;
-    if (base && F.sr == 1 && F.sc % 8 == 0) return kFR;
-    return kFScalar;
-}
-
 // 8 consecutive elements at `p`, of which the first n exist (n <= 0: none)
 __device__ __forceinline__ uint4 load8(const uint16_t *p, int64_t n) {
     if (n >= 8) return __ldg(reinterpret_cast<const uint4 *>(p));

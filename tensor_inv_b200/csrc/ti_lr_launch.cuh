@@ -21,6 +21,16 @@ inline bool copyable(const void *p, int64_t rows, int64_t ld, int64_t s_inner, i
 // Up to this many rows, project runs a cluster per row, above it tiles of 128 rows.
 constexpr int64_t kProjectRowsLimit = 256;
 
+// How a factor is read: element by element, in 16-byte vectors along c, or along the rank.
+enum { kFScalar = 0, kFC = 1, kFR = 2 };
+
+inline int factor_mode(const Factor16 &F) {
+    const bool base = (reinterpret_cast<uintptr_t>(F.p) & 15) == 0 && F.ss % 8 == 0;
+    if (base && F.sc == 1 && F.sr % 8 == 0) return kFC;
+    if (base && F.sr == 1 && F.sc % 8 == 0) return kFR;
+    return kFScalar;
+}
+
 // P = f (m M) F: the rows' projections, F a factor along M's inner dimension.
 struct ProjectOperands {
     Matrix16 M;  // unit s1, copyable
@@ -33,7 +43,9 @@ struct ProjectOperands {
     Dropout drop;
     float *P;
 };
-cudaError_t lr_project(bool half, const ProjectOperands &o, int num_sms, cudaStream_t stream);
+// With more than kProjectRowsLimit rows the copy engine reads F: factor_mode(F) != kFScalar.
+cudaError_t lr_project(bool half, const ProjectOperands &o, int num_sms, int *err,
+                       cudaStream_t stream);
 
 // out = M W + m (P F), F a factor along out's columns.
 struct ExpandOperands {

@@ -2,17 +2,19 @@
 //
 //   P[t][j] = alpha * scale[i] * sum_c m(t, c) M[t][c] F[i][c][j]        (float32, t x r)
 //
-// One pass over M: 2 r operations per element against 2 bytes, so M's bytes bound it for the
-// ranks that adapters have, and the legacy tensor path (mma.sync, operands in registers) is fast
-// enough -- what counts is that M goes from memory to registers once, with the mask applied on the
-// way, and never through shared memory.  Two kernels:
-//   tiles: 128 rows x a slice of the inner dimension per CTA; a cluster of up to 8 CTAs shares the
-//          rows and adds its slices through distributed shared memory.  Every warp walks the distinct
-//          adapters of its own 32 rows (one, for the runs of rows that prompts and training steps
-//          have), reads their factor in fragment order straight from the caches and waits for
-//          nobody; a row keeps the result of its own adapter.
+// One pass over M, 2 r operations per element against 2 bytes: M's bytes bound it.
+//   tiles: 128 rows x a slice of the inner dimension per CTA, M and F staged by the copy engine, the
+//          products on tcgen05 with up to 64 ranks per MMA.  Each distinct adapter among the rows
+//          has its own accumulator columns, so M is read once for all of them (up to kSlots; more
+//          take further passes, from L2); a row keeps the columns of its own adapter, and nothing
+//          of another reaches it.  With dropout, the mask is applied to the staged tile between
+//          the copy and the MMA.  A cluster of up to 8 CTAs shares the rows; each sends its sums
+//          to the CTA that finishes the row, which adds them in rank order.
 //   rows:  one row per cluster, plain multiply-adds: for few rows each with an adapter of its own
 //          F's bytes bound it, and no product is shared between rows.
+#include <atomic>
+#include <cstring>
+
 #include "ti_lr_dot.cuh"
 #include "ti_lr_launch.cuh"
 
@@ -33,235 +35,337 @@ struct ProjectParams {
     int mode;       // how F is read: kFC vectors along c, kFR vectors along j, kFScalar
 };
 
-template <typename T>
-__device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2,
-                                         uint32_t a3, uint32_t b0, uint32_t b1);
-template <>
-__device__ __forceinline__ void mma16816<__nv_bfloat16>(float (&d)[4], uint32_t a0, uint32_t a1,
-                                                        uint32_t a2, uint32_t a3, uint32_t b0,
-                                                        uint32_t b1) {
+constexpr int kTileRows = 128, kBK = 64;
+constexpr int kWorkers = 256, kTileThreads = 64 + kWorkers;  // copies, MMA issue, 8 workers
+constexpr int kMBytes = kTileRows * kBK * 2, kFBytes = 16384;  // per stage
+constexpr int kStageBytes = kMBytes + kFBytes, kStages = 5;
+constexpr int kBlockRanks = 64;  // ranks of one CTA
+constexpr uint32_t kTmemCols = 128;
+constexpr size_t kTileSmem = size_t(kStages) * kStageBytes + sizeof(float) * kTileRows * kBlockRanks +
+                             1024 + 1024 + 512;
+
+struct TileParams {
+    int64_t rows, r;
+    RowIndex index;
+    const float *scale;
+    float alpha;
+    Dropout drop;
+    float *P;
+    int num_kb, per_rank;   // steps of the inner dimension, and how many each rank takes
+    int rp;                 // ranks per adapter in TMEM: r, or the block's part, rounded up to 16
+    int slots, slot_bytes;  // adapters per pass, and their bytes in a stage
+    int along_rank;         // F's vectors run along the rank (N-major operand)
+    int one_adapter;        // all adapters are the same memory
+    uint32_t idesc;
+    int *err;
+};
+
+__device__ __forceinline__ void umma_f16(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc,
+                                         uint32_t accumulate) {
     asm volatile(
-        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
-        "{%8,%9}, {%0,%1,%2,%3};"
-        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+        : "memory");
 }
-template <>
-__device__ __forceinline__ void mma16816<__half>(float (&d)[4], uint32_t a0, uint32_t a1,
-                                                 uint32_t a2, uint32_t a3, uint32_t b0,
-                                                 uint32_t b1) {
+
+// 32 lanes x 16 columns of 32-bit TMEM words
+__device__ __forceinline__ void tmem_ld_32x32b_x16(uint32_t taddr, uint32_t (&r)[16]) {
     asm volatile(
-        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
-        "{%8,%9}, {%0,%1,%2,%3};"
-        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
+          "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]),
+          "=r"(r[14]), "=r"(r[15])
+        : "r"(taddr)
+        : "memory");
 }
 
-__device__ __forceinline__ void store_cluster(uint32_t addr, float v) {
-    asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(addr), "f"(v));
+__device__ __forceinline__ void store_cluster4(uint32_t addr, uint32_t a, uint32_t b, uint32_t c,
+                                               uint32_t d) {
+    asm volatile("st.shared::cluster.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(a), "r"(b),
+                 "r"(c), "r"(d));
 }
 
-constexpr int kTileRows = 128, kTileThreads = 256, kGroups = 2;  // two groups share the slice
-constexpr int kChunk = 64;  // inner elements per warp and step
-
-template <int kNT>
-constexpr size_t tile_smem() {
-    return sizeof(float) * kGroups * kTileRows * 8 * kNT;
+__device__ __forceinline__ void raise(const TileParams &P, volatile int *abort, int code) {
+    *abort = 1;
+    atomicCAS(P.err, 0, code);
 }
 
-// kNT 16-bit elements in one load (kNT = 1, 2 or 4).
-template <int kNT>
-__device__ __forceinline__ uint2 load_few(const uint16_t *p) {
-    if constexpr (kNT == 4) return __ldg(reinterpret_cast<const uint2 *>(p));
-    if constexpr (kNT == 2) return make_uint2(__ldg(reinterpret_cast<const uint32_t *>(p)), 0);
-    return make_uint2(__ldg(p), 0);
-}
-
-// F's fragments for 32 inner elements: f[n] holds, for column tile n, the thread's elements
-// c .. c + 7 of its column, in pairs.  Where F's vectors run along the rank (kFR), a thread reads
-// kNT consecutive ranks of each element, so the columns of the tiles interleave: column `g` of
-// tile n is rank kNT * g + n, else 8 * n + g.  kWhole: no element lies past the end (c + 8 <= end;
-// for kFR, r is a multiple of kNT); the general form handles every edge and every stride.
-template <int kNT, int kMode, bool kWhole>
-__device__ __forceinline__ void load_fragments(const ProjectParams &P, const uint16_t *F, int64_t c,
-                                               int64_t end, int64_t j0, int g, uint4 (&f)[kNT]) {
-    const int r = static_cast<int>(P.r);
-    if constexpr (kMode == kFR) {
-        const int j = static_cast<int>(j0) + kNT * g;
-        uint2 v[8];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            v[e] = make_uint2(0, 0);
-            const uint16_t *src = F + (c + e) * P.F.sc + j;
-            if (kWhole) {
-                if (j < r) v[e] = load_few<kNT>(src);
-            } else if (c + e < end) {
-#pragma unroll
-                for (int n = 0; n < kNT; ++n)
-                    if (j + n < r)
-                        (n < 2 ? v[e].x : v[e].y) |= static_cast<uint32_t>(__ldg(src + n))
-                                                     << (16 * (n & 1));
-            }
-        }
-#pragma unroll
-        for (int n = 0; n < kNT; ++n) {
-            const uint32_t sel = n & 1 ? 0x7632u : 0x5410u;  // upper or lower halves of two words
-            auto word = [&](int e) { return n < 2 ? v[e].x : v[e].y; };
-            f[n] = make_uint4(__byte_perm(word(0), word(1), sel), __byte_perm(word(2), word(3), sel),
-                              __byte_perm(word(4), word(5), sel), __byte_perm(word(6), word(7), sel));
-        }
-    } else {
-#pragma unroll
-        for (int n = 0; n < kNT; ++n) {
-            const int j = static_cast<int>(j0) + 8 * n + g;
-            f[n] = make_uint4(0, 0, 0, 0);
-            if (kWhole) {
-                if (j < r) f[n] = __ldg(reinterpret_cast<const uint4 *>(F + j * P.F.sr + c));
-            } else if (j < r) {
-                uint32_t w[4] = {0, 0, 0, 0};
-#pragma unroll
-                for (int e = 0; e < 8; ++e)
-                    if (c + e < end)
-                        w[e >> 1] |= static_cast<uint32_t>(__ldg(F + (c + e) * P.F.sc + j * P.F.sr))
-                                     << (16 * (e & 1));
-                f[n] = make_uint4(w[0], w[1], w[2], w[3]);
-            }
+__device__ __forceinline__ void drain_wait(const TileParams &P, uint64_t *bar, uint32_t parity) {
+    const uint32_t a = smem_u32(bar);
+    const unsigned long long t0 = globaltimer_ns();
+    while (!mbar_try_wait(a, parity)) {
+        if (globaltimer_ns() - t0 > kWaitTimeoutNs) {
+            atomicCAS(P.err, 0, kErrTimeoutDrain);
+            return;
         }
     }
 }
 
-template <typename T, int kNT, bool kDrop, int kMode>
-__global__ void __launch_bounds__(kTileThreads, 2)
-    project_tiles_kernel(const __grid_constant__ ProjectParams P) {
-    extern __shared__ __align__(16) uint8_t smem[];
-    // what this CTA finishes: [sending CTA and group][row of its share][8*kNT]
-    float *sum = reinterpret_cast<float *>(smem);
-    __shared__ int sidx[kTileRows];
-    cluster_arrive();  // awaited before anything is written to another CTA: it must have started
+// Roles: warp 0 copies, warp 1 TMEM and MMA issue, warps 2..9 the mask and the epilogue.
+template <typename T, bool kDrop>
+__global__ void __launch_bounds__(kTileThreads, 1)
+    project_tiles_kernel(const __grid_constant__ CUtensorMap tmM,
+                         const __grid_constant__ CUtensorMap tmF,
+                         const __grid_constant__ TileParams P) {
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t *ring = reinterpret_cast<uint8_t *>(
+        (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    // what this CTA finishes: [sending CTA][row of its share][rp]
+    float *sum = reinterpret_cast<float *>(ring + kStages * kStageBytes);
+    int *sidx = reinterpret_cast<int *>(sum + kTileRows * kBlockRanks);  // [128] rows' adapters
+    int *list = sidx + kTileRows;                                        // [128] distinct ones
+    uint64_t *full = reinterpret_cast<uint64_t *>(list + kTileRows);
+    uint64_t *ready = full + kStages;   // with dropout: the tile is masked
+    uint64_t *empty = ready + kStages;
+    uint64_t *tfull = empty + kStages;
+    uint64_t *tempty = tfull + 1;
+    uint64_t *drain = tempty + 1;
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(drain + 1);
+    volatile int *abort = reinterpret_cast<volatile int *>(tmem_slot + 1);
+    int *distinct = const_cast<int *>(abort) + 1;
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int g = lane >> 2, tq = lane & 3;
-    const int group = warp >> 2;
-    const uint32_t crank = cluster_rank(), csize = cluster_size();
-    const int share = kTileRows / static_cast<int>(csize);  // rows that each CTA finishes
+    const int rank = static_cast<int>(cluster_rank()), csize = static_cast<int>(cluster_size());
+    const int share = kTileRows / csize;  // rows that each CTA finishes
     const int64_t row0 = int64_t(blockIdx.x / csize) * kTileRows;
-    const int64_t j0 = int64_t(blockIdx.y) * 8 * kNT;
-    const int64_t begin = int64_t(crank) * P.slice;
-    const int64_t end = min(P.cols, begin + P.slice);
-    const uint64_t key = kDrop ? dropout_key(P.drop) : 0;
+    const int j0 = static_cast<int>(blockIdx.y) * kBlockRanks;
+    const int kb0 = rank * P.per_rank;
+    const int steps = max(0, min(P.num_kb, kb0 + P.per_rank) - kb0);
 
-    const int wrow = (warp & 3) * 32;  // this warp's 32 rows; the thread's are wrow + g + 8*i
-    const int64_t mine = row0 + wrow + lane;
-    const int my = mine < P.rows ? P.index.at(mine) : -1;
-    if (group == 0) sidx[wrow + lane] = my;
-    int idx[4];
-    const uint16_t *M[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        idx[i] = __shfl_sync(0xFFFFFFFFu, my, g + 8 * i);
-        M[i] = static_cast<const uint16_t *>(P.M) + (row0 + wrow + g + 8 * i) * P.ld;
-    }
-    // F's vectors can be read whole (a factor in neither vector order runs as kFC, by elements)
-    const bool vectors = P.mode == kMode && (kMode == kFC || P.r % kNT == 0);
-    int cur = -1;
-    bool started = false;
-    while (true) {
-        // the next adapter of the warp's rows in increasing order
-        const unsigned next = __reduce_min_sync(
-            0xFFFFFFFFu, my > cur ? static_cast<unsigned>(my) : 0x7FFFFFFFu);
-        if (next == 0x7FFFFFFFu) break;
-        cur = static_cast<int>(next);
-        const uint16_t *F = static_cast<const uint16_t *>(P.F.p) + cur * P.F.ss;
-        float acc[2][kNT][4];
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-#pragma unroll
-            for (int n = 0; n < kNT; ++n)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) acc[i][n][e] = 0.0f;
-
-        auto step = [&](int64_t c0, auto whole) {
-            constexpr bool kWhole = decltype(whole)::value;
-            uint4 x[kChunk / 32][4], f[kChunk / 32][kNT];
-#pragma unroll
-            for (int s = 0; s < kChunk / 32; ++s) {
-                const int64_t c = c0 + 32 * s + 8 * tq;
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    x[s][i] = make_uint4(0, 0, 0, 0);
-                    if (idx[i] == cur)
-                        x[s][i] = kWhole ? __ldg(reinterpret_cast<const uint4 *>(M[i] + c))
-                                         : load8(M[i] + c, end - c);
-                }
-            }
-#pragma unroll
-            for (int s = 0; s < kChunk / 32; ++s)
-                load_fragments<kNT, kMode, kWhole>(P, F, c0 + 32 * s + 8 * tq, end, j0, g, f[s]);
-#pragma unroll
-            for (int s = 0; s < kChunk / 32; ++s) {
-                if (kDrop) {
-#pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        x[s][i] = masked(x[s][i], P.drop, key,
-                                         static_cast<uint32_t>(row0 + wrow + g + 8 * i),
-                                         static_cast<uint32_t>((c0 + 32 * s + 8 * tq) >> 3));
-                }
-#pragma unroll
-                for (int n = 0; n < kNT; ++n) {
-                    // the order of the inner dimension is free: a thread's 8 consecutive
-                    // elements fill the slots of two k16 steps, in M and F alike
-#pragma unroll
-                    for (int i = 0; i < 2; ++i) {
-                        const uint4 &a = x[s][2 * i], &b = x[s][2 * i + 1];
-                        mma16816<T>(acc[i][n], a.x, b.x, a.y, b.y, f[s][n].x, f[s][n].y);
-                        mma16816<T>(acc[i][n], a.z, b.z, a.w, b.w, f[s][n].z, f[s][n].w);
-                    }
-                }
-            }
-        };
-        int64_t c0 = begin + group * kChunk;
-        if (vectors)
-#pragma unroll 1
-            for (; c0 + kChunk <= end; c0 += kGroups * kChunk) step(c0, std::true_type{});
-#pragma unroll 1
-        for (; c0 < end; c0 += kGroups * kChunk) step(c0, std::false_type{});
-        // rows of this adapter keep its sums
-        if (!started) {
-            started = true;
-            cluster_wait();
+    if (threadIdx.x == 0) {
+        prefetch_tensormap(&tmM);
+        prefetch_tensormap(&tmF);
+        for (int s = 0; s < kStages; ++s) {
+            mbar_init(&full[s], 1);
+            mbar_init(&ready[s], kWorkers / 32);
+            mbar_init(&empty[s], 1);
         }
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-            if (idx[i] == cur) {
-                const int lr = wrow + g + 8 * i;
-                float *dst = sum + ((crank * kGroups + group) * share + lr % share) * 8 * kNT;
-                const uint32_t to = map_to_rank(smem_u32(dst), lr / share);
-#pragma unroll
-                for (int n = 0; n < kNT; ++n)
-#pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        const int col = 2 * tq + e;
-                        store_cluster(to + 4 * (kMode == kFR ? kNT * col + n : 8 * n + col),
-                                      acc[i >> 1][n][2 * (i & 1) + e]);
-                    }
-            }
+        mbar_init(tfull, 1);
+        mbar_init(tempty, 4);
+        mbar_init(drain, 1);
+        *abort = 0;
+        fence_barrier_init();
     }
-    if (!started) cluster_wait();
+    if (warp == 1) {
+        tmem_alloc(tmem_slot, kTmemCols);
+        tmem_relinquish();
+    }
+    if (warp == 2) {
+        // the rows' adapters, and the distinct ones in increasing order
+        int idx[4];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            const int64_t t = row0 + 32 * q + lane;
+            idx[q] = t < P.rows ? P.index.at(t) : -1;
+            sidx[32 * q + lane] = idx[q];
+        }
+        int cur = -1, n = 0;
+        while (true) {
+            unsigned least = 0x7FFFFFFFu;
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+                if (idx[q] > cur) least = min(least, static_cast<unsigned>(idx[q]));
+            least = __reduce_min_sync(0xFFFFFFFFu, least);
+            if (least == 0x7FFFFFFFu) break;
+            cur = static_cast<int>(least);
+            if (lane == 0) list[n] = cur;
+            ++n;
+        }
+        if (lane == 0) *distinct = n;
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem_base = *tmem_slot;
+    const int nd = *distinct;
+    cluster_arrive();  // awaited before anything is written to another CTA: it must have started
+
+    if (warp == 0) {
+        if (lane == 0) {
+            // ---------------- copies ----------------
+            int stage = 0;
+            uint32_t phase = 0, issued_mask = 0, issued_phase = 0;
+            bool ok = true;
+            for (int a0 = 0; ok && a0 < nd; a0 += P.slots) {
+                const int n = min(P.slots, nd - a0);
+                for (int k = 0; k < steps; ++k) {
+                    if (!mbar_wait(&empty[stage], phase ^ 1, abort)) {
+                        raise(P, abort, kErrTimeoutProducer);
+                        ok = false;
+                        break;
+                    }
+                    mbar_arrive_expect_tx(&full[stage], kMBytes + n * P.slot_bytes);
+                    const int k0 = (kb0 + k) * kBK;
+                    uint8_t *m = ring + stage * kStageBytes;
+                    tma_load_2d(m, &tmM, &full[stage], k0, static_cast<int>(row0));
+                    for (int a = 0; a < n; ++a) {
+                        const int s = P.one_adapter ? 0 : list[a0 + a];
+                        uint8_t *f = m + kMBytes + a * P.slot_bytes;
+                        if (P.along_rank)
+                            tma_load_3d(f, &tmF, &full[stage], j0, k0, s);
+                        else
+                            tma_load_3d(f, &tmF, &full[stage], k0, j0, s);
+                    }
+                    issued_mask |= 1u << stage;
+                    issued_phase = (issued_phase & ~(1u << stage)) | (phase << stage);
+                    if (++stage == kStages) {
+                        stage = 0;
+                        phase ^= 1;
+                    }
+                }
+            }
+            if (!ok)  // every copy lands before the CTA may exit
+                for (int s = 0; s < kStages; ++s)
+                    if ((issued_mask >> s) & 1) drain_wait(P, &full[s], (issued_phase >> s) & 1);
+        }
+        __syncwarp();
+        cluster_wait();
+    } else if (warp == 1) {
+        if (lane == 0) {
+            // ---------------- MMA issuer ----------------
+            int stage = 0;
+            uint32_t phase = 0, pass = 0;
+            bool ok = true, any_issued = false;
+            for (int a0 = 0; ok && a0 < nd; a0 += P.slots, ++pass) {
+                const int n = min(P.slots, nd - a0);
+                if (!mbar_wait(tempty, (pass & 1) ^ 1, abort)) {
+                    raise(P, abort, kErrTimeoutMma);
+                    ok = false;
+                    break;
+                }
+                tc_fence_after();
+                for (int k = 0; k < steps; ++k) {
+                    if (!mbar_wait(kDrop ? &ready[stage] : &full[stage], phase, abort)) {
+                        raise(P, abort, kErrTimeoutMma);
+                        ok = false;
+                        break;
+                    }
+                    tc_fence_after();
+                    const uint32_t sm = smem_u32(ring + stage * kStageBytes);
+                    const uint64_t mdesc = make_sw128_kmajor_desc(sm);
+                    for (int a = 0; a < n; ++a) {
+                        const uint32_t sf = sm + kMBytes + a * P.slot_bytes;
+                        const uint64_t fdesc = P.along_rank ? make_sw128_mnmajor_desc(sf, 8192)
+                                                            : make_sw128_kmajor_desc(sf);
+                        const uint32_t fstep = P.along_rank ? 128 : 2;
+#pragma unroll
+                        for (int kk = 0; kk < kBK / 16; ++kk)
+                            umma_f16(tmem_base + a * P.rp, mdesc + 2 * kk, fdesc + fstep * kk,
+                                     P.idesc, (k | kk) != 0 ? 1u : 0u);
+                    }
+                    any_issued = true;
+                    umma_commit(&empty[stage]);
+                    if (++stage == kStages) {
+                        stage = 0;
+                        phase ^= 1;
+                    }
+                }
+                if (ok) umma_commit(tfull);
+            }
+            if (!ok && any_issued) {
+                umma_commit(drain);
+                drain_wait(P, drain, 0);
+            }
+        }
+        __syncwarp();
+        cluster_wait();
+    } else {
+        // ---------------- the mask, then the epilogue ----------------
+        const int wt = threadIdx.x - 64;
+        const int q = warp & 3, lr = q * 32 + lane;  // TMEM lane = row of the tile
+        const uint64_t key = kDrop ? dropout_key(P.drop) : 0;
+        const int own = sidx[lr];
+        float *dst = sum + (rank * share + lr % share) * P.rp;
+        bool started = false;
+        int stage = 0;
+        uint32_t phase = 0, pass = 0;
+        bool ok = true;
+        for (int a0 = 0; ok && a0 < nd; a0 += P.slots, ++pass) {
+            const int n = min(P.slots, nd - a0);
+            if (kDrop) {
+                for (int k = 0; k < steps; ++k) {
+                    ok = mbar_wait(&full[stage], phase, abort);
+                    if (!ok) {
+                        raise(P, abort, kErrTimeoutEpilogue);
+                        break;
+                    }
+                    uint8_t *m = ring + stage * kStageBytes;
+                    // a thread takes chunk wt % 8 of rows wt / 8, wt / 8 + 32, ...
+                    const int chunk = wt & 7;
+#pragma unroll
+                    for (int h = 0; h < kTileRows / 32; ++h) {
+                        const int mr = (wt >> 3) + 32 * h;
+                        uint4 *p = reinterpret_cast<uint4 *>(m + mr * 128 + ((chunk ^ (mr & 7)) << 4));
+                        *p = masked(*p, P.drop, key, static_cast<uint32_t>(row0 + mr),
+                                    static_cast<uint32_t>((kb0 + k) * (kBK / 8) + chunk));
+                    }
+                    fence_proxy_async_smem();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&ready[stage]);
+                    if (++stage == kStages) {
+                        stage = 0;
+                        phase ^= 1;
+                    }
+                }
+            }
+            ok = ok && mbar_wait(tfull, pass & 1, abort);
+            if (!ok) raise(P, abort, kErrTimeoutEpilogue);
+            ok = __all_sync(0xFFFFFFFFu, ok);
+            if (!started) {
+                started = true;
+                cluster_wait();
+            }
+            if (ok && warp < 6) {
+                tc_fence_after();
+                const uint32_t tbase = tmem_base + (static_cast<uint32_t>(q * 32) << 16);
+                const uint32_t to = map_to_rank(smem_u32(dst), lr / share);
+                for (int a = 0; a < n; ++a) {
+                    const bool mine = own == list[a0 + a];
+                    if (!__any_sync(0xFFFFFFFFu, mine)) continue;
+                    for (int j = 0; j < P.rp; j += 16) {
+                        uint32_t v[16];
+                        tmem_ld_32x32b_x16(tbase + a * P.rp + j, v);
+                        tmem_wait_ld();
+                        if (mine) {
+                            const uint32_t zero = steps > 0 ? 0xFFFFFFFFu : 0u;  // nothing in TMEM
+#pragma unroll
+                            for (int e = 0; e < 16; e += 4)
+                                store_cluster4(to + 4 * (j + e), v[e] & zero, v[e + 1] & zero,
+                                               v[e + 2] & zero, v[e + 3] & zero);
+                        }
+                    }
+                }
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(tempty);
+            }
+        }
+        if (!started) cluster_wait();
+    }
     // the kernel that reads P may prepare itself now; it waits for this grid before P
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 1) {
+        tc_fence_after();
+        tmem_dealloc(tmem_base, kTmemCols);
+    }
     cluster_sync_all();  // every sum has arrived; no remote access follows
     // the cluster's slices, added in order
-    for (int e = threadIdx.x; e < share * 8 * kNT; e += kTileThreads) {
-        const int lr = static_cast<int>(crank) * share + e / (8 * kNT), j = e % (8 * kNT);
+    for (int e = threadIdx.x; e < share * P.rp; e += kTileThreads) {
+        const int lr = rank * share + e / P.rp, j = j0 + e % P.rp;
         const int64_t t = row0 + lr;
-        if (t >= P.rows || j0 + j >= P.r) continue;
+        if (t >= P.rows || j >= P.r) continue;
         const int i = sidx[lr];
         float v = 0.0f;
         if (i >= 0) {
-            for (uint32_t q = 0; q < kGroups * csize; ++q) v += sum[q * share * 8 * kNT + e];
+            for (int c = 0; c < csize; ++c) v += sum[c * share * P.rp + e];
             v *= P.alpha * (P.scale ? P.scale[i] : 1.0f);
         }
-        P.P[t * P.r + j0 + j] = v;
+        P.P[t * P.r + j] = v;
     }
 }
 
@@ -411,9 +515,9 @@ __global__ void __launch_bounds__(kRowThreads, 3)
         }
 }
 
-template <typename K>
+template <typename K, typename... Args>
 cudaError_t launch_cluster(K kernel, int parts, dim3 grid, int threads, size_t smem,
-                           const ProjectParams &P, cudaStream_t stream) {
+                           cudaStream_t stream, const Args &...args) {
     // (Repeated settings are cheap and keep no state per device.)  An SM whose shared memory is
     // carved out small would have to drain before the expanding kernel's CTAs fit beside this one.
     cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout,
@@ -434,59 +538,91 @@ cudaError_t launch_cluster(K kernel, int parts, dim3 grid, int threads, size_t s
     attr.val.clusterDim.z = 1;
     cfg.attrs = &attr;
     cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, kernel, P);
+    return cudaLaunchKernelEx(&cfg, kernel, args...);
 }
 
-template <typename T, int kNT>
-cudaError_t tiles(const ProjectParams &P, int parts, dim3 grid, cudaStream_t stream) {
-    const size_t smem = tile_smem<kNT>();
-    if (P.mode == kFR)
-        return P.drop.cut ? launch_cluster(project_tiles_kernel<T, kNT, true, kFR>, parts, grid,
-                                           kTileThreads, smem, P, stream)
-                          : launch_cluster(project_tiles_kernel<T, kNT, false, kFR>, parts, grid,
-                                           kTileThreads, smem, P, stream);
-    return P.drop.cut ? launch_cluster(project_tiles_kernel<T, kNT, true, kFC>, parts, grid,
-                                       kTileThreads, smem, P, stream)
-                      : launch_cluster(project_tiles_kernel<T, kNT, false, kFC>, parts, grid,
-                                       kTileThreads, smem, P, stream);
+bool make_factor_map(CUtensorMap *map, const Factor16 &F, int mode, int64_t cols, int64_t r,
+                     int64_t adapters, int rp) {
+    EncodeTiledFn enc = get_encode_fn();
+    if (!enc) return false;
+    const bool along = mode == kFR;
+    const int64_t n_in = along ? r : cols, n_mid = along ? cols : r;
+    // (a dimension of one element has no stride of its own)
+    const int64_t s_mid = n_mid > 1 ? (along ? F.sc : F.sr) : (n_in + 7) / 8 * 8;
+    cuuint64_t dims[3] = {static_cast<cuuint64_t>(n_in), static_cast<cuuint64_t>(n_mid),
+                          static_cast<cuuint64_t>(adapters)};
+    cuuint64_t strides[2] = {static_cast<cuuint64_t>(2 * s_mid),
+                             static_cast<cuuint64_t>(2 * (adapters > 1 ? F.ss : s_mid * n_mid))};
+    cuuint32_t box[3] = {64, static_cast<cuuint32_t>(along ? kBK : rp), 1};
+    cuuint32_t estr[3] = {1, 1, 1};
+    return enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT16, 3, const_cast<void *>(F.p), dims, strides, box,
+               estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+               CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
 template <typename T>
-cudaError_t project(ProjectParams P, int num_sms, cudaStream_t stream) {
+cudaError_t project_tiles(const ProjectOperands &o, int num_sms, int *err, cudaStream_t stream) {
+    const int mode = factor_mode(o.F);
+    if (mode == kFScalar) return cudaErrorInvalidValue;  // the caller packs such a factor
+    TileParams P;
+    std::memset(&P, 0, sizeof(P));
+    P.rows = o.rows;
+    P.r = o.r;
+    P.index = o.index;
+    P.scale = o.scale;
+    P.alpha = o.alpha;
+    P.drop = o.drop;
+    P.P = o.P;
+    P.err = err;
+    P.num_kb = static_cast<int>((o.cols + kBK - 1) / kBK);
+    const int64_t blocks = (o.r + kBlockRanks - 1) / kBlockRanks;
+    P.rp = o.r >= kBlockRanks ? kBlockRanks : static_cast<int>((o.r + 15) / 16 * 16);
+    P.along_rank = mode == kFR;
+    P.one_adapter = o.F.ss == 0 || o.index.s == 1;
+    P.slot_bytes = P.along_rank ? 128 * kBK : 128 * P.rp;
+    P.slots = kFBytes / P.slot_bytes;
+    const int type = std::is_same<T, __half>::value ? 0 : 1;
+    P.idesc = (1u << 4) | (static_cast<uint32_t>(type) << 7) | (static_cast<uint32_t>(type) << 10) |
+              (P.along_rank ? 1u << 16 : 0u) | (static_cast<uint32_t>(P.rp >> 3) << 17) |
+              (static_cast<uint32_t>(kTileRows >> 4) << 24);
+    // 1, 2, 4 or 8 CTAs share a tile's inner dimension, as long as all fit one per SM
+    const int64_t tile_count = (o.rows + kTileRows - 1) / kTileRows;
     int parts = 1;
-    if (P.rows <= kProjectRowsLimit) {
-        // slices of 1024 (8 elements for each of 128 lanes) until 8 CTAs share a row
-        while (parts < 8 && P.cols > 1024 * parts) ++parts;
-        P.slice = ((P.cols + parts - 1) / parts + 255) / 256 * 256;
-        const dim3 grid(static_cast<unsigned>(parts * P.rows));
-        return P.drop.cut ? launch_cluster(project_rows_kernel<T, true>, parts, grid, kRowThreads,
-                                           0, P, stream)
-                          : launch_cluster(project_rows_kernel<T, false>, parts, grid, kRowThreads,
-                                           0, P, stream);
-    }
-    const int64_t tile_count = (P.rows + kTileRows - 1) / kTileRows;
-    // 8, 16 or 32 ranks per CTA; more of them read M again, from L2
-    const int nt = P.r <= 8 ? 1 : P.r <= 16 ? 2 : 4;
-    const int64_t blocks = (P.r + 8 * nt - 1) / (8 * nt);
-    // 1, 2, 4 or 8 CTAs share a tile's inner dimension, until two per SM have work
-    constexpr int kStep = kGroups * kChunk;
-    while (parts < 8 && tile_count * blocks * parts < 2 * num_sms && P.cols >= 2 * parts * kStep)
-        parts *= 2;
-    P.slice = ((P.cols + parts - 1) / parts + kStep - 1) / kStep * kStep;
+    while (parts < 8 && tile_count * blocks * 2 * parts <= num_sms && P.num_kb >= 4 * parts) parts *= 2;
+    P.per_rank = (P.num_kb + parts - 1) / parts;
+    CUtensorMap tmM, tmF;
+    if (!make_map16(&tmM, o.M.p, o.cols, o.rows, o.M.s0, kBK, kTileRows) ||
+        !make_factor_map(&tmF, o.F, mode, o.cols, o.r, P.one_adapter ? 1 : o.index.s, P.rp))
+        return cudaErrorInvalidValue;
     const dim3 grid(static_cast<unsigned>(parts * tile_count), static_cast<unsigned>(blocks));
-    switch (nt) {
-        case 1: return tiles<T, 1>(P, parts, grid, stream);
-        case 2: return tiles<T, 2>(P, parts, grid, stream);
-        default: return tiles<T, 4>(P, parts, grid, stream);
-    }
+    return o.drop.cut ? launch_cluster(project_tiles_kernel<T, true>, parts, grid, kTileThreads,
+                                       kTileSmem, stream, tmM, tmF, P)
+                      : launch_cluster(project_tiles_kernel<T, false>, parts, grid, kTileThreads,
+                                       kTileSmem, stream, tmM, tmF, P);
+}
+
+template <typename T>
+cudaError_t project(const ProjectOperands &o, int num_sms, int *err, cudaStream_t stream) {
+    if (o.rows > kProjectRowsLimit && o.cols > 0) return project_tiles<T>(o, num_sms, err, stream);
+    ProjectParams P{o.M.p,   o.M.s0,  o.rows,  o.cols, o.F, o.r,
+                    o.index, o.scale, o.alpha, o.drop, o.P, 0, factor_mode(o.F)};
+    // slices of 1024 (8 elements for each of 128 lanes) until 8 CTAs share a row
+    int parts = 1;
+    while (parts < 8 && P.cols > 1024 * parts) ++parts;
+    P.slice = ((P.cols + parts - 1) / parts + 255) / 256 * 256;
+    const dim3 grid(static_cast<unsigned>(parts * P.rows));
+    return P.drop.cut ? launch_cluster(project_rows_kernel<T, true>, parts, grid, kRowThreads, 0,
+                                       stream, P)
+                      : launch_cluster(project_rows_kernel<T, false>, parts, grid, kRowThreads, 0,
+                                       stream, P);
 }
 
 }  // namespace
 
-cudaError_t lr_project(bool half, const ProjectOperands &o, int num_sms, cudaStream_t stream) {
-    const ProjectParams P{o.M.p,   o.M.s0,  o.rows, o.cols, o.F, o.r,
-                          o.index, o.scale, o.alpha, o.drop, o.P, 0, factor_mode(o.F)};
-    return half ? project<__half>(P, num_sms, stream) : project<__nv_bfloat16>(P, num_sms, stream);
+cudaError_t lr_project(bool half, const ProjectOperands &o, int num_sms, int *err,
+                       cudaStream_t stream) {
+    return half ? project<__half>(o, num_sms, err, stream)
+                : project<__nv_bfloat16>(o, num_sms, err, stream);
 }
 
 }  // namespace ti
