@@ -19,13 +19,13 @@ __device__ __forceinline__ uint4 load8(const uint16_t *p, int64_t n) {
 }
 
 // 8 elements of a row with the dropout mask applied.
-__device__ __forceinline__ uint4 masked(uint4 v, const Dropout &d, uint64_t key, uint32_t row,
-                                        uint32_t block) {
+__device__ __forceinline__ uint4 masked(uint4 v, const Dropout &d, const DropoutKeys &keys,
+                                        uint32_t row, uint32_t block) {
     if (d.cut > 65535u) return make_uint4(0, 0, 0, 0);  // everything is dropped
-    const uint4 b = dropout_bits(d, key, row, block);
-    const uint32_t cut2 = d.cut * 0x10001u;
-    return make_uint4(v.x & __vcmpgeu2(b.x, cut2), v.y & __vcmpgeu2(b.y, cut2),
-                      v.z & __vcmpgeu2(b.z, cut2), v.w & __vcmpgeu2(b.w, cut2));
+    const uint4 b = dropout_bits(d, keys, row, block);
+    const uint32_t cut16 = d.cut << 16;
+    return make_uint4(keep_pair(v.x, b.x, cut16), keep_pair(v.y, b.y, cut16),
+                      keep_pair(v.z, b.z, cut16), keep_pair(v.w, b.w, cut16));
 }
 
 template <typename T>

@@ -370,7 +370,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         // ---------------- epilogue (warps 2..5, both CTAs) ----------------
         const int q = warp & 3;  // TMEM lane quadrant this warp may access
         int64_t unit = 0;
-        const uint64_t key = kDrop ? dropout_key(P.drop) : 0;
+        const DropoutKeys key(kDrop ? dropout_key(P.drop) : 0);
         T *out = static_cast<T *>(P.out);
         tiles(P, [&](int tm, int tn) {
             const int acc = static_cast<int>(unit & 1);

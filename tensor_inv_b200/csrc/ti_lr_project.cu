@@ -276,7 +276,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         // ---------------- the mask, then the epilogue ----------------
         const int wt = threadIdx.x - 64;
         const int q = warp & 3, lr = q * 32 + lane;  // TMEM lane = row of the tile
-        const uint64_t key = kDrop ? dropout_key(P.drop) : 0;
+        const DropoutKeys key(kDrop ? dropout_key(P.drop) : 0);
         const int own = sidx[lr];
         float *dst = sum + (rank * share + lr % share) * P.rp;
         bool started = false;
@@ -383,7 +383,7 @@ constexpr int kMaxRankRows = 256;
 template <typename T, bool kDrop>
 __device__ __forceinline__ void dot_slice(const ProjectParams &P, const uint16_t *x,
                                           const uint16_t *F, int64_t begin, int64_t end,
-                                          uint64_t key, uint32_t row, int warp, int lane,
+                                          const DropoutKeys &key, uint32_t row, int warp, int lane,
                                           float (*part)[kMaxRankRows]) {
     const int r = static_cast<int>(P.r);
     if (P.mode == kFR) {
@@ -496,7 +496,8 @@ __global__ void __launch_bounds__(kRowThreads, 3)
     if (i >= 0)
         dot_slice<T, kDrop>(P, static_cast<const uint16_t *>(P.M) + t * P.ld,
                             static_cast<const uint16_t *>(P.F.p) + i * P.F.ss, begin, end,
-                            kDrop ? dropout_key(P.drop) : 0, static_cast<uint32_t>(t), warp, lane,
+                            DropoutKeys(kDrop ? dropout_key(P.drop) : 0),
+                            static_cast<uint32_t>(t), warp, lane,
                             part);
     cluster_wait();
     __syncthreads();
@@ -585,10 +586,14 @@ cudaError_t project_tiles(const ProjectOperands &o, int num_sms, int *err, cudaS
     P.idesc = (1u << 4) | (static_cast<uint32_t>(type) << 7) | (static_cast<uint32_t>(type) << 10) |
               (P.along_rank ? 1u << 16 : 0u) | (static_cast<uint32_t>(P.rp >> 3) << 17) |
               (static_cast<uint32_t>(kTileRows >> 4) << 24);
-    // 1, 2, 4 or 8 CTAs share a tile's inner dimension, as long as all fit one per SM
+    // 1, 2, 4 or 8 CTAs share a tile's inner dimension, as long as all fit one per SM.  (Clusters
+    // of 8 find room in fewer places: 16 of them do not fit at once, and 2048 x 4096 took 17.6 us
+    // with 16 clusters of 8, 4096 x 4096 14.5 us with 32 of 4.)
     const int64_t tile_count = (o.rows + kTileRows - 1) / kTileRows;
     int parts = 1;
-    while (parts < 8 && tile_count * blocks * 2 * parts <= num_sms && P.num_kb >= 4 * parts) parts *= 2;
+    while (parts < 8 && tile_count * blocks * 2 * parts <= (parts == 4 ? num_sms / 2 : num_sms) &&
+           P.num_kb >= 4 * parts)
+        parts *= 2;
     P.per_rank = (P.num_kb + parts - 1) / parts;
     CUtensorMap tmM, tmF;
     if (!make_map16(&tmM, o.M.p, o.cols, o.rows, o.M.s0, kBK, kTileRows) ||

@@ -273,7 +273,7 @@ __global__ void __launch_bounds__(kThreads, 2)
         const int64_t col = col0 + lc;
         float *send = part + rank * part_rows * kCols + lc;
         float *low = S::kLowApart ? part + csize * part_rows * kCols + lc : send;
-        const uint64_t key = kDrop ? dropout_key(P.drop) : 0;
+        const DropoutKeys key(kDrop ? dropout_key(P.drop) : 0);
         if (lt < kNT) sidx[lt] = adapter;
         low_sync();
         // the served rows k = group, group + 2, ..., kBatch of them at a time

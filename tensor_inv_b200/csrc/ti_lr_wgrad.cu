@@ -154,7 +154,7 @@ __global__ void __launch_bounds__(kThreads, 2) wgrad_kernel(const __grid_constan
     const bool direct = S.part == nullptr;
     int64_t pos = int64_t(blockIdx.y) * P.chunk;
     const int64_t stop = min(total, pos + P.chunk);
-    const uint64_t key = S.drop.cut ? dropout_key(S.drop) : 0;
+    const DropoutKeys key(S.drop.cut ? dropout_key(S.drop) : 0);
 
     // the first adapter whose rows reach past pos (from the first one, where every adapter's
     // gradient is written here)
