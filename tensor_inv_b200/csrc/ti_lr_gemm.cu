@@ -3,10 +3,10 @@
 //   out[t][c] = sum_k M[t][k] W[k][c] + m(t, c) sum_j P[t][j] F[i][c][j],   i = index[t]
 //
 // The shared product is a 16-bit GEMM on tcgen05 (kind::f16, float32 accumulators in TMEM) with
-// the shape of ti_gemm2.cu: a cluster of two CTAs owns a 256 x kBN output tile, CTA r loads rows
-// [128r, 128r+128) of M's tile and half of W's columns per 64-deep stage, and CTA 0 issues
-// M = 256 MMAs for both.  W is read in either orientation (K-major or N-major descriptors), so a
-// transposed view costs nothing.
+// the shape of ti_gemm2.cu: a cluster of two CTAs owns a 256 x 256 output tile, CTA r loads rows
+// [128r, 128r+128) of M's tile and columns [128r, 128r+128) of W's per 64-deep stage, and CTA 0
+// issues M = 256, N = 256 MMAs for both.  W is read in either orientation (K-major or N-major
+// descriptors), so a transposed view costs nothing.
 //
 // The low-rank term joins the same accumulator as extra steps of the inner dimension: for every
 // distinct adapter among the tile's 256 rows and every 16 of its ranks, one step multiplies the
@@ -17,44 +17,44 @@
 // zeros of foreign rows keep adapters apart -- except for 0 * inf: entries of P or F that are not
 // finite enter the MMA as zero and raise a flag, and the epilogue of such a tile adds their
 // products itself.
-// With dropout (dX) the mask applies to the low-rank term alone, so that term has its own
-// accumulator and the epilogue joins the two; tiles are then 128 columns wide, which keeps both
-// accumulators double buffered in the 512 TMEM columns.
+//
+// With dropout (dX) the mask applies to the low-rank term alone, so that term has its own 256
+// accumulator columns and the epilogue joins the two.  The 512 TMEM columns then hold one tile
+// instead of two, and the next tile's MMAs wait for the epilogue; so it prepares its mask bits
+// while the MMAs run, holds its results in registers, and gives TMEM back before it stores.
+// (128-column tiles would keep both accumulators double buffered, but need half as much again of
+// L2 reads per product: 171 us against 109 us without dropout at 4096^3.)
 //
 // Roles (both CTAs): warp 0 TMA producer; warp 1 TMEM allocation and, in CTA 0, the MMA issuer;
-// warps 2..5 epilogue; warps 6..9 loaders of the low-rank steps, which have their own stage, so
-// they fill it while the product's steps run.  A low-rank step is taken after every fourth step
-// of the product while any are left: a fixed order, so results repeat bit for bit.
+// warps 2..9 epilogue, two per TMEM lane quadrant with 128 columns each; warps 10..13 loaders of the
+// low-rank steps, which have their own stage, so they fill it while the product's steps run.  A
+// low-rank step is taken after every fourth step of the product while any are left: a fixed order,
+// so results repeat bit for bit.  The kernel may start before the projection has finished
+// (programmatic launch); the loaders wait for it.
 // All waits are bounded; on timeout the error word is raised and the CTA leaves its loops.
 #include <atomic>
 #include <cstring>
 #include <type_traits>
 
-#include "ti_common.cuh"
+#include "ti_lr_dot.cuh"
 #include "ti_lr_launch.cuh"
 
 namespace ti {
 namespace {
 
-constexpr int kBM = 256, kBK = 64;
-constexpr int kHalf = 128;                       // rows of M per CTA
-constexpr int kABytes = kHalf * kBK * 2;         // 16 KB
-constexpr int kThreads = 320;
-constexpr int kEpiWarps = 4, kLoaders = 128;
+constexpr int kBM = 256, kBN = 256, kBK = 64;
+constexpr int kHalf = 128;                       // rows of M and columns of W per CTA
+constexpr int kABytes = kHalf * kBK * 2, kBBytes = kHalf * kBK * 2;
+constexpr int kStageBytes = kABytes + kBBytes, kStages = 6;
+constexpr int kLowBytes = 2 * kHalf * 128;       // one low-rank step per CTA: rows of P, rows of F
+constexpr int kEpiWarps = 8, kLoaders = 128;
+constexpr int kThreads = 64 + 32 * kEpiWarps + kLoaders;
 constexpr uint32_t kTmemCols = 512;
 constexpr int kEvery = 4;                        // product steps between two low-rank steps
 constexpr int kGroupM = 8;                       // raster: 8 row tiles (2048 rows) at a time
 constexpr int kRankStep = 16;
-
-template <int kBN>
-struct Shape {
-    static constexpr int kCols = kBN / 2;                   // columns of W per CTA
-    static constexpr int kBBytes = kCols * kBK * 2;
-    static constexpr int kStageBytes = kABytes + kBBytes;
-    static constexpr int kLowBytes = kHalf * 128 + kCols * 128;  // one low-rank step per CTA
-    static constexpr int kStages = kBN == 256 ? 6 : 8;
-    static constexpr size_t kSmem = size_t(kStages) * kStageBytes + kLowBytes + 1024 + 512;
-};
+constexpr int kFixSlots = 8;
+constexpr size_t kSmem = size_t(kStages) * kStageBytes + kLowBytes + 1024 + 512;
 
 struct Params {
     int64_t rows, cols;
@@ -70,6 +70,7 @@ struct Params {
     void *out;
     int64_t ldo;
     int vec;        // rows of out are 16-byte aligned
+    int pvec, fvec; // P's rows in vectors of 4, F's in vectors of 8 along the rank
     int *err;
 };
 
@@ -157,14 +158,14 @@ __device__ __forceinline__ float4 *swizzled(uint8_t *tile, int row, int c) {
     return reinterpret_cast<float4 *>(tile + row * 128 + ((c ^ (row & 7)) << 4));
 }
 
-// Columns [c0, c0 + 32) of one row of a tile whose P or F holds entries that are not finite:
+// Columns [c0, c0 + 16) of one row of a tile whose P or F holds entries that are not finite:
 // adds the products that the MMA left out.
 template <typename T>
 __device__ __noinline__ void add_nonfinite(const Params &P, int64_t row, int64_t c0, float *acc) {
     const int i = P.index.at(row);
     if (i < 0) return;
     const T *f = static_cast<const T *>(P.F.p) + i * P.F.ss;
-    for (int c = 0; c < 32 && c0 + c < P.cols; ++c)
+    for (int c = 0; c < 16 && c0 + c < P.cols; ++c)
         for (int64_t j = 0; j < P.r; ++j) {
             const float p = P.P[row * P.r + j];
             const float b = to_float(f[(c0 + c) * P.F.sc + j * P.F.sr]);
@@ -185,22 +186,43 @@ __device__ __forceinline__ uint32_t pack2<__half>(float a, float b) {
     return *reinterpret_cast<uint32_t *>(&v);
 }
 
-template <typename T, int kBN, bool kDrop>
+__device__ __forceinline__ void store_flag(uint32_t addr) {
+    asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(addr), "r"(1) : "memory");
+}
+
+// Stores 32 packed columns of a row, as far as they exist.
+template <typename T>
+__device__ __forceinline__ void store32(const Params &P, T *row_dst, int64_t row, int64_t col0, int c,
+                                        const uint32_t (&pk)[16]) {
+    if (row >= P.rows || col0 >= P.cols) return;
+    T *dst = row_dst + 32 * c;
+    if (P.vec && col0 + 32 <= P.cols) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            reinterpret_cast<uint4 *>(dst)[j] =
+                make_uint4(pk[4 * j], pk[4 * j + 1], pk[4 * j + 2], pk[4 * j + 3]);
+    } else {
+        uint16_t *d = reinterpret_cast<uint16_t *>(dst);
+#pragma unroll
+        for (int j = 0; j < 32; ++j)
+            if (col0 + j < P.cols) d[j] = static_cast<uint16_t>(pk[j >> 1] >> (16 * (j & 1)));
+    }
+}
+
+template <typename T, bool kDrop>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     lr_gemm_kernel(const __grid_constant__ CUtensorMap tmM, const __grid_constant__ CUtensorMap tmW,
                    const __grid_constant__ Params P) {
-    using S = Shape<kBN>;
-    static_assert(!kDrop || kBN == 128, "two accumulators, double buffered, in 512 columns");
     extern __shared__ uint8_t smem_raw[];
     uint8_t *smem = reinterpret_cast<uint8_t *>(
         (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     uint8_t *sA = smem;
-    uint8_t *sB = sA + S::kStages * kABytes;
-    uint8_t *sP = sB + S::kStages * S::kBBytes;   // low-rank step: 128 rows of P, hi | lo
+    uint8_t *sB = sA + kStages * kABytes;
+    uint8_t *sP = sB + kStages * kBBytes;   // low-rank step: 128 rows of P, hi | lo
     uint8_t *sF = sP + kHalf * 128;               //                kCols rows of F
-    uint64_t *full = reinterpret_cast<uint64_t *>(sF + S::kCols * 128);  // CTA 0
-    uint64_t *empty = full + S::kStages;
-    uint64_t *tfull = empty + S::kStages;   // [2] both CTAs: accumulator ready
+    uint64_t *full = reinterpret_cast<uint64_t *>(sF + kHalf * 128);  // CTA 0
+    uint64_t *empty = full + kStages;
+    uint64_t *tfull = empty + kStages;   // [2] both CTAs: accumulator ready
     uint64_t *tempty = tfull + 2;           // [2] CTA 0: drained by both epilogues
     uint64_t *lfull = tempty + 2;           // CTA 0: low-rank step written in both CTAs
     uint64_t *lempty = lfull + 1;           // both CTAs: low-rank step taken
@@ -208,15 +230,15 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(drain + 1);
     volatile int *abort = reinterpret_cast<volatile int *>(tmem_slot + 1);
     volatile int *message = abort + 1;      // CTA 0: 8-wide steps in this low-rank step, 0: no more
-    volatile int *fix = message + 1;        // [4] by tile: entries that are not finite
-    int *least = const_cast<int *>(fix) + 4;  // [2][4] loaders' smallest adapter, by warp
+    volatile int *fix = message + 1;        // [kFixSlots] by tile: entries that are not finite
+    int *least = const_cast<int *>(fix) + kFixSlots;  // [2][4] loaders' smallest adapter, by warp
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t rank = cluster_rank();
-    constexpr int kAccCols = kDrop ? 2 * kBN : kBN;  // TMEM columns per buffer
+    constexpr int kBuffers = kDrop ? 1 : 2;  // tiles in TMEM
 
     if (threadIdx.x == 0) {
-        for (int s = 0; s < S::kStages; ++s) {
+        for (int s = 0; s < kStages; ++s) {
             mbar_init(&full[s], 1);
             mbar_init(&empty[s], 1);
         }
@@ -228,6 +250,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         mbar_init(lempty, 1);
         mbar_init(drain, 1);
         *abort = 0;
+        for (int f = 0; f < kFixSlots; ++f) fix[f] = 0;
         fence_barrier_init();
         prefetch_tensormap(&tmM);
         prefetch_tensormap(&tmW);
@@ -250,27 +273,27 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             bool ok = true;
             tiles(P, [&](int tm, int tn) {
                 const int row0 = tm * kBM + static_cast<int>(rank) * kHalf;
-                const int col0 = tn * kBN + static_cast<int>(rank) * S::kCols;
+                const int col0 = tn * kBN + static_cast<int>(rank) * kHalf;
                 for (int kb = 0; kb < P.num_kb; ++kb) {
                     if (!mbar_wait(&empty[stage], phase ^ 1, abort)) {
                         raise(P, abort, kErrTimeoutProducer);
                         ok = false;
                         return false;
                     }
-                    if (rank == 0) mbar_arrive_expect_tx(&full[stage], 2 * S::kStageBytes);
+                    if (rank == 0) mbar_arrive_expect_tx(&full[stage], 2 * kStageBytes);
                     const uint32_t fb = map_to_rank(smem_u32(&full[stage]), 0);
                     tma_load_2d_pair(sA + stage * kABytes, &tmM, fb, kb * kBK, row0);
-                    uint8_t *b = sB + stage * S::kBBytes;
+                    uint8_t *b = sB + stage * kBBytes;
                     if (P.w_nmajor) {
 #pragma unroll
-                        for (int h = 0; h < S::kCols / 64; ++h)
+                        for (int h = 0; h < kHalf / 64; ++h)
                             tma_load_2d_pair(b + h * 8192, &tmW, fb, col0 + 64 * h, kb * kBK);
                     } else {
                         tma_load_2d_pair(b, &tmW, fb, kb * kBK, col0);
                     }
                     issued_mask |= 1u << stage;
                     issued_phase = (issued_phase & ~(1u << stage)) | (phase << stage);
-                    if (++stage == S::kStages) {
+                    if (++stage == kStages) {
                         stage = 0;
                         phase ^= 1;
                     }
@@ -280,7 +303,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             if (!ok) {
                 // every issued copy lands before the pair may exit; CTA 0 sees both CTAs' bytes
                 if (rank == 0) {
-                    for (int s = 0; s < S::kStages; ++s)
+                    for (int s = 0; s < kStages; ++s)
                         if ((issued_mask >> s) & 1) drain_wait(P, &full[s], (issued_phase >> s) & 1);
                 } else {
                     const unsigned long long t0 = globaltimer_ns();
@@ -299,8 +322,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             const uint64_t pdesc = make_sw128_kmajor_desc(smem_u32(sP));
             const uint64_t fdesc = make_sw128_kmajor_desc(smem_u32(sF));
             tiles(P, [&](int, int) {
-                const int acc = static_cast<int>(unit & 1);
-                const uint32_t acc_phase = static_cast<uint32_t>((unit >> 1) & 1);
+                const int acc = static_cast<int>(unit % kBuffers);
+                const uint32_t acc_phase = static_cast<uint32_t>((unit / kBuffers) & 1);
                 ++unit;
                 if (!mbar_wait(&tempty[acc], acc_phase ^ 1, abort)) {
                     raise(P, abort, kErrTimeoutMma);
@@ -308,7 +331,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                     return false;
                 }
                 tc_fence_after();
-                const uint32_t d = tmem_base + static_cast<uint32_t>(acc * kAccCols);
+                const uint32_t d = tmem_base + static_cast<uint32_t>(acc * kBN);
                 const uint32_t dlow = kDrop ? d + kBN : d;
                 bool more = true;         // low-rank steps may follow
                 uint32_t have_low = kDrop ? 0u : 1u;  // the low-rank accumulator holds something
@@ -340,7 +363,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                     }
                     tc_fence_after();
                     const uint64_t adesc = make_sw128_kmajor_desc(smem_u32(sA + stage * kABytes));
-                    const uint32_t sb = smem_u32(sB + stage * S::kBBytes);
+                    const uint32_t sb = smem_u32(sB + stage * kBBytes);
                     const uint64_t bdesc = P.w_nmajor ? make_sw128_mnmajor_desc(sb, 8192)
                                                       : make_sw128_kmajor_desc(sb);
                     const uint32_t bstep = P.w_nmajor ? 128 : 2;  // 16 inner elements further
@@ -350,7 +373,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                                       (kb | kk) != 0 ? 1u : 0u);
                     any_issued = true;
                     umma_commit_pair(&empty[stage]);
-                    if (++stage == S::kStages) {
+                    if (++stage == kStages) {
                         stage = 0;
                         phase ^= 1;
                     }
@@ -367,94 +390,117 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             }
         }
     } else if (warp < 2 + kEpiWarps) {
-        // ---------------- epilogue (warps 2..5, both CTAs) ----------------
-        const int q = warp & 3;  // TMEM lane quadrant this warp may access
+        // ---------------- epilogue (warps 2..9, both CTAs) ----------------
+        const int q = warp & 3;              // TMEM lane quadrant this warp may access
+        const int part = (warp - 2) >> 2;    // its 128 columns of the tile
         int64_t unit = 0;
         const DropoutKeys key(kDrop ? dropout_key(P.drop) : 0);
         T *out = static_cast<T *>(P.out);
+        // the whole warp has read its accumulator rows: one arrive per warp on CTA 0
+        auto release = [&](int acc) {
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive_remote(map_to_rank(smem_u32(&tempty[acc]), 0));
+        };
         tiles(P, [&](int tm, int tn) {
-            const int acc = static_cast<int>(unit & 1);
-            const uint32_t acc_phase = static_cast<uint32_t>((unit >> 1) & 1);
-            const int slot = static_cast<int>(unit & 3);
+            const int acc = static_cast<int>(unit % kBuffers);
+            const uint32_t acc_phase = static_cast<uint32_t>((unit / kBuffers) & 1);
+            const int slot = static_cast<int>(unit % kFixSlots);
             ++unit;
-            if (!mbar_wait(&tfull[acc], acc_phase, abort)) {
-                raise(P, abort, kErrTimeoutEpilogue);
-                return false;
-            }
-            tc_fence_after();
             const int64_t row = int64_t(tm) * kBM + int64_t(rank) * kHalf + q * 32 + lane;
-            const bool fixup = fix[slot] != 0;
-            const bool has_low = !kDrop || (row < P.rows && P.index.at(row) >= 0);
-            const uint32_t tbase = tmem_base + (static_cast<uint32_t>(q * 32) << 16) +
-                                   static_cast<uint32_t>(acc * kAccCols);
-#pragma unroll 1
-            for (int c = 0; c < kBN / 32; ++c) {
-                const int64_t col0 = int64_t(tn) * kBN + c * 32;
-                if (col0 >= P.cols) break;  // the same for the whole warp
-                uint32_t v[32];
-                float *y = reinterpret_cast<float *>(v);
-                tmem_ld_32x32b_x32(tbase + c * 32, v);
-                if constexpr (kDrop) {
-                    uint32_t low[32];
-                    tmem_ld_32x32b_x32(tbase + kBN + c * 32, low);
-                    tmem_wait_ld();
+            const int64_t first = int64_t(tn) * kBN + part * kHalf;
+            uint32_t keep[kHalf / 32];  // with dropout: which columns take the low-rank term
+            if constexpr (kDrop) {
+                const bool has_low = row < P.rows && P.index.at(row) >= 0;
+#pragma unroll
+                for (int c = 0; c < kHalf / 32; ++c) {
+                    uint32_t w = 0;
                     if (has_low) {
-                        float *l = reinterpret_cast<float *>(low);
-                        if (fixup) add_nonfinite<T>(P, row, col0, l);
 #pragma unroll
                         for (int b = 0; b < 4; ++b) {
                             const uint4 bits =
                                 dropout_bits(P.drop, key, static_cast<uint32_t>(row),
-                                             static_cast<uint32_t>(col0 >> 3) + b);
+                                             static_cast<uint32_t>(first >> 3) + 4 * c + b);
 #pragma unroll
                             for (int j = 0; j < 8; ++j)
-                                if (dropout_kept(bits, j, P.drop.cut)) y[8 * b + j] += l[8 * b + j];
+                                w |= static_cast<uint32_t>(dropout_kept(bits, j, P.drop.cut))
+                                     << (8 * b + j);
                         }
                     }
-                } else {
-                    tmem_wait_ld();
-                    if (fixup && row < P.rows) add_nonfinite<T>(P, row, col0, y);
-                }
-                if (row < P.rows) {
-                    T *dst = out + row * P.ldo + col0;
-                    if (P.vec && col0 + 32 <= P.cols) {
-                        uint32_t pk[16];
-#pragma unroll
-                        for (int j = 0; j < 16; ++j) pk[j] = pack2<T>(y[2 * j], y[2 * j + 1]);
-#pragma unroll
-                        for (int j = 0; j < 4; ++j)
-                            reinterpret_cast<uint4 *>(dst)[j] =
-                                make_uint4(pk[4 * j], pk[4 * j + 1], pk[4 * j + 2], pk[4 * j + 3]);
-                    } else {
-#pragma unroll
-                        for (int j = 0; j < 32; ++j)
-                            if (col0 + j < P.cols) dst[j] = from_float<T>(y[j]);
-                    }
+                    keep[c] = w;
                 }
             }
-            // the whole warp has read its accumulator rows: one arrive per warp on CTA 0
-            tc_fence_before();
+            if (!mbar_wait(&tfull[acc], acc_phase, abort)) {
+                raise(P, abort, kErrTimeoutEpilogue);
+                return false;
+            }
             __syncwarp();
-            if (lane == 0) mbar_arrive_remote(map_to_rank(smem_u32(&tempty[acc]), 0));
+            tc_fence_after();
+            const bool fixup = fix[slot] != 0;
+            const uint32_t tbase = tmem_base + (static_cast<uint32_t>(q * 32) << 16) +
+                                   static_cast<uint32_t>(acc * kBN + part * kHalf);
+            T *dst = out + row * P.ldo + first;
+            if constexpr (kDrop) {
+                uint32_t pk[kHalf / 32][16];
+#pragma unroll
+                for (int c = 0; c < kHalf / 16; ++c) {
+                    uint32_t v[16], low[16];
+                    tmem_ld_32x32b_x16(tbase + c * 16, v);
+                    tmem_ld_32x32b_x16(tbase + kBN + c * 16, low);
+                    tmem_wait_ld();
+                    float *y = reinterpret_cast<float *>(v), *l = reinterpret_cast<float *>(low);
+                    if (fixup && row < P.rows) add_nonfinite<T>(P, row, first + c * 16, l);
+#pragma unroll
+                    for (int j = 0; j < 16; ++j)
+                        if ((keep[c >> 1] >> (16 * (c & 1) + j)) & 1) y[j] += l[j];
+#pragma unroll
+                    for (int j = 0; j < 8; ++j)
+                        pk[c >> 1][8 * (c & 1) + j] = pack2<T>(y[2 * j], y[2 * j + 1]);
+                }
+                release(acc);
+#pragma unroll
+                for (int c = 0; c < kHalf / 32; ++c)
+                    store32<T>(P, dst, row, first + c * 32, c, pk[c]);
+            } else {
+#pragma unroll 1
+                for (int c = 0; c < kHalf / 32; ++c) {
+                    uint32_t v[32], pk[16];
+                    float *y = reinterpret_cast<float *>(v);
+                    tmem_ld_32x32b_x32(tbase + c * 32, v);
+                    tmem_wait_ld();
+                    if (fixup && row < P.rows) {
+                        add_nonfinite<T>(P, row, first + c * 32, y);
+                        add_nonfinite<T>(P, row, first + c * 32 + 16, y + 16);
+                    }
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) pk[j] = pack2<T>(y[2 * j], y[2 * j + 1]);
+                    store32<T>(P, dst, row, first + c * 32, c, pk);
+                }
+                release(acc);
+            }
             return true;
         });
     } else {
-        // ---------------- loaders of the low-rank steps (warps 6..9, both CTAs) ----------------
+        // ---------------- loaders of the low-rank steps (warps 10..13, both CTAs) ----------------
         const int lt = threadIdx.x - 32 * (2 + kEpiWarps);
         const uint32_t lfull0 = map_to_rank(smem_u32(lfull), 0);
         int64_t unit = 0;
         uint32_t phase = 0;
         int turn = 0;
-        const T *F = static_cast<const T *>(P.F.p);
+        const uint16_t *F = static_cast<const uint16_t *>(P.F.p);
+        asm volatile("griddepcontrol.wait;" ::: "memory");  // the projection is complete
         tiles(P, [&](int tm, int tn) {
-            const int slot = static_cast<int>(unit & 3);
+            const int slot = static_cast<int>(unit % kFixSlots);
+            // Cleared half a round ahead: the other CTA's loaders may raise the flag of the next
+            // tile already, and the epilogue is past the tile that used this slot before.
+            if (lt == 0) fix[(unit + kFixSlots / 2) % kFixSlots] = 0;
             ++unit;
             const int64_t row0 = int64_t(tm) * kBM + lt;  // this thread's rows of the pair's tile
             const int i0 = row0 < P.rows ? P.index.at(row0) : -1;
             const int i1 = row0 + kHalf < P.rows ? P.index.at(row0 + kHalf) : -1;
             const int mine = rank ? i1 : i0;
             const int64_t row = row0 + int64_t(rank) * kHalf;
-            if (lt == 0) fix[slot] = 0;
+            const int64_t col = int64_t(tn) * kBN + int64_t(rank) * kHalf + lt;
             int cur = -1;
             while (true) {
                 // the next adapter in increasing order: the smallest index above `cur`
@@ -473,31 +519,44 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                     float p[kRankStep], f[kRankStep];
                     bool odd = false;
                     const float *prow = P.P + row * P.r + j0;
+                    const bool take = mine == cur;
+#pragma unroll
+                    for (int j = 0; j < kRankStep; j += 4) {
+                        float4 w = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                        if (P.pvec) {  // r is a multiple of 4
+                            if (take && j < nj) w = *reinterpret_cast<const float4 *>(prow + j);
+                        } else if (take) {
+                            if (j < nj) w.x = prow[j];
+                            if (j + 1 < nj) w.y = prow[j + 1];
+                            if (j + 2 < nj) w.z = prow[j + 2];
+                            if (j + 3 < nj) w.w = prow[j + 3];
+                        }
+                        p[j] = w.x, p[j + 1] = w.y, p[j + 2] = w.z, p[j + 3] = w.w;
+                    }
+                    const uint16_t *src = F + cur * P.F.ss + col * P.F.sc + j0 * P.F.sr;
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const int n = col < P.cols ? nj - 8 * h : 0;
+                        uint4 w = make_uint4(0, 0, 0, 0);
+                        if (P.fvec && n >= 8) {
+                            w = __ldg(reinterpret_cast<const uint4 *>(src + 8 * h));
+                        } else {
+                            uint32_t u[4] = {0, 0, 0, 0};
+#pragma unroll
+                            for (int e = 0; e < 8; ++e)
+                                if (e < n)
+                                    u[e >> 1] |= static_cast<uint32_t>(__ldg(src + (8 * h + e) * P.F.sr))
+                                                 << (16 * (e & 1));
+                            w = make_uint4(u[0], u[1], u[2], u[3]);
+                        }
+                        unpack8<T>(w, *reinterpret_cast<float(*)[8]>(&f[8 * h]));
+                    }
 #pragma unroll
                     for (int j = 0; j < kRankStep; ++j)
-                        p[j] = mine == cur && j < nj ? prow[j] : 0.0f;
-                    // columns of this CTA's half and, for the check alone, of the other half
-#pragma unroll
-                    for (int h = 0; h < kBN / kLoaders; ++h) {
-                        const int local = h == 0 ? lt : lt + kLoaders;
-                        const int half = local / S::kCols;  // 0: own, 1: the other CTA's
-                        const int64_t col = int64_t(tn) * kBN +
-                                            (half ^ static_cast<int>(rank)) * S::kCols +
-                                            local % S::kCols;
-                        const T *src = F + cur * P.F.ss + col * P.F.sc + j0 * P.F.sr;
-                        float g[kRankStep];
-#pragma unroll
-                        for (int j = 0; j < kRankStep; ++j)
-                            g[j] = col < P.cols && j < nj ? to_float(src[j * P.F.sr]) : 0.0f;
-#pragma unroll
-                        for (int j = 0; j < kRankStep; ++j) {
-                            if (!finite(g[j])) {
-                                odd = true;
-                                g[j] = 0.0f;
-                            }
-                            if (h == 0) f[j] = g[j];
+                        if (!finite(f[j])) {
+                            odd = true;
+                            f[j] = 0.0f;
                         }
-                    }
                     float lo[kRankStep];
 #pragma unroll
                     for (int j = 0; j < kRankStep; ++j) {
@@ -519,11 +578,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                             make_float4(p[4 * c], p[4 * c + 1], p[4 * c + 2], p[4 * c + 3]);
                         *swizzled(sP, lt, 4 + c) =
                             make_float4(lo[4 * c], lo[4 * c + 1], lo[4 * c + 2], lo[4 * c + 3]);
-                        if (lt < S::kCols)
-                            *swizzled(sF, lt, c) =
-                                make_float4(f[4 * c], f[4 * c + 1], f[4 * c + 2], f[4 * c + 3]);
+                        *swizzled(sF, lt, c) =
+                            make_float4(f[4 * c], f[4 * c + 1], f[4 * c + 2], f[4 * c + 3]);
                     }
-                    if (odd) fix[slot] = 1;
+                    if (odd)  // in both CTAs: a row of one meets columns of the other
+                        for (uint32_t c = 0; c < 2; ++c)
+                            store_flag(map_to_rank(smem_u32(const_cast<const int *>(&fix[slot])), c));
                     if (lt == 0) *message = (nj + 7) / 8;
                     fence_proxy_async_smem();
                     if (loader_sync_or(gave_up)) return false;
@@ -561,10 +621,9 @@ constexpr uint32_t idesc(int type, int n, bool b_nmajor) {
            (static_cast<uint32_t>(kBM >> 4) << 24);
 }
 
-template <typename T, int kBN, bool kDrop>
+template <typename T, bool kDrop>
 cudaError_t launch(const CUtensorMap &tmM, const CUtensorMap &tmW, const Params &P,
                    cudaStream_t stream) {
-    using S = Shape<kBN>;
     // per device: pairs that fit at once (0: not asked yet)
     constexpr int kMaxDev = 64;
     static std::atomic<int> capacity[kMaxDev];
@@ -572,16 +631,16 @@ cudaError_t launch(const CUtensorMap &tmM, const CUtensorMap &tmW, const Params 
     cudaError_t e = cudaGetDevice(&dev);
     if (e != cudaSuccess) return e;
     if (dev < 0 || dev >= kMaxDev) return cudaErrorInvalidDevice;
-    auto kernel = lr_gemm_kernel<T, kBN, kDrop>;
+    auto kernel = lr_gemm_kernel<T, kDrop>;
     int pairs = capacity[dev].load(std::memory_order_acquire);
     if (pairs == 0) {
         e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                 static_cast<int>(S::kSmem));
+                                 static_cast<int>(kSmem));
         if (e != cudaSuccess) return e;
         cudaLaunchConfig_t cfg = {};
         cfg.gridDim = dim3(2 * 1024);
         cfg.blockDim = dim3(kThreads);
-        cfg.dynamicSmemBytes = S::kSmem;
+        cfg.dynamicSmemBytes = kSmem;
         cudaLaunchAttribute attr;
         attr.id = cudaLaunchAttributeClusterDimension;
         attr.val.clusterDim.x = 2;
@@ -595,25 +654,33 @@ cudaError_t launch(const CUtensorMap &tmM, const CUtensorMap &tmW, const Params 
         capacity[dev].store(pairs, std::memory_order_release);
     }
     const int64_t grid = P.total < pairs ? P.total : pairs;
-    kernel<<<static_cast<unsigned>(2 * grid), kThreads, S::kSmem, stream>>>(tmM, tmW, P);
-    return cudaGetLastError();
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(static_cast<unsigned>(2 * grid));
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = kSmem;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr;  // (the cluster's shape is the kernel's own)
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kernel, tmM, tmW, P);
 }
 
 template <typename T>
 cudaError_t expand(const ExpandOperands &o, int *err, cudaStream_t stream) {
-    const int bn = o.drop.cut ? 128 : 256;
     Params P;
     std::memset(&P, 0, sizeof(P));
     P.rows = o.rows;
     P.cols = o.cols;
     P.num_kb = static_cast<int>((o.inner + kBK - 1) / kBK);
     P.tiles_m = static_cast<int>((o.rows + kBM - 1) / kBM);
-    P.tiles_n = static_cast<int>((o.cols + bn - 1) / bn);
+    P.tiles_n = static_cast<int>((o.cols + kBN - 1) / kBN);
     P.total = int64_t(P.tiles_m) * P.tiles_n;
     P.w_nmajor = o.W.s0 != 1;
     const int type = std::is_same<T, __half>::value ? 0 : 1;
-    P.idesc16 = idesc(type, bn, P.w_nmajor);
-    P.idesc32 = idesc(2, bn, false);
+    P.idesc16 = idesc(type, kBN, P.w_nmajor);
+    P.idesc32 = idesc(2, kBN, false);
     P.P = o.P;
     P.r = o.r;
     P.F = o.F;
@@ -622,14 +689,15 @@ cudaError_t expand(const ExpandOperands &o, int *err, cudaStream_t stream) {
     P.out = o.out;
     P.ldo = o.ldo;
     P.vec = o.ldo % 8 == 0 && (reinterpret_cast<uintptr_t>(o.out) & 15) == 0;
+    P.pvec = o.r % 4 == 0 && (reinterpret_cast<uintptr_t>(o.P) & 15) == 0;
+    P.fvec = factor_mode(o.F) == kFR;
     P.err = err;
     CUtensorMap tmM, tmW;
     if (!make_map16(&tmM, o.M.p, o.inner, o.rows, o.M.s0, kBK, kHalf)) return cudaErrorInvalidValue;
     if (P.w_nmajor ? !make_map16(&tmW, o.W.p, o.cols, o.inner, o.W.s0, 64, kBK)
-                   : !make_map16(&tmW, o.W.p, o.inner, o.cols, o.W.s1, kBK, bn / 2))
+                   : !make_map16(&tmW, o.W.p, o.inner, o.cols, o.W.s1, kBK, kHalf))
         return cudaErrorInvalidValue;
-    return o.drop.cut ? launch<T, 128, true>(tmM, tmW, P, stream)
-                      : launch<T, 256, false>(tmM, tmW, P, stream);
+    return o.drop.cut ? launch<T, true>(tmM, tmW, P, stream) : launch<T, false>(tmM, tmW, P, stream);
 }
 
 }  // namespace
