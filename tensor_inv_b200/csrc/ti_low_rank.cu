@@ -172,7 +172,7 @@ int backward(const ti_low_rank_t &op, const Gradient &g, Arena &arena, int sms, 
     const Matrix16 dY = readable(Matrix16{g.dY, g.sdy0, g.sdy1}, op.t, op.n, arena, sms, st);
     const Matrix16 X = readable(Matrix16{op.x, op.sx0, op.sx1}, op.t, op.k, arena, sms, st);
     const Matrix16 Wt = readable_w(Matrix16{op.w, op.sw1, op.sw0}, op.n, op.k, arena, sms, st);
-    const WgradPlan plan = lr_wgrad_plan(op.t, op.r, op.s, op.k, op.n, index.p != nullptr);
+    const WgradPlan plan = lr_wgrad_plan(op.t, op.r, op.s, op.k, op.n, index.p != nullptr && op.s > 1);
     void *lists = arena.take(plan.list_bytes);
     float *part_a = plan.part_a ? static_cast<float *>(arena.take(plan.part_a)) : nullptr;
     float *part_b = plan.part_b ? static_cast<float *>(arena.take(plan.part_b)) : nullptr;

@@ -10,10 +10,11 @@
 // (An infinity in M meets both parts, so its column comes out infinite or NaN.)
 //
 //   lists  one CTA per adapter writes the positions of its rows, in order, so that an adapter's rows
-//          are consecutive; no atomics, so the sums have one order.
-//   wgrad  a CTA takes a chunk of that order and 512 columns (64 per warp).  A thread reads 16
-//          bytes of a row -- 8 columns that are the same fragment position of 8 MMAs -- so M goes
-//          from memory to registers with the dropout mask applied on the way.  Where a chunk
+//          are consecutive; no atomics, so the sums have one order.  A single adapter needs none.
+//   wgrad  a CTA takes a chunk of that order and 512 columns, 64 per warp.  Each warp keeps its own
+//          ring of asynchronous copies (16 rows x 128 bytes a step, four steps ahead) and waits for
+//          no other warp; a thread reads 16 bytes of a row from it -- 8 columns that are the same
+//          fragment position of 8 MMAs -- and applies the dropout mask there.  Where a chunk
 //          crosses from one adapter to the next it writes its sums to another slot: chunk + adapter
 //          numbers the (chunk, adapter) pairs that occur without gaps in either direction.
 //   join   adds an adapter's slots in order and rounds once.  One chunk needs no join.
@@ -24,7 +25,10 @@ namespace ti {
 namespace {
 
 constexpr int kThreads = 256, kWarpCols = 64, kCtaCols = 8 * kWarpCols;
-constexpr int kStage = 64;  // rows of V in shared memory at a time
+constexpr int kStage = 128;        // rows of V in shared memory at a time
+constexpr int kStep = 16;          // rows of M per copy step
+constexpr int kRing = 5;           // steps in a warp's ring: four on their way, one being read
+constexpr int kStepBytes = kStep * 128;
 
 struct Side {
     const void *M;
@@ -40,6 +44,7 @@ struct Side {
 struct WgradParams {
     Side side[2];
     int64_t rows, r, s;
+    RowIndex index;         // of a single adapter: rows of others are left out
     const int32_t *order;   // row numbers grouped by adapter, or null: all rows, adapter 0
     const int32_t *start;   // [s + 1] first position of each adapter, or null
     int64_t chunk;
@@ -62,47 +67,59 @@ __device__ __forceinline__ void mma_tf32(float (&d)[4], const float (&a)[4], flo
           "r"(__float_as_uint(a[3])), "r"(__float_as_uint(b0)), "r"(__float_as_uint(b1)));
 }
 
+// 16 bytes to shared memory, of which the first `bytes` are read and the others become zero.
+__device__ __forceinline__ void copy16(uint32_t dst, const void *src, int bytes) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes)
+                 : "memory");
+}
+
 // order[] and start[]: rows grouped by adapter, ascending within one.  CTA s compacts the rows of
-// adapter s behind those of smaller adapters, which it counts in the same pass.
+// adapter s behind those of smaller adapters, which it counts first; up to 8192 indices stay in
+// registers between the two passes.
 __global__ void __launch_bounds__(1024) lists_kernel(RowIndex index, int64_t rows, int32_t *order,
                                                      int32_t *start) {
-    __shared__ int64_t below_sum;
-    __shared__ int warp_n[32], warp_below[32];
+    constexpr int kHeld = 8;
+    __shared__ int warp_sum[32];
     const int s = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    // first pass: how many rows belong to smaller adapters
+    int held[kHeld];
     int below = 0;
-    for (int64_t t = threadIdx.x; t < rows; t += 1024) {
+#pragma unroll
+    for (int h = 0; h < kHeld; ++h) {
+        const int64_t t = int64_t(h) * 1024 + threadIdx.x;
+        held[h] = t < rows ? index.at(t) : -1;
+    }
+#pragma unroll
+    for (int h = 0; h < kHeld; ++h) below += held[h] >= 0 && held[h] < s;
+    for (int64_t t = int64_t(kHeld) * 1024 + threadIdx.x; t < rows; t += 1024) {
         const int i = index.at(t);
         below += i >= 0 && i < s;
     }
     below = __reduce_add_sync(0xFFFFFFFFu, below);
-    if (lane == 0) warp_below[warp] = below;
+    if (lane == 0) warp_sum[warp] = below;
     __syncthreads();
-    if (threadIdx.x == 0) {
-        int64_t n = 0;
-        for (int w = 0; w < 32; ++w) n += warp_below[w];
-        below_sum = n;
-        start[s] = static_cast<int32_t>(n);
-    }
+    int at = __reduce_add_sync(0xFFFFFFFFu, warp_sum[lane]);
+    if (threadIdx.x == 0) start[s] = at;
     __syncthreads();
-    // second pass: its own rows, 1024 at a time
-    int64_t at = below_sum;
-    for (int64_t t0 = 0; t0 < rows; t0 += 1024) {
-        const int64_t t = t0 + threadIdx.x;
-        const bool own = t < rows && index.at(t) == s;
+    // its own rows, 1024 at a time
+    auto place = [&](int64_t t, bool own) {
         const unsigned ballot = __ballot_sync(0xFFFFFFFFu, own);
-        if (lane == 0) warp_n[warp] = __popc(ballot);
+        if (lane == 0) warp_sum[warp] = __popc(ballot);
         __syncthreads();
-        int before = 0, all = 0;
-        for (int w = 0; w < 32; ++w) {
-            before += w < warp ? warp_n[w] : 0;
-            all += warp_n[w];
-        }
+        const int n = warp_sum[lane];
+        const int before = __reduce_add_sync(0xFFFFFFFFu, lane < warp ? n : 0);
+        const int all = __reduce_add_sync(0xFFFFFFFFu, n);
         if (own) order[at + before + __popc(ballot & ((1u << lane) - 1))] = static_cast<int32_t>(t);
         at += all;
         __syncthreads();
+    };
+#pragma unroll
+    for (int h = 0; h < kHeld; ++h)
+        if (int64_t(h) * 1024 < rows) place(int64_t(h) * 1024 + threadIdx.x, held[h] == s);
+    for (int64_t t0 = int64_t(kHeld) * 1024; t0 < rows; t0 += 1024) {
+        const int64_t t = t0 + threadIdx.x;
+        place(t, t < rows && index.at(t) == s);
     }
-    if (s == gridDim.x - 1 && threadIdx.x == 0) start[s + 1] = static_cast<int32_t>(at);
+    if (s == gridDim.x - 1 && threadIdx.x == 0) start[s + 1] = at;
 }
 
 // Accumulators of one warp: 16*kNJ ranks x 64 columns.  In MMA i, column n of the instruction is
@@ -139,11 +156,18 @@ __device__ __forceinline__ void store_sums(const WgradParams &P, const Side &S,
         }
 }
 
+template <int kNJ>
+constexpr size_t wgrad_smem() {
+    return size_t(8) * kRing * kStepBytes + sizeof(float) * kStage * (16 * kNJ + 8) +
+           sizeof(int32_t) * kStage;
+}
+
 template <typename T, int kNJ>
 __global__ void __launch_bounds__(kThreads, 2) wgrad_kernel(const __grid_constant__ WgradParams P) {
     constexpr int kVStride = 16 * kNJ + 8;  // floats: the 4 x 8 fragment reads hit all 32 banks
-    __shared__ float vhi[kStage][kVStride], vlo[kStage][kVStride];
-    __shared__ int32_t srow[kStage];
+    extern __shared__ __align__(128) uint8_t smem[];
+    float(*sv)[kVStride] = reinterpret_cast<float(*)[kVStride]>(smem + 8 * kRing * kStepBytes);
+    int32_t *srow = reinterpret_cast<int32_t *>(sv + kStage);
     const int which = blockIdx.x < static_cast<unsigned>(P.side[0].blocks) ? 0 : 1;
     const Side &S = P.side[which];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, tq = lane & 3;
@@ -170,6 +194,8 @@ __global__ void __launch_bounds__(kThreads, 2) wgrad_kernel(const __grid_constan
     }
     const int64_t col = c0 + 8 * g;
     const uint16_t *M = static_cast<const uint16_t *>(S.M);
+    const uint8_t *ring_ptr = smem + warp * kRing * kStepBytes;
+    const uint32_t ring = smem_u32(ring_ptr);
     for (; s < P.s && (direct || pos < stop); ++s) {
         const int64_t seg_end = P.start ? min(stop, int64_t(P.start[s + 1])) : stop;
         float acc[kNJ][8][4];
@@ -183,71 +209,98 @@ __global__ void __launch_bounds__(kThreads, 2) wgrad_kernel(const __grid_constan
         for (int64_t b = pos; b < seg_end; b += kStage) {
             const int n = static_cast<int>(min(int64_t(kStage), seg_end - b));
             __syncthreads();  // the previous stage has been read
-            if (threadIdx.x < kStage)
-                srow[threadIdx.x] = static_cast<int>(threadIdx.x) >= n ? -1
-                                    : P.order ? P.order[b + threadIdx.x]
-                                              : static_cast<int32_t>(b + threadIdx.x);
+            if (threadIdx.x < kStage) {
+                int t = -1;
+                if (static_cast<int>(threadIdx.x) < n) {
+                    t = P.order ? P.order[b + threadIdx.x] : static_cast<int32_t>(b + threadIdx.x);
+                    if (!P.order && P.index.at(t) != 0) t = -1;
+                }
+                srow[threadIdx.x] = t;
+            }
             __syncthreads();
+            const int steps = (n + kStep - 1) / kStep;
+            // A lane copies chunk lane % 8 of four of a step's rows.  Chunk c of row q lies at
+            // c ^ 2 (q % 4): the 16-byte reads below then hit all banks.
+            auto issue = [&](int step) {
+                if (step < steps) {
+#pragma unroll
+                    for (int h = 0; h < 4; ++h) {
+                        const int q = (lane >> 3) + 4 * h, c = lane & 7;
+                        const int t = srow[step * kStep + q];
+                        const int64_t left = S.cols - (c0 + 8 * c);
+                        const int bytes =
+                            t < 0 || left <= 0 ? 0 : left >= 8 ? 16 : static_cast<int>(2 * left);
+                        copy16(ring + (step % kRing) * kStepBytes + q * 128 +
+                                   ((c ^ ((q & 3) << 1)) << 4),
+                               M + (bytes ? t * S.ld + c0 + 8 * c : 0), bytes);
+                    }
+                }
+                asm volatile("cp.async.commit_group;" ::: "memory");
+            };
+            for (int k = 0; k < kRing - 1; ++k) issue(k);
             for (int e = threadIdx.x; e < kStage * 16 * kNJ; e += kThreads) {
                 const int q = e / (16 * kNJ), j = e % (16 * kNJ);
                 const int t = srow[q];
-                const float v = t >= 0 && j0 + j < P.r ? S.V[int64_t(t) * P.r + j0 + j] : 0.0f;
-                // infinities and NaN stay whole in the upper part
-                const uint32_t bits = __float_as_uint(v);
-                const bool odd = (bits & 0x7F800000u) == 0x7F800000u;
-                const float hi = odd ? v : __uint_as_float(bits & 0xFFFFE000u);
-                vhi[q][j] = hi;
-                vlo[q][j] = odd ? 0.0f : v - hi;
+                sv[q][j] = t >= 0 && j0 + j < P.r ? S.V[int64_t(t) * P.r + j0 + j] : 0.0f;
             }
             __syncthreads();
-            if (c0 >= S.cols) continue;
-            // rows q + 4*h + tq of a step of 16; the next step's rows are read ahead
-            uint4 x[4];
-            auto fetch = [&](int q, uint4(&v)[4]) {
-#pragma unroll
-                for (int h = 0; h < 4; ++h) {
-                    const int t = srow[q + 4 * h + tq];
-                    v[h] = t >= 0 ? load8(M + t * S.ld + col, S.cols - col) : make_uint4(0, 0, 0, 0);
-                }
-            };
-            fetch(0, x);
 #pragma unroll 1
-            for (int q = 0; q < n; q += 16) {
-                uint4 next[4];
-                if (q + 16 < n) fetch(q + 16, next);
+            for (int k = 0; k < steps; ++k) {
+                asm volatile("cp.async.wait_group %0;" ::"n"(kRing - 2) : "memory");
+                __syncwarp();
+                const int q = k * kStep;
+                const uint8_t *src = ring_ptr + (k % kRing) * kStepBytes;
+                uint4 x[4];
+#pragma unroll
+                for (int h = 0; h < 4; ++h)
+                    x[h] = *reinterpret_cast<const uint4 *>(src + (4 * h + tq) * 128 +
+                                                            ((g ^ (tq << 1)) << 4));
+                __syncwarp();
+                issue(k + kRing - 1);  // into the slot read in the step before
                 if (S.drop.cut) {
 #pragma unroll
-                    for (int h = 0; h < 4; ++h) {
+                    for (int h = 0; h < 4; ++h)
                         x[h] = masked(x[h], S.drop, key,
                                       static_cast<uint32_t>(srow[q + 4 * h + tq]),
                                       static_cast<uint32_t>(col >> 3));
-                    }
                 }
 #pragma unroll
-                for (int k = 0; k < 2; ++k) {  // two steps of 8 rows
-                    const int q0 = q + 8 * k + tq;
-                    const uint32_t m0[4] = {x[2 * k].x, x[2 * k].y, x[2 * k].z, x[2 * k].w};
-                    const uint32_t m1[4] = {x[2 * k + 1].x, x[2 * k + 1].y, x[2 * k + 1].z,
-                                            x[2 * k + 1].w};
+                for (int k8 = 0; k8 < 2; ++k8) {  // two steps of 8 rows
+                    const int q0 = q + 8 * k8 + tq;
+                    const uint4 &xa = x[2 * k8], &xb = x[2 * k8 + 1];
+                    const uint32_t m0[4] = {xa.x, xa.y, xa.z, xa.w};
+                    const uint32_t m1[4] = {xb.x, xb.y, xb.z, xb.w};
 #pragma unroll
                     for (int nj = 0; nj < kNJ; ++nj) {
                         const int j = 16 * nj + g;
-                        const float ahi[4] = {vhi[q0][j], vhi[q0][j + 8], vhi[q0 + 4][j],
-                                              vhi[q0 + 4][j + 8]};
-                        const float alo[4] = {vlo[q0][j], vlo[q0][j + 8], vlo[q0 + 4][j],
-                                              vlo[q0 + 4][j + 8]};
+                        float hi[4] = {sv[q0][j], sv[q0][j + 8], sv[q0 + 4][j], sv[q0 + 4][j + 8]};
+                        float lo[4];
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            // infinities and NaN stay whole in the upper part
+                            const uint32_t bits = __float_as_uint(hi[e]);
+                            const bool odd = (bits & 0x7F800000u) == 0x7F800000u;
+                            const float up = __uint_as_float(bits & 0xFFFFE000u);
+                            lo[e] = odd ? 0.0f : hi[e] - up;
+                            hi[e] = odd ? hi[e] : up;
+                        }
 #pragma unroll
                         for (int i = 0; i < 8; ++i) {
                             const float b0 = half_of<T>(m0[i >> 1], i & 1);
                             const float b1 = half_of<T>(m1[i >> 1], i & 1);
-                            mma_tf32(acc[nj][i], ahi, b0, b1);
-                            mma_tf32(acc[nj][i], alo, b0, b1);
+                            mma_tf32(acc[nj][i], hi, b0, b1);
+                        }
+                        // (apart from the first eight, which they would have to wait for)
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) {
+                            const float b0 = half_of<T>(m0[i >> 1], i & 1);
+                            const float b1 = half_of<T>(m1[i >> 1], i & 1);
+                            mma_tf32(acc[nj][i], lo, b0, b1);
                         }
                     }
                 }
-#pragma unroll
-                for (int h = 0; h < 4; ++h) x[h] = next[h];
             }
+            asm volatile("cp.async.wait_group 0;" ::: "memory");
         }
         if (seg_end > pos || direct)
             store_sums<T, kNJ>(P, S, acc, int64_t(blockIdx.y) + s, s, c0, j0, g, tq);
@@ -257,8 +310,9 @@ __global__ void __launch_bounds__(kThreads, 2) wgrad_kernel(const __grid_constan
 
 // out[s][c][j] = the sum of adapter s's slots, in order.
 template <typename T>
-__global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ WgradParams P, int which) {
-    const Side &S = P.side[which];
+__global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ WgradParams P) {
+    const Side &S = P.side[blockIdx.y];
+    if (!S.part) return;
     const int64_t ldc = (S.cols + 7) / 8 * 8;
     const int64_t total = P.start ? P.start[P.s] : P.rows;
     const int64_t quads = (S.cols + 3) / 4;
@@ -287,16 +341,16 @@ __global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ Wgrad
 
 }  // namespace
 
-// Chunks of rows: one wave of two CTAs per SM, so that the partial sums, which are written and
+// Chunks of rows: one wave of CTAs, two per SM, so that the partial sums, which are written and
 // read once for each chunk, stay few.
 WgradPlan lr_wgrad_plan(int64_t rows, int64_t r, int64_t s, int64_t cols_a, int64_t cols_b,
                         bool indexed) {
-    constexpr int64_t kCtas = 2 * 148;  // fixed: the workspace is sized without a device
+    constexpr int64_t kCtas = 296;  // fixed: the workspace is sized without a device
     WgradPlan p{};
     const int64_t blocks = ((cols_a + kCtaCols - 1) / kCtaCols + (cols_b + kCtaCols - 1) / kCtaCols) *
                            (r <= 16 ? 1 : (r + 31) / 32);
     int64_t chunks = blocks ? kCtas / blocks : 1;
-    const int64_t most = (rows + kStage - 1) / kStage;
+    const int64_t most = (rows + 63) / 64;  // 64 rows are worth a chunk
     if (chunks > most) chunks = most;
     if (chunks < 1) chunks = 1;
     p.chunk = (rows + chunks - 1) / chunks;
@@ -320,16 +374,17 @@ static cudaError_t wgrad(const WgradParams &P, const WgradPlan &plan, int num_sm
     const int nj = P.r <= 16 ? 1 : 2;
     const dim3 grid(static_cast<unsigned>(blocks), static_cast<unsigned>(plan.chunks),
                     static_cast<unsigned>((P.r + 16 * nj - 1) / (16 * nj)));
-    if (nj == 1)
-        wgrad_kernel<T, 1><<<grid, kThreads, 0, stream>>>(P);
-    else
-        wgrad_kernel<T, 2><<<grid, kThreads, 0, stream>>>(P);
-    for (int w = 0; w < 2; ++w)
-        if (P.side[w].part) {
-            const int64_t work = P.s * P.r * ((P.side[w].cols + 3) / 4);
-            const int64_t want = (work + 255) / 256, most = int64_t(num_sms) * 8;
-            join_kernel<T><<<static_cast<unsigned>(want < most ? want : most), 256, 0, stream>>>(P, w);
-        }
+    auto kernel = nj == 1 ? wgrad_kernel<T, 1> : wgrad_kernel<T, 2>;
+    const size_t smem = nj == 1 ? wgrad_smem<1>() : wgrad_smem<2>();
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                               static_cast<int>(smem));
+    if (e != cudaSuccess) return e;
+    kernel<<<grid, kThreads, smem, stream>>>(P);
+    if (plan.chunks > 1) {
+        const int64_t cols = P.side[0].cols > P.side[1].cols ? P.side[0].cols : P.side[1].cols;
+        const int64_t want = (P.s * P.r * ((cols + 3) / 4) + 255) / 256, most = int64_t(num_sms) * 4;
+        join_kernel<T><<<dim3(static_cast<unsigned>(want < most ? want : most), 2), 256, 0, stream>>>(P);
+    }
     return cudaGetLastError();
 }
 
@@ -349,7 +404,8 @@ cudaError_t lr_wgrad(bool half, const WgradOperand &a, const WgradOperand &b, in
                          o.ss,  o.sc,   o.sr,   blocks};
     }
     if (P.side[0].blocks + P.side[1].blocks == 0) return cudaSuccess;
-    if (index.p) {
+    P.index = index;
+    if (index.p && index.s > 1) {
         int32_t *start = static_cast<int32_t *>(lists);
         int32_t *order = start + index.s + 1;
         lists_kernel<<<static_cast<unsigned>(index.s), 1024, 0, stream>>>(index, rows, order, start);
