@@ -139,7 +139,7 @@ cudaError_t project_expand(bool half, const ProjectOperands &p, const ExpandOper
     const cudaError_t e = lr_project(half, p, sms, err, st);
     if (e != cudaSuccess || !x) return e;
     if (!x->inner) return clear(x->out, x->ldo, x->rows, x->cols, st);
-    return x->rows <= kExpandRowsLimit ? lr_expand_rows(half, *x, sms, err, st)
+    return x->rows <= expand_rows_limit(x->index.s) ? lr_expand_rows(half, *x, sms, err, st)
                                        : lr_expand_pairs(half, *x, err, st);
 }
 

@@ -69,7 +69,8 @@ struct Params {
     Dropout drop;
     void *out;
     int64_t ldo;
-    int vec;        // rows of out are 16-byte aligned
+    int align;      // bytes to which the rows of out are aligned: 16, 8, 4 or 2
+    int stages;     // of the ring: kStages, or one less where the epilogue takes its space
     int pvec, fvec; // P's rows in vectors of 4, F's in vectors of 8 along the rank
     int *err;
 };
@@ -190,23 +191,46 @@ __device__ __forceinline__ void store_flag(uint32_t addr) {
     asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(addr), "r"(1) : "memory");
 }
 
-// Stores 32 packed columns of a row, as far as they exist.
+// Stores a warp's 32 rows x 32 packed columns (lane = row), as far as they exist.  Rows that are
+// not 16-byte aligned would leave in pieces of 8, 4 or 2 bytes, 32 rows at a time; they go through
+// `turn` (32 rows of 17 words, this warp's own) instead, so that a store covers consecutive bytes.
 template <typename T>
-__device__ __forceinline__ void store32(const Params &P, T *row_dst, int64_t row, int64_t col0, int c,
-                                        const uint32_t (&pk)[16]) {
-    if (row >= P.rows || col0 >= P.cols) return;
-    T *dst = row_dst + 32 * c;
-    if (P.vec && col0 + 32 <= P.cols) {
+__device__ __forceinline__ void store_block(const Params &P, T *out, uint32_t *turn, int64_t row0,
+                                            int64_t col0, int lane, const uint32_t (&pk)[16]) {
+    if (col0 >= P.cols) return;  // the same for the whole warp
+    if (P.align == 16) {
+        const int64_t row = row0 + lane;
+        if (row >= P.rows) return;
+        T *dst = out + row * P.ldo + col0;
+        if (col0 + 32 <= P.cols) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-            reinterpret_cast<uint4 *>(dst)[j] =
-                make_uint4(pk[4 * j], pk[4 * j + 1], pk[4 * j + 2], pk[4 * j + 3]);
-    } else {
-        uint16_t *d = reinterpret_cast<uint16_t *>(dst);
+            for (int j = 0; j < 4; ++j)
+                reinterpret_cast<uint4 *>(dst)[j] =
+                    make_uint4(pk[4 * j], pk[4 * j + 1], pk[4 * j + 2], pk[4 * j + 3]);
+        } else {
+            uint16_t *d = reinterpret_cast<uint16_t *>(dst);
 #pragma unroll
-        for (int j = 0; j < 32; ++j)
-            if (col0 + j < P.cols) d[j] = static_cast<uint16_t>(pk[j >> 1] >> (16 * (j & 1)));
+            for (int j = 0; j < 32; ++j)
+                if (col0 + j < P.cols) d[j] = static_cast<uint16_t>(pk[j >> 1] >> (16 * (j & 1)));
+        }
+        return;
     }
+#pragma unroll
+    for (int j = 0; j < 16; ++j) turn[lane * 17 + j] = pk[j];
+    __syncwarp();
+    const int rows = static_cast<int>(min(int64_t(32), P.rows - row0));
+    if (P.align >= 4 && col0 + 32 <= P.cols) {  // words: two rows at a time
+        uint32_t *dst = reinterpret_cast<uint32_t *>(out + row0 * P.ldo + col0) + (lane & 15);
+#pragma unroll 4
+        for (int r = lane >> 4; r < rows; r += 2) dst[r * (P.ldo >> 1)] = turn[r * 17 + (lane & 15)];
+    } else {
+        uint16_t *dst = reinterpret_cast<uint16_t *>(out + row0 * P.ldo + col0) + lane;
+        const uint16_t *src = reinterpret_cast<const uint16_t *>(turn) + lane;
+        if (col0 + lane < P.cols)
+#pragma unroll 4
+            for (int r = 0; r < rows; ++r) dst[r * P.ldo] = src[r * 34];
+    }
+    __syncwarp();
 }
 
 template <typename T, bool kDrop>
@@ -293,7 +317,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                     }
                     issued_mask |= 1u << stage;
                     issued_phase = (issued_phase & ~(1u << stage)) | (phase << stage);
-                    if (++stage == kStages) {
+                    if (++stage == P.stages) {
                         stage = 0;
                         phase ^= 1;
                     }
@@ -373,7 +397,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                                       (kb | kk) != 0 ? 1u : 0u);
                     any_issued = true;
                     umma_commit_pair(&empty[stage]);
-                    if (++stage == kStages) {
+                    if (++stage == P.stages) {
                         stage = 0;
                         phase ^= 1;
                     }
@@ -396,6 +420,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         int64_t unit = 0;
         const DropoutKeys key(kDrop ? dropout_key(P.drop) : 0);
         T *out = static_cast<T *>(P.out);
+        // (the last stage of the ring, which such calls do without)
+        uint32_t *turn = reinterpret_cast<uint32_t *>(sA + (kStages - 1) * kABytes) + (warp - 2) * 32 * 17;
         // the whole warp has read its accumulator rows: one arrive per warp on CTA 0
         auto release = [&](int acc) {
             tc_fence_before();
@@ -439,7 +465,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             const bool fixup = fix[slot] != 0;
             const uint32_t tbase = tmem_base + (static_cast<uint32_t>(q * 32) << 16) +
                                    static_cast<uint32_t>(acc * kBN + part * kHalf);
-            T *dst = out + row * P.ldo + first;
             if constexpr (kDrop) {
                 uint32_t pk[kHalf / 32][16];
 #pragma unroll
@@ -460,7 +485,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                 release(acc);
 #pragma unroll
                 for (int c = 0; c < kHalf / 32; ++c)
-                    store32<T>(P, dst, row, first + c * 32, c, pk[c]);
+                    store_block<T>(P, out, turn, row - lane, first + c * 32, lane, pk[c]);
             } else {
 #pragma unroll 1
                 for (int c = 0; c < kHalf / 32; ++c) {
@@ -474,7 +499,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                     }
 #pragma unroll
                     for (int j = 0; j < 16; ++j) pk[j] = pack2<T>(y[2 * j], y[2 * j + 1]);
-                    store32<T>(P, dst, row, first + c * 32, c, pk);
+                    store_block<T>(P, out, turn, row - lane, first + c * 32, lane, pk);
                 }
                 release(acc);
             }
@@ -688,7 +713,9 @@ cudaError_t expand(const ExpandOperands &o, int *err, cudaStream_t stream) {
     P.drop = o.drop;
     P.out = o.out;
     P.ldo = o.ldo;
-    P.vec = o.ldo % 8 == 0 && (reinterpret_cast<uintptr_t>(o.out) & 15) == 0;
+    const uintptr_t bits = reinterpret_cast<uintptr_t>(o.out) | static_cast<uintptr_t>(2 * o.ldo) | 16;
+    P.align = static_cast<int>(bits & (~bits + 1));
+    P.stages = P.align == 16 ? kStages : kStages - 1;
     P.pvec = o.r % 4 == 0 && (reinterpret_cast<uintptr_t>(o.P) & 15) == 0;
     P.fvec = factor_mode(o.F) == kFR;
     P.err = err;
