@@ -7,8 +7,11 @@ returns ``TI_ERR_NO_DEVICE`` unless an sm_100 device is current.
 
 from __future__ import annotations
 
+import contextlib
 import ctypes
 from pathlib import Path
+
+import torch
 
 LIB_PATH = Path(__file__).resolve().parent / "libtensor_inv_crt.so"
 
@@ -275,3 +278,17 @@ def low_rank_workspace_size(op: LowRank, dY=None) -> int:
               lib().ti_low_rank_backward_workspace_size(ctypes.byref(op), dY.data_ptr(),
                                                         *dY.stride(), ctypes.byref(out)))
     return out.value
+
+
+def stream_ptr(index: int) -> int:
+    """The current stream of a CUDA device as a number (torch.cuda.current_stream builds an object
+    for it, which takes longer than a small kernel)."""
+    return torch._C._cuda_getCurrentRawStream(index)
+
+
+_here = contextlib.nullcontext()
+
+
+def on_device(index: int):
+    """A context with that device current; nothing is done where it is already."""
+    return _here if torch.cuda.current_device() == index else torch.cuda.device(index)

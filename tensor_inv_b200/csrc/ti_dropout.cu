@@ -7,11 +7,9 @@
 // them; the four blocks' copies and rounds overlap.
 #include "tensor_inv_crt.h"
 #include "ti_common.cuh"
-#include "ti_low_rank.cuh"
+#include "ti_lr_launch.cuh"
 
 namespace ti {
-
-int device_context(int *num_sms, int **err);
 
 namespace {
 
@@ -180,7 +178,7 @@ extern "C" int ti_dropout(int dtype, const void *X, int64_t sx0, int64_t sx1, vo
     if (drop->cut < 0 || drop->cut > 65536 || ldy < cols) return TI_ERR_INVALID_ARGUMENT;
     if (rows >= int64_t(1) << 32 || cols >= int64_t(1) << 34) return TI_ERR_UNSUPPORTED;
     int sms = 0, *err = nullptr;
-    const int rc = device_context(&sms, &err);
+    const int rc = low_rank_context(&sms, &err);
     if (rc != TI_OK) return rc;
     if (rows == 0 || cols == 0) return TI_OK;
     if (!X || !Y) return TI_ERR_INVALID_ARGUMENT;

@@ -204,6 +204,23 @@ bool bad_workspace(const void *ws, size_t have, size_t need) {
 }
 
 }  // namespace
+
+int low_rank_context(int *num_sms, int **err) {
+    static PerDevice<int> sms;
+    static PerDevice<int *> words;
+    std::atomic<int> *n = sms.here();
+    std::atomic<int *> *w = words.here();
+    if (!n || !w) return TI_ERR_NO_DEVICE;
+    *err = w->load(std::memory_order_acquire);
+    *num_sms = n->load(std::memory_order_acquire);
+    if (*err && *num_sms) return TI_OK;
+    const int rc = device_context(num_sms, err);
+    if (rc != TI_OK) return rc;
+    n->store(*num_sms, std::memory_order_release);
+    w->store(*err, std::memory_order_release);
+    return TI_OK;
+}
+
 }  // namespace ti
 
 using namespace ti;
@@ -239,7 +256,7 @@ int ti_low_rank_matmul(const ti_low_rank_t *op, void *Y, int64_t ldy, float *P, 
     int rc = ti_low_rank_workspace_size(op, &need);
     if (rc != TI_OK) return rc;
     int sms = 0, *err = nullptr;
-    if ((rc = device_context(&sms, &err)) != TI_OK) return rc;
+    if ((rc = low_rank_context(&sms, &err)) != TI_OK) return rc;
     if (op->t == 0) return TI_OK;
     if ((op->k && (!op->x || !op->a || (op->n && !op->w))) || (op->n && (!op->b || !Y)) ||
         ldy < op->n)
@@ -257,7 +274,7 @@ int ti_low_rank_backward(const ti_low_rank_t *op, const void *dY, int64_t sdy0, 
     int rc = ti_low_rank_backward_workspace_size(op, dY, sdy0, sdy1, &need);
     if (rc != TI_OK) return rc;
     int sms = 0, *err = nullptr;
-    if ((rc = device_context(&sms, &err)) != TI_OK) return rc;
+    if ((rc = low_rank_context(&sms, &err)) != TI_OK) return rc;
     if ((op->k && !op->a) || (op->n && !op->b) ||
         (op->t && ((op->k && !op->x) || (op->n && !dY) || (op->k && op->n && dX && !op->w) ||
                    (dB && !P))))

@@ -649,18 +649,14 @@ constexpr uint32_t idesc(int type, int n, bool b_nmajor) {
 template <typename T, bool kDrop>
 cudaError_t launch(const CUtensorMap &tmM, const CUtensorMap &tmW, const Params &P,
                    cudaStream_t stream) {
-    // per device: pairs that fit at once (0: not asked yet)
-    constexpr int kMaxDev = 64;
-    static std::atomic<int> capacity[kMaxDev];
-    int dev = 0;
-    cudaError_t e = cudaGetDevice(&dev);
-    if (e != cudaSuccess) return e;
-    if (dev < 0 || dev >= kMaxDev) return cudaErrorInvalidDevice;
     auto kernel = lr_gemm_kernel<T, kDrop>;
-    int pairs = capacity[dev].load(std::memory_order_acquire);
+    static PerDevice<int> capacity;  // pairs that fit at once
+    std::atomic<int> *known = capacity.here();
+    if (!known) return cudaErrorInvalidDevice;
+    int pairs = known->load(std::memory_order_acquire);
     if (pairs == 0) {
-        e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                 static_cast<int>(kSmem));
+        cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                             static_cast<int>(kSmem));
         if (e != cudaSuccess) return e;
         cudaLaunchConfig_t cfg = {};
         cfg.gridDim = dim3(2 * 1024);
@@ -676,7 +672,7 @@ cudaError_t launch(const CUtensorMap &tmM, const CUtensorMap &tmW, const Params 
         e = cudaOccupancyMaxActiveClusters(&pairs, kernel, &cfg);
         if (e != cudaSuccess) return e;
         if (pairs < 1) return cudaErrorNotSupported;
-        capacity[dev].store(pairs, std::memory_order_release);
+        known->store(pairs, std::memory_order_release);
     }
     const int64_t grid = P.total < pairs ? P.total : pairs;
     cudaLaunchConfig_t cfg = {};

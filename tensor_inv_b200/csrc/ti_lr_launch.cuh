@@ -3,9 +3,28 @@
 
 #include <cuda.h>
 
+#include <atomic>
+
 #include "ti_low_rank.cuh"
 
 namespace ti {
+
+// One word per device, zero at first: what a launcher has set up or found out there.  Threads that
+// race on the first call of a device do the same work twice, which is harmless.
+template <typename T>
+struct PerDevice {
+    static constexpr int kMaxDev = 64;
+    std::atomic<T> word[kMaxDev] = {};
+    // the current device's word, or null
+    std::atomic<T> *here() {
+        int dev = 0;
+        if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDev) return nullptr;
+        return &word[dev];
+    }
+};
+
+// SM count and error word of the current device (asked for once per device); a TI_* status.
+int low_rank_context(int *num_sms, int **err);
 
 // Tensor map of a matrix of 16-bit elements, `outer` rows of `inner` contiguous ones `ld` apart,
 // 128-byte swizzle; base and rows 16-byte aligned.

@@ -504,17 +504,23 @@ __global__ void __launch_bounds__(kRowThreads, 3)
         }
 }
 
+// Launches a kernel in clusters of `parts`; `ready` is the kernel's own.
 template <typename K, typename... Args>
-cudaError_t launch_cluster(K kernel, int parts, dim3 grid, int threads, size_t smem,
-                           cudaStream_t stream, const Args &...args) {
-    // (Repeated settings are cheap and keep no state per device.)  An SM whose shared memory is
-    // carved out small would have to drain before the expanding kernel's CTAs fit beside this one.
-    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout,
-                                         cudaSharedmemCarveoutMaxShared);
-    if (e == cudaSuccess && smem > 48 * 1024)
-        e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                 static_cast<int>(smem));
-    if (e != cudaSuccess) return e;
+cudaError_t launch_cluster(K kernel, PerDevice<int> &ready, int parts, dim3 grid, int threads,
+                           size_t smem, cudaStream_t stream, const Args &...args) {
+    std::atomic<int> *set = ready.here();
+    if (!set) return cudaErrorInvalidDevice;
+    if (!set->load(std::memory_order_acquire)) {
+        // An SM whose shared memory is carved out small would have to drain before the
+        // expanding kernel's CTAs fit beside this one.
+        cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout,
+                                             cudaSharedmemCarveoutMaxShared);
+        if (e == cudaSuccess && smem > 48 * 1024)
+            e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                     static_cast<int>(smem));
+        if (e != cudaSuccess) return e;
+        set->store(1, std::memory_order_release);
+    }
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = grid;
     cfg.blockDim = dim3(threads);
@@ -588,10 +594,11 @@ cudaError_t project_tiles(const ProjectOperands &o, int num_sms, int *err, cudaS
         !make_factor_map(&tmF, o.F, mode, o.cols, o.r, P.one_adapter ? 1 : o.index.s, P.rp))
         return cudaErrorInvalidValue;
     const dim3 grid(static_cast<unsigned>(parts * tile_count), static_cast<unsigned>(blocks));
-    return o.drop.cut ? launch_cluster(project_tiles_kernel<T, true>, parts, grid, kTileThreads,
-                                       kTileSmem, stream, tmM, tmF, P)
-                      : launch_cluster(project_tiles_kernel<T, false>, parts, grid, kTileThreads,
-                                       kTileSmem, stream, tmM, tmF, P);
+    static PerDevice<int> ready[2];
+    return o.drop.cut ? launch_cluster(project_tiles_kernel<T, true>, ready[1], parts, grid,
+                                       kTileThreads, kTileSmem, stream, tmM, tmF, P)
+                      : launch_cluster(project_tiles_kernel<T, false>, ready[0], parts, grid,
+                                       kTileThreads, kTileSmem, stream, tmM, tmF, P);
 }
 
 template <typename T>
@@ -604,10 +611,11 @@ cudaError_t project(const ProjectOperands &o, int num_sms, int *err, cudaStream_
     while (parts < 8 && P.cols > 1024 * parts) ++parts;
     P.slice = ((P.cols + parts - 1) / parts + 255) / 256 * 256;
     const dim3 grid(static_cast<unsigned>(parts * P.rows));
-    return P.drop.cut ? launch_cluster(project_rows_kernel<T, true>, parts, grid, kRowThreads, 0,
-                                       stream, P)
-                      : launch_cluster(project_rows_kernel<T, false>, parts, grid, kRowThreads, 0,
-                                       stream, P);
+    static PerDevice<int> ready[2];
+    return P.drop.cut ? launch_cluster(project_rows_kernel<T, true>, ready[1], parts, grid,
+                                       kRowThreads, 0, stream, P)
+                      : launch_cluster(project_rows_kernel<T, false>, ready[0], parts, grid,
+                                       kRowThreads, 0, stream, P);
 }
 
 }  // namespace

@@ -406,17 +406,14 @@ cudaError_t launch(const CUtensorMap &tmM, const CUtensorMap &tmW, const Params 
                    int ranks, cudaStream_t stream) {
     using S = Shape<kNT>;
     auto kernel = lr_rows_kernel<T, kNT, kDrop>;
-    constexpr int kMaxDev = 64;
-    static std::atomic<int> configured[kMaxDev];
-    int dev = 0;
-    cudaError_t e = cudaGetDevice(&dev);
-    if (e != cudaSuccess) return e;
-    if (dev < 0 || dev >= kMaxDev) return cudaErrorInvalidDevice;
-    if (!configured[dev].load(std::memory_order_acquire)) {
-        e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                 static_cast<int>(S::kSmem));
+    static PerDevice<int> ready;
+    std::atomic<int> *set = ready.here();
+    if (!set) return cudaErrorInvalidDevice;
+    if (!set->load(std::memory_order_acquire)) {
+        const cudaError_t e = cudaFuncSetAttribute(
+            kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(S::kSmem));
         if (e != cudaSuccess) return e;
-        configured[dev].store(1, std::memory_order_release);
+        set->store(1, std::memory_order_release);
     }
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(static_cast<unsigned>(tiles * ranks));

@@ -376,9 +376,15 @@ static cudaError_t wgrad(const WgradParams &P, const WgradPlan &plan, int num_sm
                     static_cast<unsigned>((P.r + 16 * nj - 1) / (16 * nj)));
     auto kernel = nj == 1 ? wgrad_kernel<T, 1> : wgrad_kernel<T, 2>;
     const size_t smem = nj == 1 ? wgrad_smem<1>() : wgrad_smem<2>();
-    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                               static_cast<int>(smem));
-    if (e != cudaSuccess) return e;
+    static PerDevice<int> ready[2];
+    std::atomic<int> *set = ready[nj - 1].here();
+    if (!set) return cudaErrorInvalidDevice;
+    if (!set->load(std::memory_order_acquire)) {
+        const cudaError_t e = cudaFuncSetAttribute(
+            kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+        if (e != cudaSuccess) return e;
+        set->store(1, std::memory_order_release);
+    }
     kernel<<<grid, kThreads, smem, stream>>>(P);
     if (plan.chunks > 1) {
         const int64_t cols = P.side[0].cols > P.side[1].cols ? P.side[0].cols : P.side[1].cols;

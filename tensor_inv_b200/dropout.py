@@ -23,29 +23,28 @@ _TYPE_CODES = {
 }
 
 
-def drop_spec(p, seed, offset, device) -> nat.DropoutSpec:
-    """ti_dropout_spec_t of (p, seed, offset); a seed tensor must outlive the launch."""
-    if isinstance(p, torch.Tensor) or not isinstance(p, numbers.Real) or not 0.0 <= p <= 1.0:
+def drop_numbers(p, seed, offset, device):
+    """The fields (cut, seed, seed_ptr, offset) of ti_dropout_spec_t; a seed tensor must outlive the
+    launch."""
+    if type(p) is not float and not isinstance(p, numbers.Real) or not 0.0 <= p <= 1.0:
         raise ValueError(f"dropout probability must be a number in [0, 1], got {p!r}")
-    spec = nat.DropoutSpec()
-    spec.cut = round(65536 * float(p))
-    if not isinstance(offset, numbers.Integral) or not 0 <= offset < 2**64:
+    cut = round(65536 * float(p))
+    if type(offset) is not int and not isinstance(offset, numbers.Integral) or \
+            not 0 <= offset < 2**64:
         raise ValueError(f"offset must be an integer in [0, 2^64), got {offset!r}")
-    spec.offset = int(offset)
     if seed is None:
-        if spec.cut:
+        if cut:
             raise ValueError("dropout needs a seed: an integer or a one-element int64 CUDA tensor")
-    elif isinstance(seed, torch.Tensor):
+        return cut, 0, None, int(offset)
+    if type(seed) is not int and isinstance(seed, torch.Tensor):
         if seed.dtype != torch.int64 or seed.numel() != 1 or seed.device != device:
             raise ValueError(f"a seed tensor must be one int64 on {device}, got {seed.dtype} "
                              f"{tuple(seed.shape)} on {seed.device}")
-        spec.seed_ptr = seed.data_ptr()
-    elif isinstance(seed, numbers.Integral) and 0 <= seed < 2**64:
-        spec.seed = int(seed)
-    else:
+        return cut, 0, seed.data_ptr(), int(offset)
+    if type(seed) is not int and not isinstance(seed, numbers.Integral) or not 0 <= seed < 2**64:
         raise ValueError(f"seed must be an integer in [0, 2^64) or a one-element int64 CUDA "
                          f"tensor, got {seed!r}")
-    return spec
+    return cut, int(seed), None, int(offset)
 
 
 def refuse_capture(what):
@@ -58,21 +57,21 @@ def refuse_capture(what):
 
 
 def _dropout(X, p, seed, offset):
-    spec = drop_spec(p, seed, offset, X.device)
+    numbers_ = drop_numbers(p, seed, offset, X.device)
     if not X.is_cuda:
         raise ValueError("dropout takes a CUDA tensor; it has no CPU path")
-    out = torch.empty(X.shape, dtype=X.dtype, device=X.device)
+    out = X.new_empty(X.shape)
     if X.numel() == 0:
         return out
-    flat = X.reshape(-1, X.shape[-1])  # a view where the strides allow it
+    flat = X if X.dim() == 2 else X.reshape(-1, X.shape[-1])  # a view where the strides allow it
     rows, cols = flat.shape
     if rows >= 2**32 or cols >= 2**34:
         raise ValueError(f"dropout counts rows in 32 bits and columns in 34: {rows} x {cols}")
-    with torch.cuda.device(X.device):
-        st = nat.lib().ti_dropout(_TYPE_CODES[X.dtype], flat.data_ptr(), flat.stride(0),
-                                  flat.stride(1), out.data_ptr(), cols, rows, cols,
-                                  ctypes.byref(spec),
-                                  torch.cuda.current_stream(X.device).cuda_stream)
+    index = X.get_device()
+    with nat.on_device(index):
+        st = nat.lib().ti_dropout(_TYPE_CODES[X.dtype], flat.data_ptr(), *flat.stride(),
+                                  out.data_ptr(), cols, rows, cols,
+                                  ctypes.byref(nat.DropoutSpec(*numbers_)), nat.stream_ptr(index))
     nat.check("ti_dropout", st)
     return out
 

@@ -19,15 +19,14 @@ import numbers
 import torch
 
 from . import _native as nat
-from .dropout import drop_spec, refuse_capture
+from .dropout import drop_numbers, refuse_capture
 
 _TYPE_CODES = {torch.float16: nat.TI_TYPE_F16, torch.bfloat16: nat.TI_TYPE_BF16}
 MAX_RANK = 256
 
 
-def _describe(X, W, A, B, index, scale, alpha, p, seed, offset):
-    """Checks the operands and describes them as a ti_low_rank_t.  Returns it and the tensors
-    that it points into (they must outlive the launch)."""
+def _refuse(X, W, A, B):
+    """Says what is wrong with the types, shapes or devices of the operands (if anything is)."""
     tensors = {"X": X, "W": W, "A": A, "B": B}
     for name, M in tensors.items():
         if not isinstance(M, torch.Tensor) or M.dtype not in _TYPE_CODES:
@@ -49,60 +48,73 @@ def _describe(X, W, A, B, index, scale, alpha, p, seed, offset):
         raise ValueError(f"one adapter or more of rank 1 to {MAX_RANK}, got S = {S}, r = {r}")
     if max(T, K, N, S) >= 2**31:
         raise ValueError("low_rank_matmul takes dimensions below 2^31")
+
+
+def _describe(X, W, A, B, index, scale, alpha, p, seed, offset):
+    """Checks the operands and describes them as a ti_low_rank_t.  Returns it and the tensors
+    that it points into (they must outlive the launch)."""
+    try:  # the usual case in one look; what is wrong, if anything, is found out below
+        (T, K), (K1, N), (S, K2, r), (S1, r1, N1) = X.shape, W.shape, A.shape, B.shape
+        dtype, at = X.dtype, X.get_device()
+        fits = (K1 == K and K2 == K and S1 == S and r1 == r and N1 == N and 1 <= r <= MAX_RANK and
+                1 <= S < 2**31 and T < 2**31 and K < 2**31 and N < 2**31 and
+                dtype in _TYPE_CODES and W.dtype is dtype and A.dtype is dtype and
+                B.dtype is dtype and
+                at == W.get_device() == A.get_device() == B.get_device())
+    except (AttributeError, TypeError, ValueError):
+        fits = False
+    if not fits:
+        _refuse(X, W, A, B)
+        raise ValueError("low_rank_matmul: operands do not fit together")
     if index is None:
         if S != 1:
             raise ValueError(f"{S} adapters need an index that says which one each row takes")
+        index_ptr, index_bytes = None, 0
     else:
-        if not isinstance(index, torch.Tensor) or index.dtype not in (torch.int32, torch.int64):
+        if not isinstance(index, torch.Tensor) or index.dtype not in (torch.int64, torch.int32):
             raise TypeError("index must be an int32 or int64 tensor")
-        if index.shape != (T,) or index.device != X.device:
+        if index.dim() != 1 or len(index) != T or index.get_device() != at:
             raise ValueError(f"index must have shape ({T},) on {X.device}, got "
                              f"{tuple(index.shape)} on {index.device}")
         index = index.contiguous()
-    if scale is not None:
-        if not isinstance(scale, torch.Tensor) or scale.dtype != torch.float32:
+        index_ptr, index_bytes = index.data_ptr(), index.element_size()
+    if scale is None:
+        scale_ptr = None
+    else:
+        if not isinstance(scale, torch.Tensor) or scale.dtype is not torch.float32:
             raise TypeError("scale must be a float32 tensor (one factor for all adapters: alpha)")
-        if scale.shape != (S,) or scale.device != X.device:
+        if scale.dim() != 1 or len(scale) != S or scale.get_device() != at:
             raise ValueError(f"scale must have shape ({S},) on {X.device}, got "
                              f"{tuple(scale.shape)} on {scale.device}")
-        scale = scale.detach().contiguous()
-    if not isinstance(alpha, numbers.Real):
+        scale = scale.contiguous()
+        scale_ptr = scale.data_ptr()
+    if type(alpha) is not float and not isinstance(alpha, numbers.Real):
         raise TypeError("alpha must be a number")
-    drop = drop_spec(p, seed, offset, X.device)
-    if not X.is_cuda:
+    drop = drop_numbers(p, seed, offset, X.device)
+    if at < 0:
         raise ValueError("low_rank_matmul takes CUDA tensors; it has no CPU path")
-    op = nat.LowRank()
-    op.dtype = _TYPE_CODES[X.dtype]
-    op.t, op.k, op.n, op.s, op.r = T, K, N, S, r
-    op.x, op.w, op.a, op.b = (M.data_ptr() for M in (X, W, A, B))
-    op.sx0, op.sx1 = X.stride()
-    op.sw0, op.sw1 = W.stride()
-    op.sa0, op.sa1, op.sa2 = A.stride()
-    op.sb0, op.sb1, op.sb2 = B.stride()
-    if index is not None:
-        op.index, op.index_bytes = index.data_ptr(), index.element_size()
-    op.scale = None if scale is None else scale.data_ptr()
-    op.alpha = float(alpha)
-    op.drop = drop
+    op = nat.LowRank(_TYPE_CODES[dtype], T, K, N, S, r, X.data_ptr(), *X.stride(), W.data_ptr(),
+                     *W.stride(), A.data_ptr(), *A.stride(), B.data_ptr(), *B.stride(), index_ptr,
+                     index_bytes, scale_ptr, alpha, drop)
     return op, (X, W, A, B, index, scale, seed)
 
 
-def _workspace(op, device, dY=None):
-    return torch.empty(max(nat.low_rank_workspace_size(op, dY), 256), dtype=torch.uint8,
-                       device=device)
+def _workspace(op, X, dY=None):
+    return X.new_empty(max(nat.low_rank_workspace_size(op, dY), 256), dtype=torch.uint8)
 
 
 def _forward(X, W, A, B, index, scale, alpha, p, seed, offset, want_p):
     op, keep = _describe(X, W, A, B, index, scale, alpha, p, seed, offset)
-    Y = torch.empty((op.t, op.n), dtype=X.dtype, device=X.device)
-    P = torch.empty((op.t, op.r), dtype=torch.float32, device=X.device) if want_p else None
-    if op.t == 0:
+    rows, cols, at = op.t, op.n, X.get_device()
+    Y = X.new_empty((rows, cols))
+    P = X.new_empty((rows, op.r), dtype=torch.float32) if want_p else None
+    if rows == 0:
         return Y, P
-    with torch.cuda.device(X.device):
-        ws = _workspace(op, X.device)
+    with nat.on_device(at):
+        ws = _workspace(op, X)
         st = nat.lib().ti_low_rank_matmul(
-            ctypes.byref(op), Y.data_ptr(), op.n, None if P is None else P.data_ptr(),
-            ws.data_ptr(), ws.numel(), torch.cuda.current_stream(X.device).cuda_stream)
+            ctypes.byref(op), Y.data_ptr(), cols, None if P is None else P.data_ptr(),
+            ws.data_ptr(), ws.numel(), nat.stream_ptr(at))
     nat.check("ti_low_rank_matmul", st)
     del keep
     return Y, P
@@ -130,14 +142,14 @@ def _backward(dY, X, W, A, B, index, scale, alpha, p, seed, offset, P, needs):
     # the gradients take the layout of A and B (their strides, where those are dense)
     dA = torch.empty_like(A) if want_a else None
     dB = torch.empty_like(B) if want_b else None
-    with torch.cuda.device(dev):
-        ws = _workspace(op, dev, dY)
+    with nat.on_device(dev.index):
+        ws = _workspace(op, X, dY)
         st = nat.lib().ti_low_rank_backward(
             ctypes.byref(op), dY.data_ptr(), *dY.stride(), None if P is None else P.data_ptr(),
             None if dX is None else dX.data_ptr(), op.k,
             *((None, 0, 0, 0) if dA is None else (dA.data_ptr(), *dA.stride())),
             *((None, 0, 0, 0) if dB is None else (dB.data_ptr(), *dB.stride())),
-            ws.data_ptr(), ws.numel(), torch.cuda.current_stream(dev).cuda_stream)
+            ws.data_ptr(), ws.numel(), nat.stream_ptr(dev.index))
     nat.check("ti_low_rank_backward", st)
     del keep
     return dX, dA, dB
@@ -196,12 +208,13 @@ def low_rank_matmul(X, W, A, B, index=None, scale=None, *, alpha=1.0, p=0.0, see
     reads; ``torch.no_grad()`` code, such as a captured training step, passes it there itself.
     """
     A, B, _ = _batched(A, B)
-    grads = [M for M in (X, W, A, B, scale) if isinstance(M, torch.Tensor) and M.requires_grad]
-    if torch.is_grad_enabled() and grads:
-        if any(M is W or M is scale for M in grads):
+    if torch.is_grad_enabled() and any(getattr(M, "requires_grad", False)
+                                       for M in (X, A, B, W, scale)):
+        if any(getattr(M, "requires_grad", False) for M in (W, scale)):
             raise ValueError("W and scale are fixed in low_rank_matmul: it computes no gradient "
                              "of them (detach them)")
-        refuse_capture("low_rank_matmul")
+        if X.is_cuda:
+            refuse_capture("low_rank_matmul")
         Y, P = _LowRank.apply(X, W, A, B, index, scale, alpha, p, seed, offset)
     else:
         Y, P = _forward(X, W, A, B, index, scale, alpha, p, seed, offset, return_projection)

@@ -404,7 +404,7 @@ def test_what_lies_beside_the_output_is_left(T):
     op, keep = _describe(X, W, A, B, index, scale, 1.0, 0.0, None, 0)
     for ld in (N, N + 5, 80, 96):
         out = torch.full((T + 4, ld), 7.0, dtype=X.dtype, device="cuda")
-        ws = _workspace(op, X.device)
+        ws = _workspace(op, X)
         st = nat.lib().ti_low_rank_matmul(ctypes.byref(op), out.data_ptr(), ld, None,
                                           ws.data_ptr(), ws.numel(),
                                           torch.cuda.current_stream().cuda_stream)
