@@ -17,25 +17,56 @@ int device_context(int *num_sms, int **err);
 namespace {
 
 // dst[z][i][j] = src[z][i][j], rows of `ld` elements: operands that a copy engine cannot read (odd
-// strides or addresses) are copied once.  32 x 32 tiles through shared memory, so that both sides
-// are coalesced whichever stride of src is 1.
-__global__ void pack_kernel(Matrix16 src, int64_t batch, int64_t s_batch, int64_t rows, int64_t cols,
-                            uint16_t *dst, int64_t ld) {
-    __shared__ uint16_t tile[32][33];
-    const int64_t tiles_c = (cols + 31) / 32, tiles = (rows + 31) / 32 * tiles_c;
-    const bool turned = src.s0 == 1 && src.s1 != 1;
-    for (int64_t u = blockIdx.x; u < batch * tiles; u += gridDim.x) {
-        const int64_t z = u / tiles, r0 = u % tiles / tiles_c * 32, c0 = u % tiles_c * 32;
-        const uint16_t *s = static_cast<const uint16_t *>(src.p) + z * s_batch;
-        for (int y = threadIdx.y; y < 32; y += 8) {
-            const int64_t i = r0 + (turned ? threadIdx.x : y), j = c0 + (turned ? y : threadIdx.x);
-            if (i < rows && j < cols)
-                tile[turned ? threadIdx.x : y][turned ? y : threadIdx.x] = s[i * src.s0 + j * src.s1];
+// strides or addresses) are copied once, all of a call's in one launch.  32 x 64 tiles through
+// shared memory, so that both sides are coalesced whichever stride of src is 1.
+struct PackJob {
+    Matrix16 src;
+    int64_t batch, s_batch, rows, cols;
+    uint16_t *dst;
+    int64_t ld, first;  // the job's first tile
+};
+constexpr int kMaxJobs = 4;
+struct PackJobs {
+    PackJob job[kMaxJobs];
+    int n;
+    int64_t tiles;
+};
+
+__global__ void __launch_bounds__(256) pack_kernel(const __grid_constant__ PackJobs jobs) {
+    __shared__ uint16_t tile[32][66];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    for (int64_t u = blockIdx.x; u < jobs.tiles; u += gridDim.x) {
+        int k = 0;
+        while (k + 1 < jobs.n && u >= jobs.job[k + 1].first) ++k;
+        const PackJob &J = jobs.job[k];
+        const int64_t tiles_c = (J.cols + 63) / 64, tiles = (J.rows + 31) / 32 * tiles_c;
+        const int64_t v = u - J.first, z = v / tiles;
+        const int64_t r0 = v % tiles / tiles_c * 32, c0 = v % tiles_c * 64;
+        const uint16_t *s = static_cast<const uint16_t *>(J.src.p) + z * J.s_batch;
+        const int nr = static_cast<int>(min(int64_t(32), J.rows - r0));
+        const int nc = static_cast<int>(min(int64_t(64), J.cols - c0));
+        if (J.src.s0 == 1 && J.src.s1 != 1) {  // a warp reads columns
+            const uint16_t *p = s + r0 + lane + (c0 + warp) * J.src.s1;
+#pragma unroll
+            for (int c = 0; c < 8; ++c)
+                if (lane < nr && warp + 8 * c < nc) tile[lane][warp + 8 * c] = p[8 * c * J.src.s1];
+        } else {
+            const uint16_t *p = s + (r0 + warp) * J.src.s0 + (c0 + lane) * J.src.s1;
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+                    if (warp + 8 * r < nr && lane + 32 * h < nc)
+                        tile[warp + 8 * r][lane + 32 * h] = p[8 * r * J.src.s0 + 32 * h * J.src.s1];
         }
         __syncthreads();
-        for (int y = threadIdx.y; y < 32; y += 8)
-            if (r0 + y < rows && c0 + threadIdx.x < cols)
-                dst[(z * rows + r0 + y) * ld + c0 + threadIdx.x] = tile[y][threadIdx.x];
+        // two columns per lane; the padding behind the last column belongs to the copy
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+            if (warp + 8 * r < nr && 2 * lane < nc)
+                *reinterpret_cast<uint32_t *>(J.dst + (z * J.rows + r0 + warp + 8 * r) * J.ld + c0 +
+                                              2 * lane) =
+                    *reinterpret_cast<const uint32_t *>(&tile[warp + 8 * r][2 * lane]);
         __syncthreads();
     }
 }
@@ -63,57 +94,62 @@ int status(cudaError_t e) { return e == cudaSuccess ? TI_OK : TI_ERR_CUDA; }
 
 int64_t round8(int64_t x) { return (x + 7) / 8 * 8; }
 
-// Hands out parts of the workspace; with no base it only counts bytes.
+// Hands out parts of the workspace; with no base it only counts bytes.  Operands that the copy
+// engine cannot read are noted and packed together by pack().
 struct Arena {
     uint8_t *base;
     size_t used;
+    PackJobs jobs;
     void *take(size_t bytes) {
         void *p = base ? base + used : nullptr;
         used += align256(bytes);
         return p;
     }
+    void *packed(const Matrix16 &M, int64_t batch, int64_t s_batch, int64_t rows, int64_t cols,
+                 int64_t ld) {
+        void *dst = take(sizeof(uint16_t) * static_cast<size_t>(batch * rows * ld));
+        if (batch && rows && cols) {
+            jobs.job[jobs.n++] = PackJob{M,  batch, s_batch, rows, cols, static_cast<uint16_t *>(dst),
+                                         ld, jobs.tiles};
+            jobs.tiles += batch * ((rows + 31) / 32) * ((cols + 63) / 64);
+        }
+        return dst;
+    }
+    cudaError_t pack(int sms, cudaStream_t st) const {
+        if (!jobs.n) return cudaSuccess;
+        const int64_t most = int64_t(sms) * 8;
+        pack_kernel<<<static_cast<unsigned>(jobs.tiles < most ? jobs.tiles : most), 256, 0, st>>>(jobs);
+        return cudaGetLastError();
+    }
 };
 
-void pack(const Matrix16 &M, int64_t batch, int64_t s_batch, int64_t rows, int64_t cols, void *dst,
-          int64_t ld, int sms, cudaStream_t st) {
-    const int64_t tiles = batch * ((rows + 31) / 32) * ((cols + 31) / 32), most = int64_t(sms) * 8;
-    if (tiles)
-        pack_kernel<<<static_cast<unsigned>(tiles < most ? tiles : most), dim3(32, 8), 0, st>>>(
-            M, batch, s_batch, rows, cols, static_cast<uint16_t *>(dst), ld);
-}
-
 // The matrix as `rows` rows of contiguous elements that a copy engine can read: itself, or a
-// packed copy in the workspace (launched unless the arena only counts).
-Matrix16 readable(const Matrix16 &M, int64_t rows, int64_t cols, Arena &arena, int sms,
-                  cudaStream_t st) {
+// packed copy in the workspace.
+Matrix16 readable(const Matrix16 &M, int64_t rows, int64_t cols, Arena &arena) {
     const int64_t ld = round8(cols);
     if (copyable(M.p, rows, M.s0, M.s1, cols)) return Matrix16{M.p, rows <= 1 ? ld : M.s0, 1};
-    void *dst = arena.take(sizeof(uint16_t) * static_cast<size_t>(rows * ld));
-    if (arena.base) pack(M, 1, 0, rows, cols, dst, ld, sms, st);
-    return Matrix16{dst, ld, 1};
+    return Matrix16{arena.packed(M, 1, 0, rows, cols, ld), ld, 1};
 }
 
 // A projecting factor (s adapters, cols x r) as it is, or, where the copy engine has to read it and
 // cannot, packed in rows of one rank.
 Factor16 readable_factor(const Factor16 &F, int64_t s, int64_t cols, int64_t r, int64_t rows,
-                         Arena &arena, int sms, cudaStream_t st) {
+                         Arena &arena) {
     if (rows <= kProjectRowsLimit || factor_mode(F) != kFScalar) return F;
     const int64_t ld = round8(cols), batch = F.ss == 0 ? 1 : s;
-    void *dst = arena.take(sizeof(uint16_t) * static_cast<size_t>(batch * r * ld));
-    if (arena.base) pack(Matrix16{F.p, F.sr, F.sc}, batch, F.ss, r, cols, dst, ld, sms, st);
-    return Factor16{dst, F.ss == 0 ? 0 : r * ld, 1, ld};
+    return Factor16{arena.packed(Matrix16{F.p, F.sr, F.sc}, batch, F.ss, r, cols, ld),
+                    F.ss == 0 ? 0 : r * ld, 1, ld};
 }
 
 // W (inner x cols) with one unit stride, readable in that orientation.
-Matrix16 readable_w(const Matrix16 &W, int64_t inner, int64_t cols, Arena &arena, int sms,
-                    cudaStream_t st) {
+Matrix16 readable_w(const Matrix16 &W, int64_t inner, int64_t cols, Arena &arena) {
     if (copyable(W.p, cols, W.s1, W.s0, inner))
         return Matrix16{W.p, 1, cols <= 1 ? round8(inner) : W.s1};
     if (W.s0 == 1 && W.s1 != 1) {
-        const Matrix16 t = readable(Matrix16{W.p, W.s1, W.s0}, cols, inner, arena, sms, st);
+        const Matrix16 t = readable(Matrix16{W.p, W.s1, W.s0}, cols, inner, arena);
         return Matrix16{t.p, 1, t.s0};
     }
-    return readable(W, inner, cols, arena, sms, st);
+    return readable(W, inner, cols, arena);
 }
 
 struct Gradient {
@@ -149,11 +185,13 @@ int forward(const ti_low_rank_t &op, void *Y, int64_t ldy, float *P, Arena &aren
     const Dropout drop = device_spec(op.drop);
     float *own = static_cast<float *>(arena.take(sizeof(float) * op.t * op.r));
     if (!P) P = own;
-    const Matrix16 X = readable(Matrix16{op.x, op.sx0, op.sx1}, op.t, op.k, arena, sms, st);
-    const Matrix16 W = readable_w(Matrix16{op.w, op.sw0, op.sw1}, op.k, op.n, arena, sms, st);
+    const Matrix16 X = readable(Matrix16{op.x, op.sx0, op.sx1}, op.t, op.k, arena);
+    const Matrix16 W = readable_w(Matrix16{op.w, op.sw0, op.sw1}, op.k, op.n, arena);
     const Factor16 A = readable_factor(Factor16{op.a, op.sa0, op.sa1, op.sa2}, op.s, op.k, op.r,
-                                       op.t, arena, sms, st);
+                                       op.t, arena);
     if (!arena.base) return TI_OK;
+    const cudaError_t packed = arena.pack(sms, st);
+    if (packed != cudaSuccess) return status(packed);
     const ProjectOperands p{X,     op.t,     op.k,
                             A,
                             op.r,  index,    op.scale,
@@ -169,16 +207,21 @@ int backward(const ti_low_rank_t &op, const Gradient &g, Arena &arena, int sms, 
     const RowIndex index{op.index, op.index_bytes == 8, op.s};
     const Dropout drop = device_spec(op.drop);
     float *dP = static_cast<float *>(arena.take(sizeof(float) * op.t * op.r));
-    const Matrix16 dY = readable(Matrix16{g.dY, g.sdy0, g.sdy1}, op.t, op.n, arena, sms, st);
-    const Matrix16 X = readable(Matrix16{op.x, op.sx0, op.sx1}, op.t, op.k, arena, sms, st);
-    const Matrix16 Wt = readable_w(Matrix16{op.w, op.sw1, op.sw0}, op.n, op.k, arena, sms, st);
-    const WgradPlan plan = lr_wgrad_plan(op.t, op.r, op.s, op.k, op.n, index.p != nullptr && op.s > 1);
+    const Matrix16 dY = readable(Matrix16{g.dY, g.sdy0, g.sdy1}, op.t, op.n, arena);
+    // what a missing gradient alone would read is left alone; the size counts everything
+    Matrix16 X{}, Wt{};
+    if (!arena.base || g.dA) X = readable(Matrix16{op.x, op.sx0, op.sx1}, op.t, op.k, arena);
+    if (!arena.base || g.dX) Wt = readable_w(Matrix16{op.w, op.sw1, op.sw0}, op.n, op.k, arena);
+    const WgradPlan plan = lr_wgrad_plan(op.t, op.r, op.s, op.k, op.n,
+                                         index.p != nullptr && op.s > 1, drop.cut != 0);
     void *lists = arena.take(plan.list_bytes);
-    float *part_a = plan.part_a ? static_cast<float *>(arena.take(plan.part_a)) : nullptr;
-    float *part_b = plan.part_b ? static_cast<float *>(arena.take(plan.part_b)) : nullptr;
+    float *part_a = plan.part[0] ? static_cast<float *>(arena.take(plan.part[0])) : nullptr;
+    float *part_b = plan.part[1] ? static_cast<float *>(arena.take(plan.part[1])) : nullptr;
     const Factor16 Bt = readable_factor(Factor16{op.b, op.sb0, op.sb2, op.sb1}, op.s, op.n, op.r,
-                                        op.t, arena, sms, st);
+                                        op.t, arena);
     if (!arena.base) return TI_OK;
+    const cudaError_t packed = arena.pack(sms, st);
+    if (packed != cudaSuccess) return status(packed);
     const bool half = op.dtype == TI_TYPE_F16;
     if ((g.dX || g.dA) && op.t) {
         const ProjectOperands p{dY,    op.t,     op.n,
@@ -230,7 +273,7 @@ extern "C" {
 int ti_low_rank_workspace_size(const ti_low_rank_t *op, size_t *bytes) {
     const int rc = check_op(op);
     if (rc != TI_OK || !bytes) return rc != TI_OK ? rc : TI_ERR_INVALID_ARGUMENT;
-    Arena count{nullptr, 0};
+    Arena count{};
     forward(*op, nullptr, 0, nullptr, count, 0, nullptr, nullptr);
     *bytes = count.used;
     return TI_OK;
@@ -240,7 +283,7 @@ int ti_low_rank_backward_workspace_size(const ti_low_rank_t *op, const void *dY,
                                         int64_t sdy1, size_t *bytes) {
     const int rc = check_op(op);
     if (rc != TI_OK || !bytes) return rc != TI_OK ? rc : TI_ERR_INVALID_ARGUMENT;
-    Arena count{nullptr, 0};
+    Arena count{};
     Gradient g{};
     g.dY = dY;
     g.sdy0 = sdy0;
@@ -262,7 +305,7 @@ int ti_low_rank_matmul(const ti_low_rank_t *op, void *Y, int64_t ldy, float *P, 
         ldy < op->n)
         return TI_ERR_INVALID_ARGUMENT;
     if (bad_workspace(workspace, workspace_bytes, need)) return TI_ERR_WORKSPACE;
-    Arena arena{static_cast<uint8_t *>(workspace), 0};
+    Arena arena{static_cast<uint8_t *>(workspace), 0, {}};
     return forward(*op, Y, ldy, P, arena, sms, err, static_cast<cudaStream_t>(stream));
 }
 
@@ -284,7 +327,7 @@ int ti_low_rank_backward(const ti_low_rank_t *op, const void *dY, int64_t sdy0, 
     const Gradient g{dY, sdy0, sdy1, P, dX, lddx, dA, {sda0, sda1, sda2}, dB, {sdb0, sdb1, sdb2}};
     // a call without rows may come without a workspace: there is nothing to pack then
     alignas(256) static uint8_t none[256];
-    Arena arena{workspace ? static_cast<uint8_t *>(workspace) : none, 0};
+    Arena arena{workspace ? static_cast<uint8_t *>(workspace) : none, 0, {}};
     return backward(*op, g, arena, sms, err, static_cast<cudaStream_t>(stream));
 }
 

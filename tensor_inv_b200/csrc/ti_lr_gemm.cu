@@ -28,8 +28,9 @@
 // Roles (both CTAs): warp 0 TMA producer; warp 1 TMEM allocation and, in CTA 0, the MMA issuer;
 // warps 2..9 epilogue, two per TMEM lane quadrant with 128 columns each; warps 10..13 loaders of the
 // low-rank steps, which have their own stage, so they fill it while the product's steps run.  A
-// low-rank step is taken after every fourth step of the product while any are left: a fixed order,
-// so results repeat bit for bit.  The kernel may start before the projection has finished
+// low-rank step is taken after every `every` steps of the product while any are left: a fixed
+// order, so results repeat bit for bit, and far enough apart that the loaders are ready (8192^3,
+// r = 32, whole call: 990 us with 4, 935 us with 16).  The kernel may start before the projection has finished
 // (programmatic launch); the loaders wait for it.
 // All waits are bounded; on timeout the error word is raised and the CTA leaves its loops.
 #include <atomic>
@@ -50,7 +51,6 @@ constexpr int kLowBytes = 2 * kHalf * 128;       // one low-rank step per CTA: r
 constexpr int kEpiWarps = 8, kLoaders = 128;
 constexpr int kThreads = 64 + 32 * kEpiWarps + kLoaders;
 constexpr uint32_t kTmemCols = 512;
-constexpr int kEvery = 4;                        // product steps between two low-rank steps
 constexpr int kGroupM = 8;                       // raster: 8 row tiles (2048 rows) at a time
 constexpr int kRankStep = 16;
 constexpr int kFixSlots = 8;
@@ -59,6 +59,7 @@ constexpr size_t kSmem = size_t(kStages) * kStageBytes + kLowBytes + 1024 + 512;
 struct Params {
     int64_t rows, cols;
     int num_kb, tiles_m, tiles_n;
+    int every;      // product steps between two low-rank steps
     int64_t total;
     int w_nmajor;
     uint32_t idesc16, idesc32;
@@ -358,6 +359,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                 const uint32_t d = tmem_base + static_cast<uint32_t>(acc * kBN);
                 const uint32_t dlow = kDrop ? d + kBN : d;
                 bool more = true;         // low-rank steps may follow
+                int until = P.every;
                 uint32_t have_low = kDrop ? 0u : 1u;  // the low-rank accumulator holds something
                 // takes one low-rank step, or the loaders' word that there are no more
                 auto low_step = [&]() {
@@ -401,7 +403,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                         stage = 0;
                         phase ^= 1;
                     }
-                    if (more && kb % kEvery == kEvery - 1 && !low_step()) return false;
+                    if (more && --until == 0) {
+                        until = P.every;
+                        if (!low_step()) return false;
+                    }
                 }
                 while (more)
                     if (!low_step()) return false;
@@ -695,6 +700,9 @@ cudaError_t expand(const ExpandOperands &o, int *err, cudaStream_t stream) {
     P.rows = o.rows;
     P.cols = o.cols;
     P.num_kb = static_cast<int>((o.inner + kBK - 1) / kBK);
+    // one adapter's steps and the word that there are no more, spread over the product's steps
+    P.every = P.num_kb / static_cast<int>((o.r + kRankStep - 1) / kRankStep + 1);
+    P.every = P.every > 16 ? 16 : P.every < 2 ? 2 : P.every;
     P.tiles_m = static_cast<int>((o.rows + kBM - 1) / kBM);
     P.tiles_n = static_cast<int>((o.cols + kBN - 1) / kBN);
     P.total = int64_t(P.tiles_m) * P.tiles_n;

@@ -94,11 +94,11 @@ inline int64_t expand_rows_limit(int64_t adapters) { return adapters > 1 ? 256 :
 
 // The gradients of the adapters (ti_lr_wgrad.cu).
 struct WgradPlan {
-    int64_t chunk, chunks;
-    size_t list_bytes, part_a, part_b;  // workspace
+    int64_t chunk[2], chunks[2];      // rows per chunk and their number, for dA and dB
+    size_t list_bytes, part[2];       // workspace
 };
 WgradPlan lr_wgrad_plan(int64_t rows, int64_t r, int64_t s, int64_t cols_a, int64_t cols_b,
-                        bool indexed);
+                        bool listed, bool dropped);
 
 // out[s][c][j] = sum over adapter s's rows of m(t, c) M[t][c] V[t][j]; out null: not computed
 struct WgradOperand {

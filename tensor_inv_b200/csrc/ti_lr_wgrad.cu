@@ -38,7 +38,8 @@ struct Side {
     float *part;      // [slot][r][round8(cols)], or null: one chunk, straight to out
     void *out;
     int64_t ss, sc, sr;
-    int blocks;       // column blocks of this side; 0: not computed
+    int64_t blocks;   // column blocks of this side; 0: not computed
+    int64_t chunk, chunks;  // rows per chunk, and how many
 };
 
 struct WgradParams {
@@ -47,7 +48,6 @@ struct WgradParams {
     RowIndex index;         // of a single adapter: rows of others are left out
     const int32_t *order;   // row numbers grouped by adapter, or null: all rows, adapter 0
     const int32_t *start;   // [s + 1] first position of each adapter, or null
-    int64_t chunk;
 };
 
 template <typename T>
@@ -168,16 +168,17 @@ __global__ void __launch_bounds__(kThreads, 2) wgrad_kernel(const __grid_constan
     extern __shared__ __align__(128) uint8_t smem[];
     float(*sv)[kVStride] = reinterpret_cast<float(*)[kVStride]>(smem + 8 * kRing * kStepBytes);
     int32_t *srow = reinterpret_cast<int32_t *>(sv + kStage);
-    const int which = blockIdx.x < static_cast<unsigned>(P.side[0].blocks) ? 0 : 1;
+    const int64_t units_a = P.side[0].blocks * P.side[0].chunks;
+    const int which = blockIdx.x < units_a ? 0 : 1;
     const Side &S = P.side[which];
+    const int64_t unit = blockIdx.x - (which ? units_a : 0), chunk = unit / S.blocks;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, tq = lane & 3;
-    const int64_t c0 =
-        int64_t(blockIdx.x - (which ? P.side[0].blocks : 0)) * kCtaCols + warp * kWarpCols;
-    const int64_t j0 = int64_t(blockIdx.z) * 16 * kNJ;
+    const int64_t c0 = unit % S.blocks * kCtaCols + warp * kWarpCols;
+    const int64_t j0 = int64_t(blockIdx.y) * 16 * kNJ;
     const int64_t total = P.start ? P.start[P.s] : P.rows;
     const bool direct = S.part == nullptr;
-    int64_t pos = int64_t(blockIdx.y) * P.chunk;
-    const int64_t stop = min(total, pos + P.chunk);
+    int64_t pos = chunk * S.chunk;
+    const int64_t stop = min(total, pos + S.chunk);
     const DropoutKeys key(S.drop.cut ? dropout_key(S.drop) : 0);
 
     // the first adapter whose rows reach past pos (from the first one, where every adapter's
@@ -303,7 +304,7 @@ __global__ void __launch_bounds__(kThreads, 2) wgrad_kernel(const __grid_constan
             asm volatile("cp.async.wait_group 0;" ::: "memory");
         }
         if (seg_end > pos || direct)
-            store_sums<T, kNJ>(P, S, acc, int64_t(blockIdx.y) + s, s, c0, j0, g, tq);
+            store_sums<T, kNJ>(P, S, acc, chunk + s, s, c0, j0, g, tq);
         pos = max(pos, seg_end);
     }
 }
@@ -323,7 +324,7 @@ __global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ Wgrad
         const int64_t end = P.start ? P.start[s + 1] : s == 0 ? total : 0;
         float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
         if (end > first)
-            for (int64_t k = first / P.chunk; k <= (end - 1) / P.chunk; ++k) {
+            for (int64_t k = first / S.chunk; k <= (end - 1) / S.chunk; ++k) {
                 const float4 a =
                     *reinterpret_cast<const float4 *>(S.part + ((k + s) * P.r + j) * ldc + c);
                 v.x += a.x;
@@ -342,37 +343,37 @@ __global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ Wgrad
 }  // namespace
 
 // Chunks of rows: one wave of CTAs, two per SM, so that the partial sums, which are written and
-// read once for each chunk, stay few.
+// read once for each chunk, stay few.  The mask makes a row of dA cost about twice a row of dB
+// (4096 x 4096, r = 16: 45 us against 30 us with equal chunks), so dA's chunks are half as long then.
 WgradPlan lr_wgrad_plan(int64_t rows, int64_t r, int64_t s, int64_t cols_a, int64_t cols_b,
-                        bool indexed) {
+                        bool listed, bool dropped) {
     constexpr int64_t kCtas = 296;  // fixed: the workspace is sized without a device
     WgradPlan p{};
-    const int64_t blocks = ((cols_a + kCtaCols - 1) / kCtaCols + (cols_b + kCtaCols - 1) / kCtaCols) *
-                           (r <= 16 ? 1 : (r + 31) / 32);
-    int64_t chunks = blocks ? kCtas / blocks : 1;
-    const int64_t most = (rows + 63) / 64;  // 64 rows are worth a chunk
-    if (chunks > most) chunks = most;
-    if (chunks < 1) chunks = 1;
-    p.chunk = (rows + chunks - 1) / chunks;
-    p.chunk = (p.chunk + 15) / 16 * 16;
-    if (p.chunk == 0) p.chunk = 16;
-    p.chunks = rows ? (rows + p.chunk - 1) / p.chunk : 1;
-    const int64_t slots = p.chunks + s - 1;
-    p.list_bytes = indexed ? sizeof(int32_t) * static_cast<size_t>(rows + s + 1) : 0;
-    if (p.chunks > 1) {
-        p.part_a = sizeof(float) * static_cast<size_t>(slots * r * ((cols_a + 7) / 8 * 8));
-        p.part_b = sizeof(float) * static_cast<size_t>(slots * r * ((cols_b + 7) / 8 * 8));
+    const int64_t cols[2] = {cols_a, cols_b}, weight[2] = {dropped ? 2 : 1, 1};
+    int64_t cost = 0;
+    for (int w = 0; w < 2; ++w)
+        cost += weight[w] * ((cols[w] + kCtaCols - 1) / kCtaCols) * (r <= 16 ? 1 : (r + 31) / 32);
+    for (int w = 0; w < 2; ++w) {
+        int64_t chunks = cost ? weight[w] * kCtas / cost : 1;
+        const int64_t most = (rows + 63) / 64;  // 64 rows are worth a chunk
+        if (chunks > most) chunks = most;
+        if (chunks < 1) chunks = 1;
+        p.chunk[w] = ((rows + chunks - 1) / chunks + 15) / 16 * 16;
+        if (p.chunk[w] == 0) p.chunk[w] = 16;
+        p.chunks[w] = rows ? (rows + p.chunk[w] - 1) / p.chunk[w] : 1;
+        if (p.chunks[w] > 1)
+            p.part[w] = sizeof(float) * static_cast<size_t>((p.chunks[w] + s - 1) * r *
+                                                            ((cols[w] + 7) / 8 * 8));
     }
+    p.list_bytes = listed ? sizeof(int32_t) * static_cast<size_t>(rows + s + 1) : 0;
     return p;
 }
 
 template <typename T>
-static cudaError_t wgrad(const WgradParams &P, const WgradPlan &plan, int num_sms,
-                         cudaStream_t stream) {
-    const int blocks = P.side[0].blocks + P.side[1].blocks;
-    if (blocks == 0) return cudaSuccess;
+static cudaError_t wgrad(const WgradParams &P, int num_sms, cudaStream_t stream) {
     const int nj = P.r <= 16 ? 1 : 2;
-    const dim3 grid(static_cast<unsigned>(blocks), static_cast<unsigned>(plan.chunks),
+    const int64_t units = P.side[0].blocks * P.side[0].chunks + P.side[1].blocks * P.side[1].chunks;
+    const dim3 grid(static_cast<unsigned>(units),
                     static_cast<unsigned>((P.r + 16 * nj - 1) / (16 * nj)));
     auto kernel = nj == 1 ? wgrad_kernel<T, 1> : wgrad_kernel<T, 2>;
     const size_t smem = nj == 1 ? wgrad_smem<1>() : wgrad_smem<2>();
@@ -386,7 +387,7 @@ static cudaError_t wgrad(const WgradParams &P, const WgradPlan &plan, int num_sm
         set->store(1, std::memory_order_release);
     }
     kernel<<<grid, kThreads, smem, stream>>>(P);
-    if (plan.chunks > 1) {
+    if (P.side[0].part || P.side[1].part) {
         const int64_t cols = P.side[0].cols > P.side[1].cols ? P.side[0].cols : P.side[1].cols;
         const int64_t want = (P.s * P.r * ((cols + 3) / 4) + 255) / 256, most = int64_t(num_sms) * 4;
         join_kernel<T><<<dim3(static_cast<unsigned>(want < most ? want : most), 2), 256, 0, stream>>>(P);
@@ -401,13 +402,12 @@ cudaError_t lr_wgrad(bool half, const WgradOperand &a, const WgradOperand &b, in
     P.rows = rows;
     P.r = r;
     P.s = index.s;
-    P.chunk = plan.chunk;
     const WgradOperand *ops[2] = {&a, &b};
     for (int w = 0; w < 2; ++w) {
         const WgradOperand &o = *ops[w];
-        const int blocks = o.out ? static_cast<int>((o.cols + kCtaCols - 1) / kCtaCols) : 0;
+        const int64_t blocks = o.out ? (o.cols + kCtaCols - 1) / kCtaCols : 0;
         P.side[w] = Side{o.M.p, o.M.s0, o.cols, o.V, o.drop, blocks ? o.part : nullptr, o.out,
-                         o.ss,  o.sc,   o.sr,   blocks};
+                         o.ss,  o.sc,   o.sr,   blocks, plan.chunk[w], plan.chunks[w]};
     }
     if (P.side[0].blocks + P.side[1].blocks == 0) return cudaSuccess;
     P.index = index;
@@ -418,8 +418,7 @@ cudaError_t lr_wgrad(bool half, const WgradOperand &a, const WgradOperand &b, in
         P.order = order;
         P.start = start;
     }
-    return half ? wgrad<__half>(P, plan, num_sms, stream)
-                : wgrad<__nv_bfloat16>(P, plan, num_sms, stream);
+    return half ? wgrad<__half>(P, num_sms, stream) : wgrad<__nv_bfloat16>(P, num_sms, stream);
 }
 
 }  // namespace ti
