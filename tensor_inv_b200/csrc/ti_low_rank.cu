@@ -239,7 +239,7 @@ int backward(const ti_low_rank_t &op, const Gradient &g, Arena &arena, int sms, 
         half,
         WgradOperand{X, op.k, dP, drop, part_a, g.dA, g.sda[0], g.sda[1], g.sda[2]},
         WgradOperand{dY, op.n, g.P, Dropout{}, part_b, g.dB, g.sdb[0], g.sdb[2], g.sdb[1]}, op.t,
-        op.r, index, plan, lists, sms, st));
+        op.r, index, plan, lists, sms, err, st));
 }
 
 bool bad_workspace(const void *ws, size_t have, size_t need) {

@@ -112,6 +112,6 @@ struct WgradOperand {
 };
 cudaError_t lr_wgrad(bool half, const WgradOperand &a, const WgradOperand &b, int64_t rows,
                      int64_t r, const RowIndex &index, const WgradPlan &plan, void *lists,
-                     int num_sms, cudaStream_t stream);
+                     int num_sms, int *err, cudaStream_t stream);
 
 }  // namespace ti

@@ -5,30 +5,41 @@
 //
 // Both are out[s] = M^T V with a wide 16-bit M (rows x cols) and a thin float32 V (rows x r); both
 // run in one launch.  M's bytes bound them: each element is read once and meets r values of V.
-// V keeps its 32 bits by entering mma.sync (tf32) in two parts, its upper 11 bits and the rest, while
-// M's 16-bit values are exact in tf32; the legacy tensor path is enough for a product this thin.
-// (An infinity in M meets both parts, so its column comes out infinite or NaN.)
 //
 //   lists  one CTA per adapter writes the positions of its rows, in order, so that an adapter's rows
 //          are consecutive; no atomics, so the sums have one order.  A single adapter needs none.
-//   wgrad  a CTA takes a chunk of that order and 512 columns, 64 per warp.  Each warp keeps its own
-//          ring of asynchronous copies (16 rows x 128 bytes a step, four steps ahead) and waits for
-//          no other warp; a thread reads 16 bytes of a row from it -- 8 columns that are the same
-//          fragment position of 8 MMAs -- and applies the dropout mask there.  Where a chunk
-//          crosses from one adapter to the next it writes its sums to another slot: chunk + adapter
-//          numbers the (chunk, adapter) pairs that occur without gaps in either direction.
+//   wgrad  a CTA takes a chunk of that order and 256 columns, in stages of 64 rows.  The copy engine
+//          gathers the rows (four row numbers per copy; places without a row get one past the end,
+//          which reads as zeros, so that no row of another adapter enters).  M stays as it lies in
+//          memory: its columns are the 128-row side of the MMA, read in the orientation whose
+//          consecutive elements run along the columns.  Eight warps turn V into the other operand:
+//          16-bit values in two parts, the rounded value and what is left of it.  That keeps 22 bits
+//          of V for fp16 and 16 for bf16 (2^-17, where dA and dB are rounded to 2^-9).  For fp16,
+//          whose exponents V may leave, each rank's column is first scaled by a power of two that
+//          brings its largest value of the CTA's rows to 2^14; the sums are scaled back.  With
+//          dropout the same warps mask the staged tile.  Where a chunk crosses from one adapter to
+//          the next the sums go to another slot: chunk + adapter numbers the (chunk, adapter) pairs
+//          that occur without gaps in either direction.
 //   join   adds an adapter's slots in order and rounds once.  One chunk needs no join.
+//
+// (An infinity in M meets both parts of V, so its column comes out infinite or NaN.)
+#include <cstring>
+
 #include "ti_lr_dot.cuh"
 #include "ti_lr_launch.cuh"
 
 namespace ti {
 namespace {
 
-constexpr int kThreads = 256, kWarpCols = 64, kCtaCols = 8 * kWarpCols;
-constexpr int kStage = 128;        // rows of V in shared memory at a time
-constexpr int kStep = 16;          // rows of M per copy step
-constexpr int kRing = 5;           // steps in a warp's ring: four on their way, one being read
-constexpr int kStepBytes = kStep * 128;
+constexpr int kCtaCols = 256, kRows = 64;     // columns of a CTA, rows of a stage
+constexpr int kAtomBytes = kRows * 128;       // 64 columns of a stage
+constexpr int kMBytes = 4 * kAtomBytes;
+constexpr int kBlockRanks = 64;               // ranks of a CTA
+constexpr int kPartBytes = kBlockRanks * 128; // one part of V's stage
+constexpr int kStageBytes = kMBytes + 2 * kPartBytes, kStages = 4;
+constexpr int kWorkers = 256, kThreads = 64 + kWorkers;
+constexpr uint32_t kTmemCols = 128;           // two halves of the columns, 64 ranks each
+constexpr size_t kSmem = size_t(kStages) * kStageBytes + 1024 + 1024;
 
 struct Side {
     const void *M;
@@ -44,33 +55,109 @@ struct Side {
 
 struct WgradParams {
     Side side[2];
+    int rp;                 // ranks per CTA in TMEM: r, or the block's part, rounded up to 16
+    uint32_t idesc;
+    int *err;
     int64_t rows, r, s;
     RowIndex index;         // of a single adapter: rows of others are left out
     const int32_t *order;   // row numbers grouped by adapter, or null: all rows, adapter 0
     const int32_t *start;   // [s + 1] first position of each adapter, or null
 };
 
-template <typename T>
-__device__ __forceinline__ float half_of(uint32_t w, int hi) {
-    if constexpr (std::is_same<T, __nv_bfloat16>::value)
-        return __uint_as_float(hi ? w & 0xFFFF0000u : w << 16);
-    else
-        return __half2float(__ushort_as_half(static_cast<unsigned short>(hi ? w >> 16 : w)));
-}
-
-__device__ __forceinline__ void mma_tf32(float (&d)[4], const float (&a)[4], float b0, float b1) {
+__device__ __forceinline__ void umma_f16(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc,
+                                         uint32_t accumulate) {
     asm volatile(
-        "mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
-        "{%8,%9}, {%0,%1,%2,%3};"
-        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-        : "r"(__float_as_uint(a[0])), "r"(__float_as_uint(a[1])), "r"(__float_as_uint(a[2])),
-          "r"(__float_as_uint(a[3])), "r"(__float_as_uint(b0)), "r"(__float_as_uint(b1)));
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+        : "memory");
 }
 
-// 16 bytes to shared memory, of which the first `bytes` are read and the others become zero.
-__device__ __forceinline__ void copy16(uint32_t dst, const void *src, int bytes) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes)
-                 : "memory");
+// Four rows of a matrix whose map's box is one row high, 64 columns from c0, one below the other.
+__device__ __forceinline__ void tma_gather4(void *dst, const CUtensorMap *map, uint64_t *bar, int c0,
+                                            const int (&row)[4]) {
+    asm volatile(
+        "cp.async.bulk.tensor.2d.shared::cluster.global.tile::gather4.mbarrier::complete_tx::bytes"
+        " [%0], [%1, {%3, %4, %5, %6, %7}], [%2];" ::"r"(smem_u32(dst)),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(c0), "r"(row[0]), "r"(row[1]),
+        "r"(row[2]), "r"(row[3])
+        : "memory");
+}
+
+__device__ __forceinline__ void raise(const WgradParams &P, volatile int *abort, int code) {
+    *abort = 1;
+    atomicCAS(P.err, 0, code);
+}
+
+__device__ __forceinline__ void drain_wait(const WgradParams &P, uint64_t *bar, uint32_t parity) {
+    const uint32_t a = smem_u32(bar);
+    const unsigned long long t0 = globaltimer_ns();
+    while (!mbar_try_wait(a, parity)) {
+        if (globaltimer_ns() - t0 > kWaitTimeoutNs) {
+            atomicCAS(P.err, 0, kErrTimeoutDrain);
+            return;
+        }
+    }
+}
+
+__device__ __forceinline__ void worker_sync() {
+    asm volatile("bar.sync 1, %0;" ::"n"(kWorkers) : "memory");
+}
+
+// worker_sync that also tells every worker whether any of them saw `flag`.
+__device__ __forceinline__ bool worker_sync_or(bool flag) {
+    uint32_t any;
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\t"
+        "setp.ne.u32 p, %1, 0;\n\t"
+        "bar.red.or.pred q, 1, %2, p;\n\t"
+        "selp.u32 %0, 1, 0, q;\n\t}"
+        : "=r"(any)
+        : "r"(static_cast<uint32_t>(flag)), "n"(kWorkers)
+        : "memory");
+    return any != 0;
+}
+
+// The row at position p of the order, or `rows` (one past the end) where there is none.
+__device__ __forceinline__ int row_at(const WgradParams &P, int64_t p, int64_t stop) {
+    if (p >= stop) return static_cast<int>(P.rows);
+    if (P.order) return P.order[p];
+    return P.index.at(p) == 0 ? static_cast<int>(p) : static_cast<int>(P.rows);
+}
+
+// The first adapter whose rows reach past pos (P.s: none), found by a whole warp, 32 at a time.
+__device__ __forceinline__ int64_t first_adapter(const WgradParams &P, int64_t pos, int lane) {
+    int64_t lo = 0, n = P.s;
+    while (n > 0) {
+        const int64_t step = (n + 31) / 32;
+        const int64_t last = lo + min((lane + 1) * step, n) - 1;  // of this lane's share
+        const unsigned past = __ballot_sync(0xFFFFFFFFu, P.start[last + 1] > pos);
+        if (!past) return P.s;
+        const int64_t skip = (__ffs(past) - 1) * step;
+        lo += skip;
+        if (step == 1) return lo;
+        n = min(step, n - skip);
+    }
+    return P.s;
+}
+
+// The segments of a chunk, adapter by adapter from `s` on: f(s, from, to) for positions [from, to);
+// returns false to stop.  With `every`, adapters without rows too.
+template <class Fn>
+__device__ __forceinline__ void segments(const WgradParams &P, int64_t s, int64_t pos, int64_t stop,
+                                         bool every, Fn &&f) {
+    for (; s < P.s && (every || pos < stop); ++s) {
+        const int64_t end = P.start ? min(stop, int64_t(P.start[s + 1])) : stop;
+        if ((end > pos || every) && !f(s, pos, max(pos, end))) return;
+        pos = max(pos, end);
+    }
+}
+
+template <typename T>
+__device__ __forceinline__ uint16_t bits16(float v) {
+    const T h = from_float<T>(v);
+    return *reinterpret_cast<const uint16_t *>(&h);
 }
 
 // order[] and start[]: rows grouped by adapter, ascending within one.  CTA s compacts the rows of
@@ -122,244 +209,415 @@ __global__ void __launch_bounds__(1024) lists_kernel(RowIndex index, int64_t row
     if (s == gridDim.x - 1 && threadIdx.x == 0) start[s + 1] = at;
 }
 
-// Accumulators of one warp: 16*kNJ ranks x 64 columns.  In MMA i, column n of the instruction is
-// column 8n + i of the warp's 64, so a thread's two columns of a row are 16tq + i and 16tq + 8 + i.
-template <typename T, int kNJ>
-__device__ __forceinline__ void store_sums(const WgradParams &P, const Side &S,
-                                           const float (&acc)[kNJ][8][4], int64_t slot, int64_t s,
-                                           int64_t c0, int64_t j0, int g, int tq) {
-    const int64_t ldc = (S.cols + 7) / 8 * 8;
-#pragma unroll
-    for (int nj = 0; nj < kNJ; ++nj)
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {  // rank g or g + 8
-            const int64_t j = j0 + 16 * nj + g + 8 * h;
-            if (j >= P.r) continue;
-#pragma unroll
-            for (int k = 0; k < 2; ++k) {  // columns 16tq + 8k ..
-                const int64_t c = c0 + 16 * tq + 8 * k;
-                if (c >= S.cols) continue;
-                if (S.part) {
-                    float4 *dst = reinterpret_cast<float4 *>(S.part + (slot * P.r + j) * ldc + c);
-                    dst[0] = make_float4(acc[nj][0][2 * h + k], acc[nj][1][2 * h + k],
-                                         acc[nj][2][2 * h + k], acc[nj][3][2 * h + k]);
-                    dst[1] = make_float4(acc[nj][4][2 * h + k], acc[nj][5][2 * h + k],
-                                         acc[nj][6][2 * h + k], acc[nj][7][2 * h + k]);
-                } else {
-                    T *dst = static_cast<T *>(S.out) + s * S.ss + j * S.sr;
-#pragma unroll
-                    for (int i = 0; i < 8; ++i)
-                        if (c + i < S.cols)
-                            dst[(c + i) * S.sc] = from_float<T>(acc[nj][i][2 * h + k]);
-                }
-            }
-        }
-}
+// Maps of dA's and dB's matrices: boxes of 64 rows, and of one row for gathering.
+struct Maps {
+    CUtensorMap tile[2], row[2];
+};
 
-template <int kNJ>
-constexpr size_t wgrad_smem() {
-    return size_t(8) * kRing * kStepBytes + sizeof(float) * kStage * (16 * kNJ + 8) +
-           sizeof(int32_t) * kStage;
-}
+// Roles: warp 0 copies (16 lanes, four rows each), warp 1 TMEM and MMA issue, warps 2..9 V, the
+// mask and the epilogue.
+template <typename T>
+__global__ void __launch_bounds__(kThreads, 1)
+    wgrad_kernel(const __grid_constant__ Maps maps, const __grid_constant__ WgradParams P) {
+    constexpr bool kScaled = std::is_same<T, __half>::value;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t *ring = reinterpret_cast<uint8_t *>(
+        (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    float *scale = reinterpret_cast<float *>(ring + kStages * kStageBytes);  // [64] 2^-e by rank
+    uint64_t *full = reinterpret_cast<uint64_t *>(scale + kBlockRanks);
+    uint64_t *ready = full + kStages;   // V is in place, and M masked
+    uint64_t *empty = ready + kStages;
+    uint64_t *tfull = empty + kStages;
+    uint64_t *tempty = tfull + 1;
+    uint64_t *drain = tempty + 1;
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(drain + 1);
+    volatile int *abort = reinterpret_cast<volatile int *>(tmem_slot + 1);
+    int *start_at = const_cast<int *>(abort) + 1;
 
-template <typename T, int kNJ>
-__global__ void __launch_bounds__(kThreads, 2) wgrad_kernel(const __grid_constant__ WgradParams P) {
-    constexpr int kVStride = 16 * kNJ + 8;  // floats: the 4 x 8 fragment reads hit all 32 banks
-    extern __shared__ __align__(128) uint8_t smem[];
-    float(*sv)[kVStride] = reinterpret_cast<float(*)[kVStride]>(smem + 8 * kRing * kStepBytes);
-    int32_t *srow = reinterpret_cast<int32_t *>(sv + kStage);
     const int64_t units_a = P.side[0].blocks * P.side[0].chunks;
     const int which = blockIdx.x < units_a ? 0 : 1;
     const Side &S = P.side[which];
+    const CUtensorMap *tile_map = &maps.tile[which], *row_map = &maps.row[which];
     const int64_t unit = blockIdx.x - (which ? units_a : 0), chunk = unit / S.blocks;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, tq = lane & 3;
-    const int64_t c0 = unit % S.blocks * kCtaCols + warp * kWarpCols;
-    const int64_t j0 = int64_t(blockIdx.y) * 16 * kNJ;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int64_t c0 = unit % S.blocks * kCtaCols;
+    const int j0 = static_cast<int>(blockIdx.y) * kBlockRanks;
     const int64_t total = P.start ? P.start[P.s] : P.rows;
     const bool direct = S.part == nullptr;
-    int64_t pos = chunk * S.chunk;
-    const int64_t stop = min(total, pos + S.chunk);
-    const DropoutKeys key(S.drop.cut ? dropout_key(S.drop) : 0);
+    const int64_t first = chunk * S.chunk, stop = min(total, first + S.chunk);
 
-    // the first adapter whose rows reach past pos (from the first one, where every adapter's
-    // gradient is written here)
-    int64_t s = 0;
-    if (P.start && !direct) {
-        int64_t lo = 0, hi = P.s;
-        while (lo < hi) {
-            const int64_t mid = (lo + hi) / 2;
-            if (P.start[mid + 1] > pos) hi = mid;
-            else lo = mid + 1;
+    if (threadIdx.x == 0) {
+        if (P.rows) prefetch_tensormap(tile_map);
+        for (int s = 0; s < kStages; ++s) {
+            mbar_init(&full[s], 1);
+            mbar_init(&ready[s], kWorkers / 32);
+            mbar_init(&empty[s], 1);
         }
-        s = lo;
+        mbar_init(tfull, 1);
+        mbar_init(tempty, kWorkers / 32);
+        mbar_init(drain, 1);
+        *abort = 0;
+        fence_barrier_init();
     }
-    const int64_t col = c0 + 8 * g;
-    const uint16_t *M = static_cast<const uint16_t *>(S.M);
-    const uint8_t *ring_ptr = smem + warp * kRing * kStepBytes;
-    const uint32_t ring = smem_u32(ring_ptr);
-    for (; s < P.s && (direct || pos < stop); ++s) {
-        const int64_t seg_end = P.start ? min(stop, int64_t(P.start[s + 1])) : stop;
-        float acc[kNJ][8][4];
-#pragma unroll
-        for (int nj = 0; nj < kNJ; ++nj)
-#pragma unroll
-            for (int i = 0; i < 8; ++i)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) acc[nj][i][e] = 0.0f;
+    if (warp == 1) {
+        tmem_alloc(tmem_slot, kTmemCols);
+        tmem_relinquish();
+    }
+    if (warp == 2) {
+        const int64_t s = P.start && !direct ? first_adapter(P, first, lane) : 0;
+        if (lane == 0) *start_at = static_cast<int>(s);
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem_base = *tmem_slot;
+    const int64_t s0 = *start_at;
 
-        for (int64_t b = pos; b < seg_end; b += kStage) {
-            const int n = static_cast<int>(min(int64_t(kStage), seg_end - b));
-            __syncthreads();  // the previous stage has been read
-            if (threadIdx.x < kStage) {
-                int t = -1;
-                if (static_cast<int>(threadIdx.x) < n) {
-                    t = P.order ? P.order[b + threadIdx.x] : static_cast<int32_t>(b + threadIdx.x);
-                    if (!P.order && P.index.at(t) != 0) t = -1;
-                }
-                srow[threadIdx.x] = t;
-            }
-            __syncthreads();
-            const int steps = (n + kStep - 1) / kStep;
-            // A lane copies chunk lane % 8 of four of a step's rows.  Chunk c of row q lies at
-            // c ^ 2 (q % 4): the 16-byte reads below then hit all banks.
-            auto issue = [&](int step) {
-                if (step < steps) {
+    if (warp == 0) {
+        // ---------------- copies ----------------
+        int stage = 0;
+        uint32_t phase = 0, issued_mask = 0, issued_phase = 0;
+        bool ok = true;
+        segments(P, s0, first, stop, direct, [&](int64_t, int64_t from, int64_t to) {
+            int row[4];
+            auto ask = [&](int64_t b) {
 #pragma unroll
-                    for (int h = 0; h < 4; ++h) {
-                        const int q = (lane >> 3) + 4 * h, c = lane & 7;
-                        const int t = srow[step * kStep + q];
-                        const int64_t left = S.cols - (c0 + 8 * c);
-                        const int bytes =
-                            t < 0 || left <= 0 ? 0 : left >= 8 ? 16 : static_cast<int>(2 * left);
-                        copy16(ring + (step % kRing) * kStepBytes + q * 128 +
-                                   ((c ^ ((q & 3) << 1)) << 4),
-                               M + (bytes ? t * S.ld + c0 + 8 * c : 0), bytes);
-                    }
-                }
-                asm volatile("cp.async.commit_group;" ::: "memory");
+                for (int e = 0; e < 4; ++e) row[e] = row_at(P, b + 4 * (lane & 15) + e, to);
             };
-            for (int k = 0; k < kRing - 1; ++k) issue(k);
-            for (int e = threadIdx.x; e < kStage * 16 * kNJ; e += kThreads) {
-                const int q = e / (16 * kNJ), j = e % (16 * kNJ);
-                const int t = srow[q];
-                sv[q][j] = t >= 0 && j0 + j < P.r ? S.V[int64_t(t) * P.r + j0 + j] : 0.0f;
-            }
-            __syncthreads();
-#pragma unroll 1
-            for (int k = 0; k < steps; ++k) {
-                asm volatile("cp.async.wait_group %0;" ::"n"(kRing - 2) : "memory");
-                __syncwarp();
-                const int q = k * kStep;
-                const uint8_t *src = ring_ptr + (k % kRing) * kStepBytes;
-                uint4 x[4];
-#pragma unroll
-                for (int h = 0; h < 4; ++h)
-                    x[h] = *reinterpret_cast<const uint4 *>(src + (4 * h + tq) * 128 +
-                                                            ((g ^ (tq << 1)) << 4));
-                __syncwarp();
-                issue(k + kRing - 1);  // into the slot read in the step before
-                if (S.drop.cut) {
-#pragma unroll
-                    for (int h = 0; h < 4; ++h)
-                        x[h] = masked(x[h], S.drop, key,
-                                      static_cast<uint32_t>(srow[q + 4 * h + tq]),
-                                      static_cast<uint32_t>(col >> 3));
+            ask(from);
+            for (int64_t b = from; b < to; b += kRows) {
+                if (!mbar_wait(&empty[stage], phase ^ 1, abort)) {
+                    raise(P, abort, kErrTimeoutProducer);
+                    ok = false;
                 }
+                ok = __all_sync(0xFFFFFFFFu, ok);
+                if (!ok) return false;
+                if (lane == 0) mbar_arrive_expect_tx(&full[stage], kMBytes);
+                __syncwarp();
+                // 64 consecutive rows are one box; a copy of four rows at a time is much slower
+                const int row0 = __shfl_sync(0xFFFFFFFFu, row[0], 0);
+                bool run = true;
 #pragma unroll
-                for (int k8 = 0; k8 < 2; ++k8) {  // two steps of 8 rows
-                    const int q0 = q + 8 * k8 + tq;
-                    const uint4 &xa = x[2 * k8], &xb = x[2 * k8 + 1];
-                    const uint32_t m0[4] = {xa.x, xa.y, xa.z, xa.w};
-                    const uint32_t m1[4] = {xb.x, xb.y, xb.z, xb.w};
+                for (int e = 0; e < 4; ++e)
+                    run = run && row[e] == row0 + 4 * (lane & 15) + e && row[e] < P.rows;
+                run = __all_sync(0xFFFFFFFFu, run);
+                uint8_t *dst = ring + stage * kStageBytes;
+                if (run) {
+                    if (lane < 4)
+                        tma_load_2d(dst + lane * kAtomBytes, tile_map, &full[stage],
+                                    static_cast<int>(c0) + 64 * lane, row0);
+                } else if (lane < 16) {
 #pragma unroll
-                    for (int nj = 0; nj < kNJ; ++nj) {
-                        const int j = 16 * nj + g;
-                        float hi[4] = {sv[q0][j], sv[q0][j + 8], sv[q0 + 4][j], sv[q0 + 4][j + 8]};
-                        float lo[4];
+                    for (int a = 0; a < 4; ++a)
+                        tma_gather4(dst + 512 * lane + a * kAtomBytes, row_map, &full[stage],
+                                    static_cast<int>(c0) + 64 * a, row);
+                }
+                ask(b + kRows);  // the next stage's rows are on their way
+                issued_mask |= 1u << stage;
+                issued_phase = (issued_phase & ~(1u << stage)) | (phase << stage);
+                if (++stage == kStages) {
+                    stage = 0;
+                    phase ^= 1;
+                }
+            }
+            return true;
+        });
+        if (!ok && lane == 0)  // every copy lands before the CTA may exit
+            for (int s = 0; s < kStages; ++s)
+                if ((issued_mask >> s) & 1) drain_wait(P, &full[s], (issued_phase >> s) & 1);
+    } else if (warp == 1) {
+        if (lane == 0) {
+            // ---------------- MMA issuer ----------------
+            int stage = 0;
+            uint32_t phase = 0, seg = 0;
+            bool ok = true, any_issued = false;
+            segments(P, s0, first, stop, direct, [&](int64_t, int64_t from, int64_t to) {
+                if (from == to) return true;
+                if (!mbar_wait(tempty, (seg & 1) ^ 1, abort)) {
+                    raise(P, abort, kErrTimeoutMma);
+                    ok = false;
+                    return false;
+                }
+                ++seg;
+                tc_fence_after();
+                for (int64_t b = from; b < to; b += kRows) {
+                    if (!mbar_wait(&full[stage], phase, abort) ||
+                        !mbar_wait(&ready[stage], phase, abort)) {
+                        raise(P, abort, kErrTimeoutMma);
+                        ok = false;
+                        return false;
+                    }
+                    tc_fence_after();
+                    const uint32_t sm = smem_u32(ring + stage * kStageBytes);
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            // infinities and NaN stay whole in the upper part
-                            const uint32_t bits = __float_as_uint(hi[e]);
-                            const bool odd = (bits & 0x7F800000u) == 0x7F800000u;
-                            const float up = __uint_as_float(bits & 0xFFFFE000u);
-                            lo[e] = odd ? 0.0f : hi[e] - up;
-                            hi[e] = odd ? hi[e] : up;
-                        }
+                    for (int h = 0; h < 2; ++h) {
+                        const uint64_t mdesc =
+                            make_sw128_mnmajor_desc(sm + 2 * h * kAtomBytes, kAtomBytes);
 #pragma unroll
-                        for (int i = 0; i < 8; ++i) {
-                            const float b0 = half_of<T>(m0[i >> 1], i & 1);
-                            const float b1 = half_of<T>(m1[i >> 1], i & 1);
-                            mma_tf32(acc[nj][i], hi, b0, b1);
-                        }
-                        // (apart from the first eight, which they would have to wait for)
+                        for (int part = 0; part < 2; ++part) {
+                            const uint64_t vdesc =
+                                make_sw128_kmajor_desc(sm + kMBytes + part * kPartBytes);
 #pragma unroll
-                        for (int i = 0; i < 8; ++i) {
-                            const float b0 = half_of<T>(m0[i >> 1], i & 1);
-                            const float b1 = half_of<T>(m1[i >> 1], i & 1);
-                            mma_tf32(acc[nj][i], lo, b0, b1);
+                            for (int kk = 0; kk < kRows / 16; ++kk)
+                                umma_f16(tmem_base + h * kBlockRanks, mdesc + 128 * kk,
+                                         vdesc + 2 * kk, P.idesc,
+                                         b > from || part > 0 || kk > 0 ? 1u : 0u);
                         }
                     }
+                    any_issued = true;
+                    umma_commit(&empty[stage]);
+                    if (++stage == kStages) {
+                        stage = 0;
+                        phase ^= 1;
+                    }
+                }
+                umma_commit(tfull);
+                return true;
+            });
+            if (!ok && any_issued) {
+                umma_commit(drain);
+                drain_wait(P, drain, 0);
+            }
+        }
+    } else {
+        // ---------------- V, the mask, the epilogue ----------------
+        const int wt = threadIdx.x - 64, w = warp - 2;
+        const int half = w & 1;                  // this warp's 32 rows of a stage
+        const int quads = P.rp / 4;              // and every fourth quad of ranks from w / 2
+        const DropoutKeys key(S.drop.cut ? dropout_key(S.drop) : 0);
+        const bool vec = P.r % 4 == 0 && (reinterpret_cast<uintptr_t>(S.V) & 15) == 0;
+        auto load_v = [&](int row, int quad) {
+            float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            const int64_t j = j0 + 4 * quad;
+            if (row >= P.rows || j >= P.r) return v;
+            const float *p = S.V + row * P.r + j;
+            if (vec) return *reinterpret_cast<const float4 *>(p);
+            v.x = p[0];
+            if (j + 1 < P.r) v.y = p[1];
+            if (j + 2 < P.r) v.z = p[2];
+            if (j + 3 < P.r) v.w = p[3];
+            return v;
+        };
+        int stage = 0;
+        uint32_t phase = 0, seg = 0;
+        bool ok = true;  // a wait that gave up ends all workers at their next barrier
+        segments(P, s0, first, stop, direct, [&](int64_t s, int64_t from, int64_t to) {
+            if (kScaled) {
+                // 2^-e with the largest finite value of the segment's column near 2^14
+                if (worker_sync_or(!ok)) return false;  // the previous scales have been read
+                for (int q = w; q < quads; q += kWorkers / 32) {
+                    float m[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                    for (int64_t b = from + lane; b - lane < to; b += 32 * 8) {
+                        int row[8];
+                        float4 v[8];
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) row[i] = row_at(P, b + 32 * i, to);
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) v[i] = load_v(row[i], q);
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) {
+                            const float x[4] = {fabsf(v[i].x), fabsf(v[i].y), fabsf(v[i].z),
+                                                fabsf(v[i].w)};
+#pragma unroll
+                            for (int e = 0; e < 4; ++e)
+                                if (x[e] < __int_as_float(0x7F800000)) m[e] = fmaxf(m[e], x[e]);
+                        }
+                    }
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const uint32_t top = __reduce_max_sync(0xFFFFFFFFu, __float_as_uint(m[e]));
+                        // exponent of the largest value; the power stays a normal number
+                        const int x = static_cast<int>(top >> 23);  // biased
+                        const int y = top ? min(max(127 + 14 + 127 - x, 1), 253) : 127;
+                        if (lane == 0) scale[4 * q + e] = __int_as_float(y << 23);
+                    }
+                }
+                worker_sync();
+            }
+            // row numbers are read two stages ahead and values one, so that neither is waited for
+            const int t = 32 * half + lane;
+            float4 v[4], ahead[4];
+            auto fetch = [&](int r, float4(&x)[4]) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if ((w >> 1) + 4 * i < quads) x[i] = load_v(r, (w >> 1) + 4 * i);
+            };
+            fetch(row_at(P, from + t, to), v);
+            int row = row_at(P, from + kRows + t, to);
+            int mask_next = S.drop.cut ? row_at(P, from + (wt >> 2), to) : 0;
+            for (int64_t b = from; b < to; b += kRows) {
+                const int mask_row = mask_next;
+                fetch(row, ahead);
+                row = row_at(P, b + 2 * kRows + t, to);
+                if (S.drop.cut) mask_next = row_at(P, b + kRows + (wt >> 2), to);
+                if (!mbar_wait(&empty[stage], phase ^ 1, abort)) {
+                    raise(P, abort, kErrTimeoutProducer);
+                    ok = false;
+                    break;
+                }
+                uint8_t *m = ring + stage * kStageBytes;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int quad = (w >> 1) + 4 * i;
+                    if (quad >= quads) break;
+                    const float x[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const int j = 4 * quad + e;
+                        const float y = kScaled ? x[e] * scale[j] : x[e];
+                        const uint16_t hi = bits16<T>(y);
+                        const float up = to_float(*reinterpret_cast<const T *>(&hi));
+                        // infinities and NaN stay whole in the first part
+                        const float rest = fabsf(up) < __int_as_float(0x7F800000) ? y - up : 0.0f;
+                        const uint32_t at = j * 128 + ((((t >> 3) ^ (j & 7)) << 4) | ((t & 7) << 1));
+                        *reinterpret_cast<uint16_t *>(m + kMBytes + at) = hi;
+                        *reinterpret_cast<uint16_t *>(m + kMBytes + kPartBytes + at) =
+                            bits16<T>(rest);
+                    }
+                }
+#pragma unroll
+                for (int i = 0; i < 4; ++i) v[i] = ahead[i];
+                if (S.drop.cut) {
+                    if (!mbar_wait(&full[stage], phase, abort)) {
+                        raise(P, abort, kErrTimeoutEpilogue);
+                        ok = false;
+                        break;
+                    }
+                    // a thread takes 64 columns of one row
+                    const int mr = wt >> 2, a = wt & 3;
+                    uint8_t *p = m + a * kAtomBytes + mr * 128;
+#pragma unroll
+                    for (int c = 0; c < 8; ++c) {
+                        uint4 *x = reinterpret_cast<uint4 *>(p + ((c ^ (mr & 7)) << 4));
+                        *x = masked(*x, S.drop, key, static_cast<uint32_t>(mask_row),
+                                    static_cast<uint32_t>(c0 >> 3) + 8 * a + c);
+                    }
+                }
+                fence_proxy_async_smem();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&ready[stage]);
+                if (++stage == kStages) {
+                    stage = 0;
+                    phase ^= 1;
                 }
             }
-            asm volatile("cp.async.wait_group 0;" ::: "memory");
-        }
-        if (seg_end > pos || direct)
-            store_sums<T, kNJ>(P, S, acc, chunk + s, s, c0, j0, g, tq);
-        pos = max(pos, seg_end);
+            // ---------------- the segment's sums ----------------
+            const int q = warp & 3, h = w >> 2;  // TMEM lane quadrant, half of the columns
+            const int64_t c = c0 + 128 * h + 32 * q + lane;
+            const bool some = from < to;
+            if (ok && some && !mbar_wait(tfull, seg & 1, abort)) {
+                raise(P, abort, kErrTimeoutEpilogue);
+                ok = false;
+            }
+            ok = __all_sync(0xFFFFFFFFu, ok);
+            if (!ok) return kScaled;  // on to the barrier, where there is one
+            tc_fence_after();
+            const int64_t ldc = (S.cols + 7) / 8 * 8;
+            for (int jb = 0; jb < P.rp; jb += 16) {
+                uint32_t x[16];
+                if (some) {
+                    tmem_ld_32x32b_x16(tmem_base + (static_cast<uint32_t>(q * 32) << 16) +
+                                           h * kBlockRanks + jb,
+                                       x);
+                    tmem_wait_ld();
+                }
+                if (c < S.cols)
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) {
+                        const int64_t j = j0 + jb + e;
+                        if (j >= P.r) continue;
+                        float y = some ? __uint_as_float(x[e]) : 0.0f;
+                        // (a power of two, and its inverse by exponent arithmetic)
+                        if (kScaled && some)
+                            y *= __int_as_float((254 << 23) - __float_as_int(scale[jb + e]));
+                        if (direct)
+                            static_cast<T *>(S.out)[s * S.ss + c * S.sc + j * S.sr] = from_float<T>(y);
+                        else
+                            S.part[((chunk + s) * P.r + j) * ldc + c] = y;
+                    }
+            }
+            if (some) {
+                ++seg;
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(tempty);
+            }
+            return true;
+        });
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 1) {
+        tc_fence_after();
+        tmem_dealloc(tmem_base, kTmemCols);
     }
 }
 
-// out[s][c][j] = the sum of adapter s's slots, in order.
+// out[s][c][j] = the sum of adapter s's slots, in order.  A block takes 32 ranks x 32 columns, reads
+// them along the columns and writes them along whichever of the two is consecutive in out.
 template <typename T>
 __global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ WgradParams P) {
     const Side &S = P.side[blockIdx.y];
     if (!S.part) return;
+    __shared__ float tile[32][33];
+    const int x = threadIdx.x & 31, y = threadIdx.x >> 5;
     const int64_t ldc = (S.cols + 7) / 8 * 8;
     const int64_t total = P.start ? P.start[P.s] : P.rows;
-    const int64_t quads = (S.cols + 3) / 4;
-    for (int64_t u = blockIdx.x * int64_t(blockDim.x) + threadIdx.x; u < P.s * P.r * quads;
-         u += int64_t(gridDim.x) * blockDim.x) {
-        const int64_t c = u % quads * 4, j = u / quads % P.r, s = u / (quads * P.r);
+    const int64_t blocks_c = (S.cols + 31) / 32, blocks_j = (P.r + 31) / 32;
+    for (int64_t u = blockIdx.x; u < P.s * blocks_j * blocks_c; u += gridDim.x) {
+        const int64_t c0 = u % blocks_c * 32, j0 = u / blocks_c % blocks_j * 32;
+        const int64_t s = u / (blocks_c * blocks_j);
         const int64_t first = P.start ? P.start[s] : 0;
         const int64_t end = P.start ? P.start[s + 1] : s == 0 ? total : 0;
-        float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        if (end > first)
-            for (int64_t k = first / S.chunk; k <= (end - 1) / S.chunk; ++k) {
-                const float4 a =
-                    *reinterpret_cast<const float4 *>(S.part + ((k + s) * P.r + j) * ldc + c);
-                v.x += a.x;
-                v.y += a.y;
-                v.z += a.z;
-                v.w += a.w;
-            }
-        T *dst = static_cast<T *>(S.out) + s * S.ss + j * S.sr;
-        const float w[4] = {v.x, v.y, v.z, v.w};
+        const int64_t k0 = first / S.chunk, k1 = end > first ? (end - 1) / S.chunk : k0 - 1;
+        T *out = static_cast<T *>(S.out) + s * S.ss;
+        const int64_t c = c0 + x;
+        float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        for (int64_t k = k0; k <= k1; ++k)
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-            if (c + e < S.cols) dst[(c + e) * S.sc] = from_float<T>(w[e]);
+            for (int h = 0; h < 4; ++h) {
+                const int64_t j = j0 + y + 8 * h;
+                if (c < S.cols && j < P.r) v[h] += S.part[((k + s) * P.r + j) * ldc + c];
+            }
+        if (S.sr == 1 && S.sc != 1) {
+#pragma unroll
+            for (int h = 0; h < 4; ++h) tile[y + 8 * h][x] = v[h];
+            __syncthreads();
+#pragma unroll
+            for (int h = 0; h < 4; ++h)
+                if (c0 + y + 8 * h < S.cols && j0 + x < P.r)
+                    out[(c0 + y + 8 * h) * S.sc + j0 + x] = from_float<T>(tile[x][y + 8 * h]);
+            __syncthreads();
+        } else {
+#pragma unroll
+            for (int h = 0; h < 4; ++h) {
+                const int64_t j = j0 + y + 8 * h;
+                if (c < S.cols && j < P.r) out[c * S.sc + j * S.sr] = from_float<T>(v[h]);
+            }
+        }
     }
 }
 
 }  // namespace
 
-// Chunks of rows: one wave of CTAs, two per SM, so that the partial sums, which are written and
-// read once for each chunk, stay few.  The mask makes a row of dA cost about twice a row of dB
-// (4096 x 4096, r = 16: 45 us against 30 us with equal chunks), so dA's chunks are half as long then.
+// Chunks of rows: one wave of CTAs, one per SM, so that the partial sums, which are written and
+// read once for each chunk, stay few.
 WgradPlan lr_wgrad_plan(int64_t rows, int64_t r, int64_t s, int64_t cols_a, int64_t cols_b,
                         bool listed, bool dropped) {
-    constexpr int64_t kCtas = 296;  // fixed: the workspace is sized without a device
+    constexpr int64_t kCtas = 148;  // fixed: the workspace is sized without a device
     WgradPlan p{};
-    const int64_t cols[2] = {cols_a, cols_b}, weight[2] = {dropped ? 2 : 1, 1};
+    // with a mask a row of dA costs more than a row of dB
+    const int64_t cols[2] = {cols_a, cols_b}, weight[2] = {dropped ? 3 : 2, 2};
     int64_t cost = 0;
     for (int w = 0; w < 2; ++w)
-        cost += weight[w] * ((cols[w] + kCtaCols - 1) / kCtaCols) * (r <= 16 ? 1 : (r + 31) / 32);
+        cost += weight[w] * ((cols[w] + kCtaCols - 1) / kCtaCols) * ((r + kBlockRanks - 1) / kBlockRanks);
     for (int w = 0; w < 2; ++w) {
         int64_t chunks = cost ? weight[w] * kCtas / cost : 1;
-        const int64_t most = (rows + 63) / 64;  // 64 rows are worth a chunk
+        const int64_t most = (rows + 127) / 128;  // 128 rows are worth a chunk
         if (chunks > most) chunks = most;
         if (chunks < 1) chunks = 1;
-        p.chunk[w] = ((rows + chunks - 1) / chunks + 15) / 16 * 16;
-        if (p.chunk[w] == 0) p.chunk[w] = 16;
+        p.chunk[w] = ((rows + chunks - 1) / chunks + kRows - 1) / kRows * kRows;
+        if (p.chunk[w] == 0) p.chunk[w] = kRows;
         p.chunks[w] = rows ? (rows + p.chunk[w] - 1) / p.chunk[w] : 1;
         if (p.chunks[w] > 1)
             p.part[w] = sizeof(float) * static_cast<size_t>((p.chunks[w] + s - 1) * r *
@@ -370,26 +628,38 @@ WgradPlan lr_wgrad_plan(int64_t rows, int64_t r, int64_t s, int64_t cols_a, int6
 }
 
 template <typename T>
-static cudaError_t wgrad(const WgradParams &P, int num_sms, cudaStream_t stream) {
-    const int nj = P.r <= 16 ? 1 : 2;
-    const int64_t units = P.side[0].blocks * P.side[0].chunks + P.side[1].blocks * P.side[1].chunks;
-    const dim3 grid(static_cast<unsigned>(units),
-                    static_cast<unsigned>((P.r + 16 * nj - 1) / (16 * nj)));
-    auto kernel = nj == 1 ? wgrad_kernel<T, 1> : wgrad_kernel<T, 2>;
-    const size_t smem = nj == 1 ? wgrad_smem<1>() : wgrad_smem<2>();
-    static PerDevice<int> ready[2];
-    std::atomic<int> *set = ready[nj - 1].here();
+static cudaError_t wgrad(WgradParams &P, int num_sms, cudaStream_t stream) {
+    P.rp = P.r >= kBlockRanks ? kBlockRanks : static_cast<int>((P.r + 15) / 16 * 16);
+    const int type = std::is_same<T, __half>::value ? 0 : 1;
+    P.idesc = (1u << 4) | (static_cast<uint32_t>(type) << 7) | (static_cast<uint32_t>(type) << 10) |
+              (1u << 15) | (static_cast<uint32_t>(P.rp >> 3) << 17) | ((128u >> 4) << 24);
+    Maps maps;
+    std::memset(&maps, 0, sizeof(maps));
+    int64_t units = 0;
+    for (int w = 0; w < 2; ++w) {
+        const Side &S = P.side[w];
+        units += S.blocks * S.chunks;
+        // (without rows the sums are zeros and nothing is copied)
+        if (S.blocks && P.rows &&
+            (!make_map16(&maps.tile[w], S.M, S.cols, P.rows, S.ld, 64, kRows) ||
+             !make_map16(&maps.row[w], S.M, S.cols, P.rows, S.ld, 64, 1)))
+            return cudaErrorInvalidValue;
+    }
+    static PerDevice<int> ready;
+    std::atomic<int> *set = ready.here();
     if (!set) return cudaErrorInvalidDevice;
     if (!set->load(std::memory_order_acquire)) {
         const cudaError_t e = cudaFuncSetAttribute(
-            kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+            wgrad_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kSmem));
         if (e != cudaSuccess) return e;
         set->store(1, std::memory_order_release);
     }
-    kernel<<<grid, kThreads, smem, stream>>>(P);
+    const dim3 grid(static_cast<unsigned>(units),
+                    static_cast<unsigned>((P.r + kBlockRanks - 1) / kBlockRanks));
+    wgrad_kernel<T><<<grid, kThreads, kSmem, stream>>>(maps, P);
     if (P.side[0].part || P.side[1].part) {
         const int64_t cols = P.side[0].cols > P.side[1].cols ? P.side[0].cols : P.side[1].cols;
-        const int64_t want = (P.s * P.r * ((cols + 3) / 4) + 255) / 256, most = int64_t(num_sms) * 4;
+        const int64_t want = P.s * ((P.r + 31) / 32) * ((cols + 31) / 32), most = int64_t(num_sms) * 8;
         join_kernel<T><<<dim3(static_cast<unsigned>(want < most ? want : most), 2), 256, 0, stream>>>(P);
     }
     return cudaGetLastError();
@@ -397,8 +667,9 @@ static cudaError_t wgrad(const WgradParams &P, int num_sms, cudaStream_t stream)
 
 cudaError_t lr_wgrad(bool half, const WgradOperand &a, const WgradOperand &b, int64_t rows,
                      int64_t r, const RowIndex &index, const WgradPlan &plan, void *lists,
-                     int num_sms, cudaStream_t stream) {
+                     int num_sms, int *err, cudaStream_t stream) {
     WgradParams P{};
+    P.err = err;
     P.rows = rows;
     P.r = r;
     P.s = index.s;
