@@ -27,7 +27,7 @@
 //
 // Roles (both CTAs): warp 0 TMA producer; warp 1 TMEM allocation and, in CTA 0, the MMA issuer;
 // warps 2..9 epilogue, two per TMEM lane quadrant with 128 columns each; warps 10..13 loaders of the
-// low-rank steps, which have their own stage, so they fill it while the product's steps run.  A
+// low-rank steps, which have two stages of their own and fill them while the product's steps run.  A
 // low-rank step is taken after every `every` steps of the product while any are left: a fixed
 // order, so results repeat bit for bit, and far enough apart that the loaders are ready (8192^3,
 // r = 32, whole call: 990 us with 4, 935 us with 16).  The kernel may start before the projection has finished
@@ -46,15 +46,15 @@ namespace {
 constexpr int kBM = 256, kBN = 256, kBK = 64;
 constexpr int kHalf = 128;                       // rows of M and columns of W per CTA
 constexpr int kABytes = kHalf * kBK * 2, kBBytes = kHalf * kBK * 2;
-constexpr int kStageBytes = kABytes + kBBytes, kStages = 6;
+constexpr int kStageBytes = kABytes + kBBytes, kStages = 5;
 constexpr int kLowBytes = 2 * kHalf * 128;       // one low-rank step per CTA: rows of P, rows of F
 constexpr int kEpiWarps = 8, kLoaders = 128;
 constexpr int kThreads = 64 + 32 * kEpiWarps + kLoaders;
 constexpr uint32_t kTmemCols = 512;
 constexpr int kGroupM = 8;                       // raster: 8 row tiles (2048 rows) at a time
 constexpr int kRankStep = 16;
-constexpr int kFixSlots = 8;
-constexpr size_t kSmem = size_t(kStages) * kStageBytes + kLowBytes + 1024 + 512;
+constexpr int kFixSlots = 16;
+constexpr size_t kSmem = size_t(kStages) * kStageBytes + 2 * kLowBytes + 1024 + 512;
 
 struct Params {
     int64_t rows, cols;
@@ -243,19 +243,19 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     uint8_t *sA = smem;
     uint8_t *sB = sA + kStages * kABytes;
-    uint8_t *sP = sB + kStages * kBBytes;   // low-rank step: 128 rows of P, hi | lo
-    uint8_t *sF = sP + kHalf * 128;               //                kCols rows of F
-    uint64_t *full = reinterpret_cast<uint64_t *>(sF + kHalf * 128);  // CTA 0
+    uint8_t *sLow = sB + kStages * kBBytes;  // two low-rank steps: 128 rows of P, hi | lo, then
+                                             // 128 rows of F
+    uint64_t *full = reinterpret_cast<uint64_t *>(sLow + 2 * kLowBytes);  // CTA 0
     uint64_t *empty = full + kStages;
     uint64_t *tfull = empty + kStages;   // [2] both CTAs: accumulator ready
     uint64_t *tempty = tfull + 2;           // [2] CTA 0: drained by both epilogues
-    uint64_t *lfull = tempty + 2;           // CTA 0: low-rank step written in both CTAs
-    uint64_t *lempty = lfull + 1;           // both CTAs: low-rank step taken
-    uint64_t *drain = lempty + 1;
+    uint64_t *lfull = tempty + 2;           // [2] CTA 0: low-rank step written in both CTAs
+    uint64_t *lempty = lfull + 2;           // [2] both CTAs: low-rank step taken
+    uint64_t *drain = lempty + 2;
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(drain + 1);
     volatile int *abort = reinterpret_cast<volatile int *>(tmem_slot + 1);
-    volatile int *message = abort + 1;      // CTA 0: 8-wide steps in this low-rank step, 0: no more
-    volatile int *fix = message + 1;        // [kFixSlots] by tile: entries that are not finite
+    volatile int *message = abort + 1;      // [2] CTA 0: 8-wide steps in a low-rank step, 0: no more
+    volatile int *fix = message + 2;        // [kFixSlots] by tile: entries that are not finite
     int *least = const_cast<int *>(fix) + kFixSlots;  // [2][4] loaders' smallest adapter, by warp
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -270,9 +270,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         for (int a = 0; a < 2; ++a) {
             mbar_init(&tfull[a], 1);
             mbar_init(&tempty[a], 2 * kEpiWarps);
+            mbar_init(&lfull[a], 2);
+            mbar_init(&lempty[a], 1);
         }
-        mbar_init(lfull, 2);
-        mbar_init(lempty, 1);
         mbar_init(drain, 1);
         *abort = 0;
         for (int f = 0; f < kFixSlots; ++f) fix[f] = 0;
@@ -341,11 +341,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         if (lane == 0 && rank == 0) {
             // ---------------- MMA issuer (CTA 0) ----------------
             int stage = 0;
-            uint32_t phase = 0, lphase = 0;
+            uint32_t phase = 0, taken = 0;  // low-rank steps taken: stage taken % 2
             bool ok = true, any_issued = false;
             int64_t unit = 0;
-            const uint64_t pdesc = make_sw128_kmajor_desc(smem_u32(sP));
-            const uint64_t fdesc = make_sw128_kmajor_desc(smem_u32(sF));
             tiles(P, [&](int, int) {
                 const int acc = static_cast<int>(unit % kBuffers);
                 const uint32_t acc_phase = static_cast<uint32_t>((unit / kBuffers) & 1);
@@ -363,21 +361,25 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                 uint32_t have_low = kDrop ? 0u : 1u;  // the low-rank accumulator holds something
                 // takes one low-rank step, or the loaders' word that there are no more
                 auto low_step = [&]() {
-                    if (!mbar_wait_cluster(lfull, lphase, abort)) {
+                    const uint32_t at = taken & 1;
+                    if (!mbar_wait_cluster(&lfull[at], (taken >> 1) & 1, abort)) {
                         raise(P, abort, kErrTimeoutMma);
                         ok = false;
                         return false;
                     }
-                    lphase ^= 1;
+                    ++taken;
                     tc_fence_after();
-                    const int n8 = *message;
+                    const int n8 = message[at];
+                    const uint32_t low = smem_u32(sLow + at * kLowBytes);
+                    const uint64_t pdesc = make_sw128_kmajor_desc(low);
+                    const uint64_t fdesc = make_sw128_kmajor_desc(low + kHalf * 128);
                     for (int part = 0; part < 2; ++part)  // upper bits, then the rest
                         for (int h = 0; h < n8; ++h) {
                             umma_tf32_pair(dlow, pdesc + 4 * part + 2 * h, fdesc + 2 * h,
                                            P.idesc32, have_low);
                             have_low = 1;
                         }
-                    umma_commit_pair(lempty);
+                    umma_commit_pair(&lempty[at]);
                     more = n8 != 0;
                     return true;
                 };
@@ -513,16 +515,15 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     } else {
         // ---------------- loaders of the low-rank steps (warps 10..13, both CTAs) ----------------
         const int lt = threadIdx.x - 32 * (2 + kEpiWarps);
-        const uint32_t lfull0 = map_to_rank(smem_u32(lfull), 0);
         int64_t unit = 0;
-        uint32_t phase = 0;
+        uint32_t sent = 0;  // low-rank steps and closing words sent: stage sent % 2
         int turn = 0;
         const uint16_t *F = static_cast<const uint16_t *>(P.F.p);
         asm volatile("griddepcontrol.wait;" ::: "memory");  // the projection is complete
         tiles(P, [&](int tm, int tn) {
             const int slot = static_cast<int>(unit % kFixSlots);
-            // Cleared half a round ahead: the other CTA's loaders may raise the flag of the next
-            // tile already, and the epilogue is past the tile that used this slot before.
+            // Cleared half a round ahead: the other CTA's loaders may be two tiles ahead and raise
+            // their flag already, and the epilogue is past the tile that used this slot before.
             if (lt == 0) fix[(unit + kFixSlots / 2) % kFixSlots] = 0;
             ++unit;
             const int64_t row0 = int64_t(tm) * kBM + lt;  // this thread's rows of the pair's tile
@@ -599,9 +600,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                         p[j] = hi;
                     }
                     // a wait that gave up is acted on at the barrier, by all loaders alike
-                    const bool gave_up = !mbar_wait(lempty, phase ^ 1, abort);
+                    const uint32_t at = sent & 1;
+                    const bool gave_up = !mbar_wait(&lempty[at], ((sent >> 1) & 1) ^ 1, abort);
                     if (gave_up) raise(P, abort, kErrTimeoutProducer);
-                    phase ^= 1;
+                    ++sent;
+                    uint8_t *sP = sLow + at * kLowBytes, *sF = sP + kHalf * 128;
 #pragma unroll
                     for (int c = 0; c < 4; ++c) {
                         *swizzled(sP, lt, c) =
@@ -614,19 +617,20 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                     if (odd)  // in both CTAs: a row of one meets columns of the other
                         for (uint32_t c = 0; c < 2; ++c)
                             store_flag(map_to_rank(smem_u32(const_cast<const int *>(&fix[slot])), c));
-                    if (lt == 0) *message = (nj + 7) / 8;
+                    if (lt == 0) message[at] = (nj + 7) / 8;
                     fence_proxy_async_smem();
                     if (loader_sync_or(gave_up)) return false;
-                    if (lt == 0) mbar_arrive_remote(lfull0);
+                    if (lt == 0) mbar_arrive_remote(map_to_rank(smem_u32(&lfull[at]), 0));
                 }
             }
-            const bool gave_up = !mbar_wait(lempty, phase ^ 1, abort);
+            const uint32_t at = sent & 1;
+            const bool gave_up = !mbar_wait(&lempty[at], ((sent >> 1) & 1) ^ 1, abort);
             if (gave_up) raise(P, abort, kErrTimeoutProducer);
-            phase ^= 1;
+            ++sent;
             if (loader_sync_or(gave_up)) return false;
             if (lt == 0) {
-                *message = 0;
-                mbar_arrive_remote(lfull0);
+                message[at] = 0;
+                mbar_arrive_remote(map_to_rank(smem_u32(&lfull[at]), 0));
             }
             return true;
         });

@@ -37,10 +37,10 @@ struct ProjectParams {
 
 constexpr int kTileRows = 128, kBK = 64;
 constexpr int kWorkers = 256, kTileThreads = 64 + kWorkers;  // copies, MMA issue, 8 workers
-constexpr int kMBytes = kTileRows * kBK * 2, kFBytes = 16384;  // per stage
-constexpr int kStageBytes = kMBytes + kFBytes, kStages = 5;
+constexpr int kMBytes = kTileRows * kBK * 2, kFBytes = 32768;  // per stage
+constexpr int kStageBytes = kMBytes + kFBytes, kStages = 4;
 constexpr int kBlockRanks = 64;  // ranks of one CTA
-constexpr uint32_t kTmemCols = 128;
+constexpr uint32_t kTmemCols = 256;  // kFBytes / 128 ranks
 constexpr size_t kTileSmem = size_t(kStages) * kStageBytes + sizeof(float) * kTileRows * kBlockRanks +
                              1024 + 1024 + 512;
 
