@@ -519,6 +519,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         uint32_t sent = 0;  // low-rank steps and closing words sent: stage sent % 2
         int turn = 0;
         const uint16_t *F = static_cast<const uint16_t *>(P.F.p);
+        const int r = static_cast<int>(P.r);
         asm volatile("griddepcontrol.wait;" ::: "memory");  // the projection is complete
         tiles(P, [&](int tm, int tn) {
             const int slot = static_cast<int>(unit % kFixSlots);
@@ -532,9 +533,19 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             const int mine = rank ? i1 : i0;
             const int64_t row = row0 + int64_t(rank) * kHalf;
             const int64_t col = int64_t(tn) * kBN + int64_t(rank) * kHalf + lt;
-            int cur = -1;
-            while (true) {
-                // the next adapter in increasing order: the smallest index above `cur`
+            // a step's reads: 16 ranks of the thread's row and column, as they lie in memory
+            struct Reads {
+                float4 p[4];
+                uint32_t f[kRankStep];  // 8 packed words, or 16 elements
+                int nj;
+            };
+            int cur = -1, j0 = r;
+            // The next step: 16 ranks further, or the next adapter in increasing order (the smallest
+            // index above `cur` among the pair's rows).
+            auto advance = [&]() {
+                j0 += kRankStep;
+                if (j0 < r) return true;
+                j0 = 0;
                 const unsigned none = 0x7FFFFFFFu;
                 const unsigned c0 = i0 > cur ? static_cast<unsigned>(i0) : none;
                 const unsigned c1 = i1 > cur ? static_cast<unsigned>(i1) : none;
@@ -544,84 +555,97 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                 const int *l = least + 4 * turn;
                 turn ^= 1;
                 cur = min(min(l[0], l[1]), min(l[2], l[3]));
-                if (cur == static_cast<int>(none)) break;
-                for (int64_t j0 = 0; j0 < P.r; j0 += kRankStep) {
-                    const int nj = static_cast<int>(min(int64_t(kRankStep), P.r - j0));
-                    float p[kRankStep], f[kRankStep];
-                    bool odd = false;
-                    const float *prow = P.P + row * P.r + j0;
-                    const bool take = mine == cur;
+                return cur != static_cast<int>(none);
+            };
+            auto fetch = [&](Reads &x) {
+                x.nj = min(kRankStep, r - j0);
+                const float *prow = P.P + row * P.r + j0;
+                const bool take = mine == cur;
 #pragma unroll
-                    for (int j = 0; j < kRankStep; j += 4) {
-                        float4 w = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                        if (P.pvec) {  // r is a multiple of 4
-                            if (take && j < nj) w = *reinterpret_cast<const float4 *>(prow + j);
-                        } else if (take) {
-                            if (j < nj) w.x = prow[j];
-                            if (j + 1 < nj) w.y = prow[j + 1];
-                            if (j + 2 < nj) w.z = prow[j + 2];
-                            if (j + 3 < nj) w.w = prow[j + 3];
-                        }
-                        p[j] = w.x, p[j + 1] = w.y, p[j + 2] = w.z, p[j + 3] = w.w;
+                for (int q = 0; q < 4; ++q) {
+                    const int j = 4 * q;
+                    x.p[q] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                    if (P.pvec) {  // r is a multiple of 4
+                        if (take && j < x.nj) x.p[q] = *reinterpret_cast<const float4 *>(prow + j);
+                    } else if (take) {
+                        if (j < x.nj) x.p[q].x = prow[j];
+                        if (j + 1 < x.nj) x.p[q].y = prow[j + 1];
+                        if (j + 2 < x.nj) x.p[q].z = prow[j + 2];
+                        if (j + 3 < x.nj) x.p[q].w = prow[j + 3];
                     }
-                    const uint16_t *src = F + cur * P.F.ss + col * P.F.sc + j0 * P.F.sr;
+                }
+                const uint16_t *src = F + cur * P.F.ss + col * P.F.sc + j0 * P.F.sr;
+                const int n = col < P.cols ? x.nj : 0;
+                if (P.fvec) {
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
-                        const int n = col < P.cols ? nj - 8 * h : 0;
-                        uint4 w = make_uint4(0, 0, 0, 0);
-                        if (P.fvec && n >= 8) {
-                            w = __ldg(reinterpret_cast<const uint4 *>(src + 8 * h));
-                        } else {
-                            uint32_t u[4] = {0, 0, 0, 0};
-#pragma unroll
-                            for (int e = 0; e < 8; ++e)
-                                if (e < n)
-                                    u[e >> 1] |= static_cast<uint32_t>(__ldg(src + (8 * h + e) * P.F.sr))
-                                                 << (16 * (e & 1));
-                            w = make_uint4(u[0], u[1], u[2], u[3]);
-                        }
-                        unpack8<T>(w, *reinterpret_cast<float(*)[8]>(&f[8 * h]));
+                        const uint4 w = load8(src + 8 * h, n - 8 * h);
+                        x.f[4 * h] = w.x, x.f[4 * h + 1] = w.y;
+                        x.f[4 * h + 2] = w.z, x.f[4 * h + 3] = w.w;
                     }
+                } else {
 #pragma unroll
-                    for (int j = 0; j < kRankStep; ++j)
-                        if (!finite(f[j])) {
-                            odd = true;
-                            f[j] = 0.0f;
-                        }
-                    float lo[kRankStep];
-#pragma unroll
-                    for (int j = 0; j < kRankStep; ++j) {
-                        if (!finite(p[j])) {
-                            odd = true;
-                            p[j] = 0.0f;
-                        }
-                        const float hi = __uint_as_float(__float_as_uint(p[j]) & 0xFFFFE000u);
-                        lo[j] = p[j] - hi;  // exact
-                        p[j] = hi;
-                    }
-                    // a wait that gave up is acted on at the barrier, by all loaders alike
-                    const uint32_t at = sent & 1;
-                    const bool gave_up = !mbar_wait(&lempty[at], ((sent >> 1) & 1) ^ 1, abort);
-                    if (gave_up) raise(P, abort, kErrTimeoutProducer);
-                    ++sent;
-                    uint8_t *sP = sLow + at * kLowBytes, *sF = sP + kHalf * 128;
-#pragma unroll
-                    for (int c = 0; c < 4; ++c) {
-                        *swizzled(sP, lt, c) =
-                            make_float4(p[4 * c], p[4 * c + 1], p[4 * c + 2], p[4 * c + 3]);
-                        *swizzled(sP, lt, 4 + c) =
-                            make_float4(lo[4 * c], lo[4 * c + 1], lo[4 * c + 2], lo[4 * c + 3]);
-                        *swizzled(sF, lt, c) =
-                            make_float4(f[4 * c], f[4 * c + 1], f[4 * c + 2], f[4 * c + 3]);
-                    }
-                    if (odd)  // in both CTAs: a row of one meets columns of the other
-                        for (uint32_t c = 0; c < 2; ++c)
-                            store_flag(map_to_rank(smem_u32(const_cast<const int *>(&fix[slot])), c));
-                    if (lt == 0) message[at] = (nj + 7) / 8;
-                    fence_proxy_async_smem();
-                    if (loader_sync_or(gave_up)) return false;
-                    if (lt == 0) mbar_arrive_remote(map_to_rank(smem_u32(&lfull[at]), 0));
+                    for (int e = 0; e < kRankStep; ++e) x.f[e] = e < n ? __ldg(src + e * P.F.sr) : 0;
                 }
+            };
+            auto send = [&](const Reads &x) {
+                float p[kRankStep], lo[kRankStep], f[kRankStep];
+                bool odd = false;
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    p[4 * q] = x.p[q].x, p[4 * q + 1] = x.p[q].y;
+                    p[4 * q + 2] = x.p[q].z, p[4 * q + 3] = x.p[q].w;
+                }
+#pragma unroll
+                for (int j = 0; j < kRankStep; ++j) {
+                    const uint32_t w = P.fvec ? x.f[j >> 1] >> (16 * (j & 1)) : x.f[j];
+                    const uint16_t h = static_cast<uint16_t>(w);
+                    f[j] = to_float(*reinterpret_cast<const T *>(&h));
+                    if (!finite(f[j])) {
+                        odd = true;
+                        f[j] = 0.0f;
+                    }
+                    if (!finite(p[j])) {
+                        odd = true;
+                        p[j] = 0.0f;
+                    }
+                    const float hi = __uint_as_float(__float_as_uint(p[j]) & 0xFFFFE000u);
+                    lo[j] = p[j] - hi;  // exact
+                    p[j] = hi;
+                }
+                // a wait that gave up is acted on at the barrier, by all loaders alike
+                const uint32_t at = sent & 1;
+                const bool gave_up = !mbar_wait(&lempty[at], ((sent >> 1) & 1) ^ 1, abort);
+                if (gave_up) raise(P, abort, kErrTimeoutProducer);
+                ++sent;
+                uint8_t *sP = sLow + at * kLowBytes, *sF = sP + kHalf * 128;
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    *swizzled(sP, lt, c) =
+                        make_float4(p[4 * c], p[4 * c + 1], p[4 * c + 2], p[4 * c + 3]);
+                    *swizzled(sP, lt, 4 + c) =
+                        make_float4(lo[4 * c], lo[4 * c + 1], lo[4 * c + 2], lo[4 * c + 3]);
+                    *swizzled(sF, lt, c) =
+                        make_float4(f[4 * c], f[4 * c + 1], f[4 * c + 2], f[4 * c + 3]);
+                }
+                if (odd)  // in both CTAs: a row of one meets columns of the other
+                    for (uint32_t c = 0; c < 2; ++c)
+                        store_flag(map_to_rank(smem_u32(const_cast<const int *>(&fix[slot])), c));
+                if (lt == 0) message[at] = (x.nj + 7) / 8;
+                fence_proxy_async_smem();
+                if (loader_sync_or(gave_up)) return false;
+                if (lt == 0) mbar_arrive_remote(map_to_rank(smem_u32(&lfull[at]), 0));
+                return true;
+            };
+            // the next step's reads are on their way while one is written
+            Reads now, next;
+            bool have = advance();
+            if (have) fetch(now);
+            while (have) {
+                have = advance();
+                if (have) fetch(next);
+                if (!send(now)) return false;
+                now = next;
             }
             const uint32_t at = sent & 1;
             const bool gave_up = !mbar_wait(&lempty[at], ((sent >> 1) & 1) ^ 1, abort);
