@@ -17,6 +17,14 @@ from tensor_inv_b200 import _native as nat
 TYPES = [torch.bfloat16, torch.float16]
 
 
+@pytest.fixture(autouse=True)
+def no_device_error(request):
+    """No kernel gave up on a wait."""
+    yield
+    if request.node.get_closest_marker("gpu"):
+        assert nat.device_error() == 0
+
+
 def operands(T, K, N, S, r, dtype=torch.bfloat16, whole=True, outer=False, pad=0, seed=0,
              device="cuda", rows="mixed"):
     """X, W, A, B, index, scale, dY; outer: factors stored transposed; pad: rows of X and dY cut out
