@@ -45,8 +45,8 @@ enum { kFScalar = 0, kFC = 1, kFR = 2 };
 
 inline int factor_mode(const Factor16 &F) {
     const bool base = (reinterpret_cast<uintptr_t>(F.p) & 15) == 0 && F.ss % 8 == 0;
-    if (base && F.sc == 1 && F.sr % 8 == 0) return kFC;
-    if (base && F.sr == 1 && F.sc % 8 == 0) return kFR;
+    if (base && F.sc == 1 && F.sr % 8 == 0 && F.sr > 0) return kFC;
+    if (base && F.sr == 1 && F.sc % 8 == 0 && F.sc > 0) return kFR;
     return kFScalar;
 }
 

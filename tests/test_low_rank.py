@@ -6,12 +6,16 @@ made of the roundings that the kernels do (``bound`` below).
 """
 
 import ctypes
+import subprocess
+import sys
+import threading
 
 import pytest
 import torch
 
 import low_rank_reference as ref
 import tensor_inv_b200 as ti
+from conftest import ROOT
 from tensor_inv_b200 import _native as nat
 
 TYPES = [torch.bfloat16, torch.float16]
@@ -456,6 +460,147 @@ def test_factors_of_a_weight_difference():
     assert torch.isfinite(A.grad).all() and torch.isfinite(B.grad).all()
     assert (B.grad[1] != 0).any() and (A.grad[1] == 0).all()  # B[1] is zero, so A[1] has no slope
     assert nat.device_error() == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T", [5, 300])
+def test_odd_layouts_of_factors(T):
+    """Adapters whose ranks or columns are the slowest dimension, and operands that repeat one row or
+    column (stride 0)."""
+    K, N, S, r = 72, 136, 4, 16
+    X, W, A, B, index, scale, dY = operands(T, K, N, S, r, seed=1)
+    for a, b in ((A.permute(2, 0, 1).contiguous().permute(1, 2, 0),
+                  B.permute(2, 0, 1).contiguous().permute(1, 2, 0)),
+                 (A.permute(1, 0, 2).contiguous().permute(1, 0, 2),
+                  B.permute(1, 0, 2).contiguous().permute(1, 0, 2)),
+                 (A[:, :, :1].expand(S, K, r), B[:, :, :1].expand(S, r, N)),
+                 (A[:, :1].expand(S, K, r), B[:, :1].expand(S, r, N))):
+        check_forward((X, W, a, b, index, scale, dY))
+        check_backward((X, W, a, b, index, scale, dY), p=0.5, seed=1)
+    ops = X[:1].expand(T, K), W[:, :1].expand(K, N), A, B, index, scale, dY[:, :1].expand(T, N)
+    check_forward(ops)
+    check_backward(ops, p=0.5, seed=1)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T", [3, 100, 300])
+def test_everything_dropped(T):
+    ops = operands(T, 72, 136, 4, 16, seed=1)
+    check_forward(ops, p=1.0, seed=3)
+    check_backward(ops, p=1.0, seed=3)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T", [10, 300])
+def test_gradients_of_empty_dimensions(T):
+    X, W, A, B, index, scale, dY = operands(T, 32, 24, 3, 4)
+    for K, N in ((0, 24), (32, 0)):
+        a, b = A[:, :K], B[:, :, :N]
+        grads = ti.low_rank_matmul_backward(dY[:, :N], X[:, :K], W[:K, :N], a, b, index, scale)
+        for G, shape in zip(grads, ((T, K), a.shape, b.shape)):
+            assert G.shape == shape and (G == 0).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("size", [
+    (300, 64, 72, 300, 8), (1000, 72, 64, 1000, 5), (600, 264, 136, 3, 256), (40000, 64, 72, 5, 8),
+    (5000, 40, 24, 1, 16), (129, 64, 64, 1, 16), (8200, 64, 64, 9, 16)])
+def test_many_adapters_many_rows(size):
+    """As many adapters as rows, the largest rank, many tiles of few columns, the first rows past a
+    rule's border."""
+    ops = operands(*size, seed=3, pad=5)
+    check_forward(ops)
+    check_backward(ops, p=0.5, seed=2)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("size", [(300, 70000, 8, 2, 4), (20, 70000, 8, 2, 4), (300, 8, 70000, 2, 4)])
+def test_long_dimensions(size):
+    """Inner and outer dimensions past 2^16; factors thinned out so that sums stay below 2^24."""
+    X, W, A, B, index, scale, dY = operands(*size, seed=3)
+    g = torch.Generator("cuda").manual_seed(1)
+    A = torch.where(torch.rand(A.shape, device="cuda", generator=g) < 0.02, A, 0)
+    B = torch.where(torch.rand(B.shape, device="cuda", generator=g) < 0.02, B, 0)
+    check_forward((X, W, A, B, index, scale, dY))
+    check_backward((X, W, A, B, index, scale, dY), p=0.5, seed=2)
+
+
+@pytest.mark.gpu
+def test_a_broadcast_gradient():
+    """Y.sum() hands an expanded gradient (strides 0) to the backward pass."""
+    X, W, A, B, index, scale, dY = operands(300, 72, 136, 4, 16, seed=1)
+    A.requires_grad_()
+    X.requires_grad_()
+    ti.low_rank_matmul(X, W, A, B, index, scale).sum().backward()
+    exact = ref.backward(torch.ones_like(dY), X, W, A, B, index, scale)
+    assert torch.equal(X.grad.cpu(), exact[0].to(X.dtype))
+    assert torch.equal(A.grad.cpu(), exact[1].to(X.dtype))
+
+
+@pytest.mark.gpu
+def test_calls_from_several_threads():
+    ops = [operands(300 + i, 72, 136, 4, 16, seed=i) for i in range(4)]
+    want = [(ti.low_rank_matmul(*o[:6]), *ti.low_rank_matmul_backward(o[6], *o[:6])) for o in ops]
+    torch.cuda.synchronize()
+    wrong = []
+
+    def work(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(20):
+                got = (ti.low_rank_matmul(*ops[i][:6]),
+                       *ti.low_rank_matmul_backward(ops[i][6], *ops[i][:6]))
+                torch.cuda.current_stream().synchronize()
+                if not all(torch.equal(a, b) for a, b in zip(got, want[i])):
+                    wrong.append(i)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong
+
+
+CAPTURES = """
+import sys, torch
+sys.path.insert(0, {root!r})
+import tensor_inv_b200 as ti
+def ones(*shape):
+    return torch.ones(*shape, device="cuda").bfloat16()
+X, W, A, B = ones(300, 64), ones(64, 64), ones(2, 64, 8), ones(2, 8, 64)
+index = torch.zeros(300, dtype=torch.int64, device="cuda")
+if {first}:  # the process's first calls are captured ones
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        Y = ti.low_rank_matmul(X, W, A, B, index)
+        y = ti.low_rank_matmul(X[:3], W, A, B, index[:3])
+        grads = ti.low_rank_matmul_backward(X, X, W, A, B, index)
+    graph.replay()
+    assert (Y == 576).all() and (y == 576).all() and (grads[0] == 576).all()
+else:  # a backward pass captured while an eager graph of the same leaves lives
+    A.requires_grad_()
+    kept = ti.low_rank_matmul(X, W, A, B, index)
+    Y = ti.low_rank_matmul(X, W, A, B, index)
+    kept.backward(torch.ones_like(Y), retain_graph=True)
+    torch.cuda.synchronize()
+    try:
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            Y.backward(torch.ones_like(Y))
+        raise SystemExit("captured")
+    except RuntimeError:
+        pass
+    assert (ti.low_rank_matmul(X, W, A, B, index) == 576).all()
+torch.cuda.synchronize()
+print("fine")
+"""
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("first", [True, False])
+def test_captures_in_a_process_of_their_own(first):
+    code = CAPTURES.format(root=str(ROOT), first=first)
+    done = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300)
+    assert done.returncode == 0 and "fine" in done.stdout, done.stderr[-2000:]
 
 
 # ---------------------------------------------------------------------------------------
