@@ -37,7 +37,7 @@
 #include <cstring>
 #include <type_traits>
 
-#include "ti_lr_dot.cuh"
+#include "ti_lr_loads.cuh"
 #include "ti_lr_launch.cuh"
 
 namespace ti {

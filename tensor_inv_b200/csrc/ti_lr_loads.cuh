@@ -1,4 +1,4 @@
-// ti_lr_dot.cuh -- loads and small pieces shared by the kernels of the low-rank products.
+// ti_lr_loads.cuh -- loads and small pieces shared by the kernels of the low-rank products.
 #pragma once
 
 #include <type_traits>

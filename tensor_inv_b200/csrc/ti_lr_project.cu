@@ -15,7 +15,7 @@
 #include <atomic>
 #include <cstring>
 
-#include "ti_lr_dot.cuh"
+#include "ti_lr_loads.cuh"
 #include "ti_lr_launch.cuh"
 
 namespace ti {

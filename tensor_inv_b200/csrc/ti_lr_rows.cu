@@ -24,7 +24,7 @@
 #include <cstring>
 #include <type_traits>
 
-#include "ti_lr_dot.cuh"
+#include "ti_lr_loads.cuh"
 #include "ti_lr_launch.cuh"
 
 namespace ti {
@@ -36,6 +36,7 @@ constexpr int kThreads = 64 + kLowThreads;
 constexpr int kWBytes = kCols * kBK * 2;  // 16 KB
 constexpr int kEarly = 2;                 // copies that do not wait for the reads of F
 constexpr int kBatch = 4;                 // rows of a group whose reads of F overlap
+constexpr int kProjBytes = 24 * 1024;     // the served rows' projections, as far as they fit
 
 template <int kNT>
 struct Shape {
@@ -46,9 +47,10 @@ struct Shape {
     // and the serving CTA adds its own part to it.
     static constexpr bool kLowApart = kNT < 128;
     static constexpr int kPartBytes = (kLowApart ? 2 * kNT : kNT + 8) * kCols * 4;
-    static constexpr int kStages = kNT <= 32 ? 8 : kNT == 64 ? 6 : 4;
-    static constexpr size_t kSmem =
-        size_t(kStages) * kStageBytes + kPartBytes + 1024 + 256 + sizeof(int) * kNT;
+    // four stages stream W as fast as nine do
+    static constexpr int kStages = 4;
+    static constexpr size_t kSmem = size_t(kStages) * kStageBytes + kPartBytes + kProjBytes + 1024 +
+                                    256 + sizeof(int) * kNT;
     static constexpr uint32_t kTmemCols = kNT < 32 ? 32 : kNT;
 };
 
@@ -148,7 +150,8 @@ __global__ void __launch_bounds__(kThreads, 2)
     uint8_t *sW = smem;
     uint8_t *sM = sW + S::kStages * kWBytes;
     float *part = reinterpret_cast<float *>(sM + S::kStages * S::kMBytes);
-    uint64_t *full = reinterpret_cast<uint64_t *>(part + S::kPartBytes / 4);
+    float *proj = part + S::kPartBytes / 4;
+    uint64_t *full = reinterpret_cast<uint64_t *>(proj + kProjBytes / 4);
     uint64_t *empty = full + S::kStages;
     uint64_t *tfull = empty + S::kStages;
     uint64_t *drain = tfull + 1;
@@ -276,6 +279,10 @@ __global__ void __launch_bounds__(kThreads, 2)
         const DropoutKeys key(kDrop ? dropout_key(P.drop) : 0);
         if (lt < kNT) sidx[lt] = adapter;
         low_sync();
+        // Served row k's projection lies at proj[k * r]; where they do not all fit they are read from
+        // memory each time (and every read of a step is waited for).
+        const int served = (here - rank + csize - 1) / csize;
+        const bool staged = served * P.r * 4 <= kProjBytes;
         // the served rows k = group, group + 2, ..., kBatch of them at a time
         bool waited = false;
         for (int k0 = group; rank + csize * k0 < here || !waited; k0 += 2 * kBatch) {
@@ -305,11 +312,18 @@ __global__ void __launch_bounds__(kThreads, 2)
                                     col * P.F.sc));
                         }
                     asm volatile("griddepcontrol.wait;" ::: "memory");  // the projection is complete
+                    if (staged) {
+                        for (int e = lt; e < served * P.r; e += kLowThreads)
+                            proj[e] = P.P[(row0 + rank + csize * (e / P.r)) * P.r + e % P.r];
+                        low_sync();
+                    }
                 }
 #pragma unroll
                 for (int u = 0; u < kBatch; ++u) {
                     if (i[u] < 0) continue;
-                    const float *p = P.P + (row0 + rank + csize * (k0 + 2 * u)) * P.r + j0;
+                    const float *p =
+                        staged ? proj + (k0 + 2 * u) * P.r + j0
+                               : P.P + (row0 + rank + csize * (k0 + 2 * u)) * P.r + j0;
                     float v[16];
                     unpack8<T>(f[u][0], *reinterpret_cast<float(*)[8]>(&v[0]));
                     unpack8<T>(f[u][1], *reinterpret_cast<float(*)[8]>(&v[8]));

@@ -25,7 +25,7 @@
 // (An infinity in M meets both parts of V, so its column comes out infinite or NaN.)
 #include <cstring>
 
-#include "ti_lr_dot.cuh"
+#include "ti_lr_loads.cuh"
 #include "ti_lr_launch.cuh"
 
 namespace ti {
