@@ -9,7 +9,8 @@
 //
 // The low-rank term is a few multiply-adds per output and runs on the plain cores while the copies
 // of W are in flight: thread c of the serving CTA holds column c, and the row's P meets its
-// adapter's F in float32.  It reads only the adapters that rows ask for, each once per row, and
+// adapter's F in float32 (where F's vectors run along the columns, a lane reads four columns of a
+// quarter of the ranks: 48 x 4096 x 8192, r = 16, 16-bit reads took 49 us).  It reads only the adapters that rows ask for, each once per row, and
 // nothing of one row's adapter can reach another row.
 //
 // The kernel starts while the projection still runs (programmatic launch): W, M, the indices and F,
@@ -139,7 +140,34 @@ __device__ __forceinline__ void load_factors(const Params &P, const int (&i)[kBa
 }
 
 // (Registers are held to what lets a CTA start beside two CTAs of the projection.)
-template <typename T, int kNT, bool kDrop>
+// F[i][c .. c+4)[j .. j+4) of kBatch rows' adapters (F's vectors run along the columns).
+__device__ __forceinline__ void load_columns(const Params &P, const int (&i)[kBatch], int64_t c,
+                                             int j, uint2 (&f)[kBatch][4]) {
+#pragma unroll
+    for (int u = 0; u < kBatch; ++u) {
+        const uint16_t *src = static_cast<const uint16_t *>(P.F.p) + max(i[u], 0) * P.F.ss + c;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            f[u][e] = make_uint2(0, 0);
+            if (i[u] < 0 || j + e >= P.r) continue;
+            const uint16_t *q = src + (j + e) * P.F.sr;
+            if (c + 4 <= P.cols) {
+                asm volatile("ld.global.nc.v2.u32 {%0, %1}, [%2];"
+                             : "=r"(f[u][e].x), "=r"(f[u][e].y)
+                             : "l"(q)
+                             : "memory");
+            } else {
+#pragma unroll
+                for (int d = 0; d < 3; ++d)
+                    if (c + d < P.cols)
+                        (d < 2 ? f[u][e].x : f[u][e].y) |= static_cast<uint32_t>(__ldg(q + d))
+                                                           << (16 * (d & 1));
+            }
+        }
+    }
+}
+
+template <typename T, int kNT, bool kDrop, bool kCol>
 __global__ void __launch_bounds__(kThreads, 2)
     lr_rows_kernel(const __grid_constant__ CUtensorMap tmM, const __grid_constant__ CUtensorMap tmW,
                    const __grid_constant__ Params P) {
@@ -287,17 +315,22 @@ __global__ void __launch_bounds__(kThreads, 2)
         bool waited = false;
         for (int k0 = group; rank + csize * k0 < here || !waited; k0 += 2 * kBatch) {
             int i[kBatch];
-            float acc[kBatch];
+            // kCol: a lane takes four columns and a quarter of the ranks
+            float acc[kBatch][kCol ? 4 : 1] = {};
 #pragma unroll
             for (int u = 0; u < kBatch; ++u) {
                 const int t = rank + csize * (k0 + 2 * u);
                 i[u] = t < here ? sidx[t] : -1;
-                acc[u] = 0.0f;
             }
 #pragma unroll 1
             for (int j0 = 0; j0 < P.r; j0 += 16) {
                 uint4 f[kBatch][2];
-                load_factors<T>(P, i, col, j0, f);
+                uint2 fc[kBatch][4];
+                const int jc = j0 + 4 * (lane >> 3);  // kCol: the lane's ranks
+                if constexpr (kCol)
+                    load_columns(P, i, col0 + q * 32 + 4 * (lane & 7), jc, fc);
+                else
+                    load_factors<T>(P, i, col, j0, f);
                 if (!waited) {
                     waited = true;
                     __syncwarp();
@@ -324,6 +357,23 @@ __global__ void __launch_bounds__(kThreads, 2)
                     const float *p =
                         staged ? proj + (k0 + 2 * u) * P.r + j0
                                : P.P + (row0 + rank + csize * (k0 + 2 * u)) * P.r + j0;
+                    if constexpr (kCol) {
+                        float w[4];
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            w[e] = jc + e < P.r ? p[4 * (lane >> 3) + e] : 0.0f;
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const float2 lo = unpack2<T>(fc[u][e].x), hi = unpack2<T>(fc[u][e].y);
+                            if (jc + e < P.r) {
+                                acc[u][0] += w[e] * lo.x;
+                                acc[u][1] += w[e] * lo.y;
+                                acc[u][2] += w[e] * hi.x;
+                                acc[u][3] += w[e] * hi.y;
+                            }
+                        }
+                        continue;
+                    }
                     float v[16];
                     unpack8<T>(f[u][0], *reinterpret_cast<float(*)[8]>(&v[0]));
                     unpack8<T>(f[u][1], *reinterpret_cast<float(*)[8]>(&v[8]));
@@ -332,15 +382,15 @@ __global__ void __launch_bounds__(kThreads, 2)
                         if (P.pvec) {  // r is a multiple of 4
                             if (j0 + e < P.r) {
                                 const float4 w = *reinterpret_cast<const float4 *>(p + e);
-                                acc[u] += w.x * v[e];
-                                acc[u] += w.y * v[e + 1];
-                                acc[u] += w.z * v[e + 2];
-                                acc[u] += w.w * v[e + 3];
+                                acc[u][0] += w.x * v[e];
+                                acc[u][0] += w.y * v[e + 1];
+                                acc[u][0] += w.z * v[e + 2];
+                                acc[u][0] += w.w * v[e + 3];
                             }
                         } else {
 #pragma unroll
                             for (int d = 0; d < 4; ++d)
-                                if (j0 + e + d < P.r) acc[u] += p[e + d] * v[e + d];
+                                if (j0 + e + d < P.r) acc[u][0] += p[e + d] * v[e + d];
                         }
                     }
                 }
@@ -349,12 +399,24 @@ __global__ void __launch_bounds__(kThreads, 2)
             for (int u = 0; u < kBatch; ++u) {
                 const int t = rank + csize * (k0 + 2 * u);
                 if (t >= here) break;
+                float sum = acc[u][0];
+                if constexpr (kCol) {
+                    // the ranks' quarters added, then each lane its own column
+#pragma unroll
+                    for (int d = 0; d < 4; ++d) {
+                        float x = acc[u][d];
+                        x += __shfl_xor_sync(0xFFFFFFFFu, x, 8);
+                        x += __shfl_xor_sync(0xFFFFFFFFu, x, 16);
+                        x = __shfl_sync(0xFFFFFFFFu, x, lane >> 2);
+                        if ((lane & 3) == d) sum = x;
+                    }
+                }
                 if (kDrop && i[u] >= 0) {
                     const uint4 bits = dropout_bits(P.drop, key, static_cast<uint32_t>(row0 + t),
                                                     static_cast<uint32_t>(col >> 3));
-                    if (!dropout_kept(bits, static_cast<int>(col & 7), P.drop.cut)) acc[u] = 0.0f;
+                    if (!dropout_kept(bits, static_cast<int>(col & 7), P.drop.cut)) sum = 0.0f;
                 }
-                low[(k0 + 2 * u) * kCols] = acc[u];
+                low[(k0 + 2 * u) * kCols] = sum;
             }
         }
         cluster_wait();
@@ -415,11 +477,11 @@ __global__ void __launch_bounds__(kThreads, 2)
     }
 }
 
-template <typename T, int kNT, bool kDrop>
+template <typename T, int kNT, bool kDrop, bool kCol>
 cudaError_t launch(const CUtensorMap &tmM, const CUtensorMap &tmW, const Params &P, int64_t tiles,
                    int ranks, cudaStream_t stream) {
     using S = Shape<kNT>;
-    auto kernel = lr_rows_kernel<T, kNT, kDrop>;
+    auto kernel = lr_rows_kernel<T, kNT, kDrop, kCol>;
     static PerDevice<int> ready;
     std::atomic<int> *set = ready.here();
     if (!set) return cudaErrorInvalidDevice;
@@ -479,8 +541,11 @@ cudaError_t expand(const ExpandOperands &o, int num_sms, int *err, cudaStream_t 
     if (P.w_nmajor ? !make_map16(&tmW, o.W.p, o.cols, o.inner, o.W.s0, 64, kBK)
                    : !make_map16(&tmW, o.W.p, o.inner, o.cols, o.W.s1, kBK, kCols))
         return cudaErrorInvalidValue;
-    return o.drop.cut ? launch<T, kNT, true>(tmM, tmW, P, tiles, ranks, stream)
-                      : launch<T, kNT, false>(tmM, tmW, P, tiles, ranks, stream);
+    if (factor_mode(o.F) == kFC)
+        return o.drop.cut ? launch<T, kNT, true, true>(tmM, tmW, P, tiles, ranks, stream)
+                          : launch<T, kNT, false, true>(tmM, tmW, P, tiles, ranks, stream);
+    return o.drop.cut ? launch<T, kNT, true, false>(tmM, tmW, P, tiles, ranks, stream)
+                      : launch<T, kNT, false, false>(tmM, tmW, P, tiles, ranks, stream);
 }
 
 template <typename T>
