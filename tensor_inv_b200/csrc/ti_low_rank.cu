@@ -135,7 +135,7 @@ Matrix16 readable(const Matrix16 &M, int64_t rows, int64_t cols, Arena &arena) {
 // cannot, packed in rows of one rank.
 Factor16 readable_factor(const Factor16 &F, int64_t s, int64_t cols, int64_t r, int64_t rows,
                          Arena &arena) {
-    if (rows <= kProjectRowsLimit || factor_mode(F) != kFScalar) return F;
+    if (rows <= project_rows_limit(s) || factor_mode(F) != kFScalar) return F;
     const int64_t ld = round8(cols), batch = F.ss == 0 ? 1 : s;
     return Factor16{arena.packed(Matrix16{F.p, F.sr, F.sc}, batch, F.ss, r, cols, ld),
                     F.ss == 0 ? 0 : r * ld, 1, ld};

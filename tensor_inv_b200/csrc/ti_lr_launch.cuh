@@ -37,8 +37,22 @@ inline bool copyable(const void *p, int64_t rows, int64_t ld, int64_t s_inner, i
            (rows <= 1 || (ld % 8 == 0 && ld >= inner));
 }
 
-// Up to this many rows, project runs a cluster per row, above it tiles of 128 rows.
-constexpr int64_t kProjectRowsLimit = 256;
+// Up to these many rows, project runs a cluster per row and expand streams W past the rows; above
+// them, project takes tiles of 128 rows and expand tiles of 256 on CTA pairs.
+// One adapter: 4096 x 4096, r = 16, expand on pairs against rows: 128 rows 32 against 21 us, 256 rows
+// 34 against 33 us.
+// Several: a tile multiplies with every adapter that any of its rows takes, which in a batch of short
+// requests is all of them, while the rows' cost does not depend on it.  Both kernels together, tiles
+// against rows, r = 16: 512 rows of 64 adapters in any order 205 against 78 us, in order (8 rows each)
+// 108 against 78 us; of 16 adapters 89 against 77 us and 55 against 76 us; r = 64, 64 adapters: 462
+// against 298 us and 231 against 254 us.  1024 rows of 64 adapters in order: 80 against 147 us.
+inline int64_t many_adapter_rows(int64_t adapters) {
+    return adapters < 32 ? 256 : adapters < 64 ? 8 * adapters : 512;
+}
+inline int64_t project_rows_limit(int64_t adapters) { return many_adapter_rows(adapters); }
+inline int64_t expand_rows_limit(int64_t adapters) {
+    return adapters > 1 ? many_adapter_rows(adapters) : 128;
+}
 
 // How a factor is read: element by element, in 16-byte vectors along c, or along the rank.
 enum { kFScalar = 0, kFC = 1, kFR = 2 };
@@ -62,7 +76,7 @@ struct ProjectOperands {
     Dropout drop;
     float *P;
 };
-// With more than kProjectRowsLimit rows the copy engine reads F: factor_mode(F) != kFScalar.
+// With more than project_rows_limit rows the copy engine reads F: factor_mode(F) != kFScalar.
 cudaError_t lr_project(bool half, const ProjectOperands &o, int num_sms, int *err,
                        cudaStream_t stream);
 
@@ -86,11 +100,6 @@ cudaError_t lr_expand_pairs(bool half, const ExpandOperands &o, int *err, cudaSt
 // o.P, whose other operands it reads before that has finished.
 cudaError_t lr_expand_rows(bool half, const ExpandOperands &o, int num_sms, int *err,
                            cudaStream_t stream);
-
-// Up to this many rows, expand streams W past the rows; above it, CTA pairs take 256-row tiles.
-// (4096 x 4096, r = 16, pairs against rows: 128 rows 32 against 21 us, 256 rows 34 against 33 us.  With
-// 64 adapters in any order the pairs take 91 and 106 us, the rows no longer than before.)
-inline int64_t expand_rows_limit(int64_t adapters) { return adapters > 1 ? 256 : 128; }
 
 // The gradients of the adapters (ti_lr_wgrad.cu).
 struct WgradPlan {

@@ -19,6 +19,10 @@
 // takes several microseconds; so all but the first copies wait until the first rows of F, the one
 // dependent chain of reads here, have been asked for.
 //
+// Measured on a B200, projection and launches included, replayed from a graph over weights larger
+// than L2: 4096 x 4096, r = 16: 1 row 13.4 us, 8 rows of 8 adapters 13.6 us, 24 rows 14.6 us;
+// 8192 x 8192, 8 rows: 32.5 us (4.1 TB/s of W); 4096 x 8192, 48 rows of 64 adapters: 25 us.
+//
 // Roles: warp 0 copies, warp 1 TMEM and MMA issue, warps 2..9 low-rank term and epilogue (two
 // groups of 128 threads, one thread per column, that share the rows).
 #include <atomic>

@@ -22,6 +22,12 @@
 //          that occur without gaps in either direction.
 //   join   adds an adapter's slots in order and rounds once.  One chunk needs no join.
 //
+// Measured on a B200: 4096 rows, 4096 + 4096 columns, r = 16: 22 us (3.0 TB/s of M), 38 us with
+// dropout, 35 us for fp16 (its scales take a pass over V); 8192 rows, r = 64: 56 us (144 us in a form
+// on mma.sync that kept M in registers).  Copies of four rows at a time cost more than boxes, so 64
+// consecutive rows go as one box: the first case's shape with rows of 16 adapters in random order,
+// which cannot, takes 55 us.
+//
 // (An infinity in M meets both parts of V, so its column comes out infinite or NaN.)
 #include <cstring>
 

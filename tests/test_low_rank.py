@@ -461,6 +461,24 @@ def test_factors_of_a_weight_difference():
     assert (B.grad[1] != 0).any() and (A.grad[1] == 0).all()  # B[1] is zero, so A[1] has no slope
     assert nat.device_error() == 0
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("T", [3, 40, 300])
+@pytest.mark.parametrize("N", [73, 74, 75, 76])
+def test_factor_cut_from_a_wider_buffer(T, N):
+    """Columns that end inside a vector, in rows that are aligned for one: what stands behind them
+    (NaN here) is not used, on either side."""
+    K, S, r = 75, 3, 8
+    X, W, A, B, index, scale, dY = operands(T, K, N, S, r, seed=7)
+    wide = torch.full((S, r, 80), float("nan"), dtype=B.dtype, device=B.device)
+    wide[:, :, :N] = B
+    tall = torch.full((S, r, 80), float("nan"), dtype=A.dtype, device=A.device)
+    tall[:, :, :K] = A.transpose(1, 2)
+    for a, b in ((A, wide[:, :, :N]), (tall[:, :, :K].transpose(1, 2), B),
+                 (tall[:, :, :K].transpose(1, 2), wide[:, :, :N])):
+        check_forward((X, W, a, b, index, scale, dY))
+        check_backward((X, W, a, b, index, scale, dY), p=0.5, seed=1)
+
+
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("T", [5, 300])
@@ -499,6 +517,19 @@ def test_gradients_of_empty_dimensions(T):
         grads = ti.low_rank_matmul_backward(dY[:, :N], X[:, :K], W[:K, :N], a, b, index, scale)
         for G, shape in zip(grads, ((T, K), a.shape, b.shape)):
             assert G.shape == shape and (G == 0).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("outer", [False, True])
+@pytest.mark.parametrize("size", [
+    (256, 200, 136, 32, 16), (257, 200, 136, 32, 16), (320, 328, 257, 40, 13), (321, 328, 257, 40, 13),
+    (512, 256, 392, 64, 24), (513, 256, 392, 64, 24), (512, 72, 64, 500, 8)])
+def test_borders_between_forms(size, outer):
+    """With many adapters the form for few rows reaches further: both sides of its borders."""
+    for rows in ("mixed", "runs"):
+        ops = operands(*size, outer=outer, rows=rows, seed=4, pad=3)
+        check_forward(ops)
+        check_backward(ops, p=0.5, seed=8)
 
 
 @pytest.mark.gpu
