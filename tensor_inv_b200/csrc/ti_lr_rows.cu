@@ -9,8 +9,9 @@
 //
 // The low-rank term is a few multiply-adds per output and runs on the plain cores while the copies
 // of W are in flight: thread c of the serving CTA holds column c, and the row's P meets its
-// adapter's F in float32 (where F's vectors run along the columns, a lane reads four columns of a
-// quarter of the ranks: 48 x 4096 x 8192, r = 16, 16-bit reads took 49 us).  It reads only the adapters that rows ask for, each once per row, and
+// adapter's F in float32.  (Where F's vectors run along the columns, a lane reads four columns of a
+// quarter of the ranks: 48 x 4096 x 8192, r = 16, 29 us where 16-bit reads took 49 us, projection not
+// counted.)  It reads only the adapters that rows ask for, each once per row, and
 // nothing of one row's adapter can reach another row.
 //
 // The kernel starts while the projection still runs (programmatic launch): W, M, the indices and F,
@@ -143,7 +144,6 @@ __device__ __forceinline__ void load_factors(const Params &P, const int (&i)[kBa
     }
 }
 
-// (Registers are held to what lets a CTA start beside two CTAs of the projection.)
 // F[i][c .. c+4)[j .. j+4) of kBatch rows' adapters (F's vectors run along the columns).
 __device__ __forceinline__ void load_columns(const Params &P, const int (&i)[kBatch], int64_t c,
                                              int j, uint2 (&f)[kBatch][4]) {
@@ -171,6 +171,7 @@ __device__ __forceinline__ void load_columns(const Params &P, const int (&i)[kBa
     }
 }
 
+// (Registers are held to what lets a CTA start beside two CTAs of the projection.)
 template <typename T, int kNT, bool kDrop, bool kCol>
 __global__ void __launch_bounds__(kThreads, 2)
     lr_rows_kernel(const __grid_constant__ CUtensorMap tmM, const __grid_constant__ CUtensorMap tmW,
