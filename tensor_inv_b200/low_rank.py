@@ -196,7 +196,9 @@ def low_rank_matmul(X, W, A, B, index=None, scale=None, *, alpha=1.0, p=0.0, see
     type, any strides (a weight stored outputs x inputs is passed as its transposed view); one
     adapter may be given as ``A`` (K, r), ``B`` (r, N).  Rank r from 1 to 256.  ``index`` (T,)
     int32 or int64: the adapter of each row, in any order; a value outside [0, S), such as -1,
-    gives the row no low-rank term.  It may be left out when S is 1.  ``scale`` (S,) float32 and
+    gives the row no low-rank term.  It may be left out when S is 1.  (With several hundred rows
+    or more, rows of one adapter next to each other are faster: a tile of rows multiplies with
+    every adapter that any of them takes.)  ``scale`` (S,) float32 and
     the number ``alpha`` multiply the term.  ``p``, ``seed``, ``offset``: dropout on X in the
     low-rank term only, with ``dropout``'s mask.
 
