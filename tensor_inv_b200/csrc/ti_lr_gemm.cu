@@ -59,6 +59,11 @@ constexpr int kGroupM = 8;                       // raster: 8 row tiles (2048 ro
 constexpr int kRankStep = 16;
 constexpr int kFixSlots = 16;
 constexpr size_t kSmem = size_t(kStages) * kStageBytes + 2 * kLowBytes + 1024 + 512;
+// Rows that leave through shared memory: a warp's 32 rows of 16 words, one word apart.  Such calls
+// use a ring of kStages - 1 stages, and four warps each share the last stage of sA and of sB.
+constexpr int kTurnWords = 32 * 17;
+static_assert(4 * kTurnWords * 4 <= kABytes && kABytes == kBBytes,
+              "the warps' rows do not fit the stage that is left to them");
 
 struct Params {
     int64_t rows, cols;
@@ -431,8 +436,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         int64_t unit = 0;
         const DropoutKeys key(kDrop ? dropout_key(P.drop) : 0);
         T *out = static_cast<T *>(P.out);
-        // (the last stage of the ring, which such calls do without)
-        uint32_t *turn = reinterpret_cast<uint32_t *>(sA + (kStages - 1) * kABytes) + (warp - 2) * 32 * 17;
+        uint32_t *turn = reinterpret_cast<uint32_t *>((part ? sB : sA) + (kStages - 1) * kABytes) +
+                         q * kTurnWords;
         // the whole warp has read its accumulator rows: one arrive per warp on CTA 0
         auto release = [&](int acc) {
             tc_fence_before();

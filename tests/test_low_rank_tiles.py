@@ -1,0 +1,48 @@
+"""Low-rank products of more tiles, passes and segments than one CTA holds at a time.
+
+Whole numbers throughout: every sum is exact in float32, so a result is the exact value rounded
+once, and calls repeat bit for bit.
+"""
+
+import pytest
+import torch
+
+import low_rank_reference as ref
+import tensor_inv_b200 as ti
+from test_low_rank import TYPES, no_device_error, operands  # noqa: F401 (a fixture)
+
+
+def repeats(call, exact, times=4):
+    for _ in range(times):
+        got = call()
+        assert torch.equal(got.cpu(), exact.to(got.dtype))
+
+
+# Rows of the result that are aligned to 2, 4, 8 and 16 bytes, in 150 tiles of 256 x 256 or more:
+# each of the 74 CTA pairs of a B200 takes several, so that the copies of a tile's operands run
+# while the tile before it is stored.
+COLUMNS = [4001, 4002, 4004, 4008]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("outer", [False, True])
+@pytest.mark.parametrize("N", COLUMNS)
+@pytest.mark.parametrize("T, K", [(4096, 136), (2500, 520)])
+def test_forward_of_many_tiles(T, K, N, outer):
+    X, W, A, B, index, scale, _ = operands(T, K, N, 3, 16, dtype=TYPES[N % 8 // 4], outer=outer,
+                                           seed=N)
+    exact, _ = ref.forward(X, W, A, B, index, scale)
+    repeats(lambda: ti.low_rank_matmul(X, W, A, B, index, scale), exact)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("outer", [False, True])
+@pytest.mark.parametrize("K", COLUMNS)
+@pytest.mark.parametrize("p", [0.0, 0.5])
+def test_gradient_of_many_tiles(p, K, outer):
+    X, W, A, B, index, scale, dY = operands(4096, K, 136, 3, 16, dtype=TYPES[K % 8 // 4],
+                                            outer=outer, seed=K)
+    rest = dict(p=p, seed=5)
+    exact = ref.backward(dY, X, W, A, B, index, scale, **rest)[0]
+    repeats(lambda: ti.low_rank_matmul_backward(dY, X, W, A, B, index, scale,
+                                                needs=(True, False, False), **rest)[0], exact)
