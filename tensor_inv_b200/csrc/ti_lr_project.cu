@@ -305,7 +305,9 @@ __global__ void __launch_bounds__(kTileThreads, 1)
                     }
                 }
             }
-            ok = ok && mbar_wait(tfull, pass & 1, abort);
+            // Only the warps that arrive on tempty may wait here: nothing would hold the next pass
+            // back for another, and a phase that it missed would leave it two passes behind.
+            ok = ok && (warp >= 6 || mbar_wait(tfull, pass & 1, abort));
             if (!ok) raise(P, abort, kErrTimeoutEpilogue);
             ok = __all_sync(0xFFFFFFFFu, ok);
             if (!started) {

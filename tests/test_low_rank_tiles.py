@@ -46,3 +46,25 @@ def test_gradient_of_many_tiles(p, K, outer):
     exact = ref.backward(dY, X, W, A, B, index, scale, **rest)[0]
     repeats(lambda: ti.low_rank_matmul_backward(dY, X, W, A, B, index, scale,
                                                 needs=(True, False, False), **rest)[0], exact)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("p", [0.0, 0.5])
+@pytest.mark.parametrize("T, K, S, r", [
+    (1024, 40, 300, 64), (1024, 64, 700, 8),  # a step per pass: 32 passes of 4 adapters, 8 of 16
+    (700, 1088, 200, 64), (520, 1088, 300, 16),  # 17 steps for clusters of 8: two CTAs have none
+])
+def test_projection_of_many_short_passes(T, K, S, r, p):
+    """Tiles whose rows take more adapters than a pass holds: P of the forward pass and, with the
+    inner dimension N, of the backward pass (seen through dX)."""
+    X, W, A, B, index, scale, dY = operands(T, K, K, S, r, seed=T + r)
+    rest = dict(p=p, seed=2)
+    exact, exact_p = ref.forward(X, W, A, B, index, scale, **rest)
+    dx = ref.backward(dY, X, W, A, B, index, scale, **rest)[0]
+    for _ in range(5):
+        Y, P = ti.low_rank_matmul(X, W, A, B, index, scale, return_projection=True, **rest)
+        assert torch.equal(P.cpu(), exact_p.float())
+        assert torch.equal(Y.cpu(), exact.to(Y.dtype))
+        dX = ti.low_rank_matmul_backward(dY, X, W, A, B, index, scale,
+                                         needs=(True, False, False), **rest)[0]
+        assert torch.equal(dX.cpu(), dx.to(dX.dtype))
