@@ -28,7 +28,11 @@
 // consecutive rows go as one box: the first case's shape with rows of 16 adapters in random order,
 // which cannot, takes 55 us.
 //
-// (An infinity in M meets both parts of V, so its column comes out infinite or NaN.)
+// Infinities and NaN: an infinity in M meets both parts of V, and infinity * 0 or infinity - infinity
+// is NaN where the formula has an infinity (and a V near float32's end rounds to one).  So a CTA that
+// meets a sum that is not finite forms those sums again at its end, by multiply-adds of M and V as
+// they are.  A sum that is finite met no infinity in either part.  (8192 rows, 8192 + 8192 columns,
+// r = 64, bf16: 192 us; 474 us where all of M is NaN; up to some ms with infinities.)
 #include <cstring>
 
 #include "ti_lr_loads.cuh"
@@ -166,6 +170,68 @@ __device__ __forceinline__ uint16_t bits16(float v) {
     return *reinterpret_cast<const uint16_t *>(&h);
 }
 
+// Forms the sums of the CTA's segments that are not finite again, as sums of M's and V's own products
+// in the order of the rows.  For results that hold infinities or NaN only: each thread takes a column
+// and 16 ranks at a time, and reads M once for them.
+template <typename T>
+__device__ __noinline__ void add_nonfinite(const WgradParams &P, const Side &S, int64_t chunk,
+                                           int64_t s0, int64_t first, int64_t stop, int64_t c0,
+                                           int j0) {
+    const int64_t ldc = (S.cols + 7) / 8 * 8;
+    const bool direct = S.part == nullptr;
+    const int ranks = static_cast<int>(min(int64_t(kBlockRanks), P.r - j0));
+    const DropoutKeys key(S.drop.cut ? dropout_key(S.drop) : 0);
+    auto finite = [](float x) { return fabsf(x) < __int_as_float(0x7F800000); };
+    segments(P, s0, first, stop, direct, [&](int64_t s, int64_t from, int64_t to) {
+        for (int64_t c = c0 + threadIdx.x; c < min(c0 + kCtaCols, S.cols); c += kThreads) {
+            T *out = static_cast<T *>(S.out) + s * S.ss + c * S.sc + j0 * S.sr;
+            float *part = S.part + ((chunk + s) * P.r + j0) * ldc + c;
+            for (int jb = 0; jb < ranks; jb += 16) {
+                const int n = min(16, ranks - jb);
+                uint32_t wrong = 0;
+                for (int e = 0; e < n; ++e)
+                    if (!finite(direct ? to_float(out[(jb + e) * S.sr]) : part[(jb + e) * ldc]))
+                        wrong |= 1u << e;
+                if (!wrong) continue;
+                float sum[16];
+#pragma unroll
+                for (int e = 0; e < 16; ++e) sum[e] = 0.0f;
+                uint32_t open = wrong;  // a sum that is NaN stays so
+                for (int64_t b = from; b < to && open; b += 32) {
+                    const int64_t end = min(to, b + 32);
+#pragma unroll 4
+                    for (int64_t p = b; p < end; ++p) {
+                        const int64_t row = row_at(P, p, to);
+                        if (row >= P.rows) continue;
+                        float m = to_float(static_cast<const T *>(S.M)[row * S.ld + c]);
+                        if (S.drop.cut &&
+                            !dropout_kept(dropout_bits(S.drop, key, static_cast<uint32_t>(row),
+                                                       static_cast<uint32_t>(c >> 3)),
+                                          static_cast<int>(c & 7), S.drop.cut))
+                            m = 0.0f;
+                        const float *v = S.V + row * P.r + j0 + jb;
+#pragma unroll
+                        for (int e = 0; e < 16; ++e)
+                            if (e < n) sum[e] += m * v[e];
+                    }
+#pragma unroll
+                    for (int e = 0; e < 16; ++e)
+                        if (sum[e] != sum[e]) open &= ~(1u << e);
+                }
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    if (!((wrong >> e) & 1)) continue;
+                    if (direct)
+                        out[(jb + e) * S.sr] = from_float<T>(sum[e]);
+                    else
+                        part[(jb + e) * ldc] = sum[e];
+                }
+            }
+        }
+        return true;
+    });
+}
+
 // order[] and start[]: rows grouped by adapter, ascending within one.  CTA s compacts the rows of
 // adapter s behind those of smaller adapters, which it counts first; up to 8192 indices stay in
 // registers between the two passes.
@@ -239,6 +305,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(drain + 1);
     volatile int *abort = reinterpret_cast<volatile int *>(tmem_slot + 1);
     int *start_at = const_cast<int *>(abort) + 1;
+    volatile int *fix = start_at + 1;  // some sum is not finite
 
     const int64_t units_a = P.side[0].blocks * P.side[0].chunks;
     const int which = blockIdx.x < units_a ? 0 : 1;
@@ -263,6 +330,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         mbar_init(tempty, kWorkers / 32);
         mbar_init(drain, 1);
         *abort = 0;
+        *fix = 0;
         fence_barrier_init();
     }
     if (warp == 1) {
@@ -533,6 +601,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                         const int64_t j = j0 + jb + e;
                         if (j >= P.r) continue;
                         float y = some ? __uint_as_float(x[e]) : 0.0f;
+                        if (!(fabsf(y) < __int_as_float(0x7F800000))) *fix = 1;
                         // (a power of two, and its inverse by exponent arithmetic)
                         if (kScaled && some)
                             y *= __int_as_float((254 << 23) - __float_as_int(scale[jb + e]));
@@ -557,6 +626,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         tc_fence_after();
         tmem_dealloc(tmem_base, kTmemCols);
     }
+    if (*fix && !*abort) add_nonfinite<T>(P, S, chunk, s0, first, stop, c0, j0);
 }
 
 // out[s][c][j] = the sum of adapter s's slots, in order.  A block takes 32 ranks x 32 columns, reads

@@ -231,7 +231,7 @@ def low_rank_matmul_backward(dY, X, W, A, B, index=None, scale=None, *, P=None, 
     projection it returned (made again when left out).  ``needs`` says which of the three are
     computed; the others are None.  dX is (T, K); dA and dB have the shapes and the layout of A and
     B and are zero for an adapter that no row takes.  Sums over rows are held in float32 in a
-    fixed order.
+    fixed order; infinities and NaN appear where the formula has them.
     """
     if len(needs) != 3:
         raise ValueError("needs has three entries: dX, dA, dB")
