@@ -13,11 +13,11 @@
 //          which reads as zeros, so that no row of another adapter enters).  M stays as it lies in
 //          memory: its columns are the 128-row side of the MMA, read in the orientation whose
 //          consecutive elements run along the columns.  Eight warps turn V into the other operand:
-//          16-bit values in two parts, the rounded value and what is left of it.  That keeps 22 bits
-//          of V for fp16 and 16 for bf16 (2^-17, where dA and dB are rounded to 2^-9).  For fp16,
-//          whose exponents V may leave, each rank's column is first scaled by a power of two that
-//          brings its largest value of the CTA's rows to 2^14; the sums are scaled back.  With
-//          dropout the same warps mask the staged tile.  Where a chunk crosses from one adapter to
+//          16-bit values in parts, the rounded value and what is left of it.  Three parts of bf16 hold
+//          all 24 bits of V, two of fp16 hold 22 (a sum whose terms cancel keeps what float32 values
+//          give it).  For fp16, whose exponents V may leave, each rank's column is first scaled by a
+//          power of two that brings its largest value of the CTA's rows to 2^14; the sums are scaled
+//          back.  With dropout the same warps mask the staged tile.  Where a chunk crosses from one adapter to
 //          the next the sums go to another slot: chunk + adapter numbers the (chunk, adapter) pairs
 //          that occur without gaps in either direction.
 //   join   adds an adapter's slots in order and rounds once.  One chunk needs no join.
@@ -28,11 +28,11 @@
 // consecutive rows go as one box: the first case's shape with rows of 16 adapters in random order,
 // which cannot, takes 55 us.
 //
-// Infinities and NaN: an infinity in M meets both parts of V, and infinity * 0 or infinity - infinity
+// Infinities and NaN: an infinity in M meets every part of V, and infinity * 0 or infinity - infinity
 // is NaN where the formula has an infinity (and a V near float32's end rounds to one).  So a CTA that
 // meets a sum that is not finite forms those sums again at its end, by multiply-adds of M and V as
-// they are.  A sum that is finite met no infinity in either part.  (8192 rows, 8192 + 8192 columns,
-// r = 64, bf16: 192 us; 474 us where all of M is NaN; up to some ms with infinities.)
+// they are.  A sum that is finite met no infinity in any part.  (8192 rows, 8192 + 8192 columns,
+// r = 64, bf16: 218 us; 554 us where all of M is NaN; up to some ms with infinities.)
 #include <cstring>
 
 #include "ti_lr_loads.cuh"
@@ -46,10 +46,16 @@ constexpr int kAtomBytes = kRows * 128;       // 64 columns of a stage
 constexpr int kMBytes = 4 * kAtomBytes;
 constexpr int kBlockRanks = 64;               // ranks of a CTA
 constexpr int kPartBytes = kBlockRanks * 128; // one part of V's stage
-constexpr int kStageBytes = kMBytes + 2 * kPartBytes, kStages = 4;
+constexpr int kStages = 4;
 constexpr int kWorkers = 256, kThreads = 64 + kWorkers;
 constexpr uint32_t kTmemCols = 128;           // two halves of the columns, 64 ranks each
-constexpr size_t kSmem = size_t(kStages) * kStageBytes + 1024 + 1024;
+
+template <typename T>
+struct Stage {
+    static constexpr int kParts = std::is_same<T, __half>::value ? 2 : 3;  // of V
+    static constexpr int kBytes = kMBytes + kParts * kPartBytes;
+    static constexpr size_t kSmem = size_t(kStages) * kBytes + 1024 + 1024;
+};
 
 struct Side {
     const void *M;
@@ -292,6 +298,7 @@ template <typename T>
 __global__ void __launch_bounds__(kThreads, 1)
     wgrad_kernel(const __grid_constant__ Maps maps, const __grid_constant__ WgradParams P) {
     constexpr bool kScaled = std::is_same<T, __half>::value;
+    constexpr int kParts = Stage<T>::kParts, kStageBytes = Stage<T>::kBytes;
     extern __shared__ uint8_t smem_raw[];
     uint8_t *ring = reinterpret_cast<uint8_t *>(
         (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -428,7 +435,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                         const uint64_t mdesc =
                             make_sw128_mnmajor_desc(sm + 2 * h * kAtomBytes, kAtomBytes);
 #pragma unroll
-                        for (int part = 0; part < 2; ++part) {
+                        for (int part = 0; part < kParts; ++part) {
                             const uint64_t vdesc =
                                 make_sw128_kmajor_desc(sm + kMBytes + part * kPartBytes);
 #pragma unroll
@@ -538,15 +545,16 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
                         const int j = 4 * quad + e;
-                        const float y = kScaled ? x[e] * scale[j] : x[e];
-                        const uint16_t hi = bits16<T>(y);
-                        const float up = to_float(*reinterpret_cast<const T *>(&hi));
-                        // infinities and NaN stay whole in the first part
-                        const float rest = fabsf(up) < __int_as_float(0x7F800000) ? y - up : 0.0f;
+                        float y = kScaled ? x[e] * scale[j] : x[e];
                         const uint32_t at = j * 128 + ((((t >> 3) ^ (j & 7)) << 4) | ((t & 7) << 1));
-                        *reinterpret_cast<uint16_t *>(m + kMBytes + at) = hi;
-                        *reinterpret_cast<uint16_t *>(m + kMBytes + kPartBytes + at) =
-                            bits16<T>(rest);
+#pragma unroll
+                        for (int part = 0; part < kParts; ++part) {
+                            const uint16_t h = bits16<T>(y);
+                            const float up = to_float(*reinterpret_cast<const T *>(&h));
+                            // infinities and NaN stay whole in the first part
+                            y = fabsf(up) < __int_as_float(0x7F800000) ? y - up : 0.0f;
+                            *reinterpret_cast<uint16_t *>(m + kMBytes + part * kPartBytes + at) = h;
+                        }
                     }
                 }
 #pragma unroll
@@ -726,13 +734,14 @@ static cudaError_t wgrad(WgradParams &P, int num_sms, cudaStream_t stream) {
     if (!set) return cudaErrorInvalidDevice;
     if (!set->load(std::memory_order_acquire)) {
         const cudaError_t e = cudaFuncSetAttribute(
-            wgrad_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kSmem));
+            wgrad_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+            static_cast<int>(Stage<T>::kSmem));
         if (e != cudaSuccess) return e;
         set->store(1, std::memory_order_release);
     }
     const dim3 grid(static_cast<unsigned>(units),
                     static_cast<unsigned>((P.r + kBlockRanks - 1) / kBlockRanks));
-    wgrad_kernel<T><<<grid, kThreads, kSmem, stream>>>(maps, P);
+    wgrad_kernel<T><<<grid, kThreads, Stage<T>::kSmem, stream>>>(maps, P);
     if (P.side[0].part || P.side[1].part) {
         const int64_t cols = P.side[0].cols > P.side[1].cols ? P.side[0].cols : P.side[1].cols;
         const int64_t want = P.s * ((P.r + 31) / 32) * ((cols + 31) / 32), most = int64_t(num_sms) * 8;

@@ -68,3 +68,31 @@ def test_projection_of_many_short_passes(T, K, S, r, p):
         dX = ti.low_rank_matmul_backward(dY, X, W, A, B, index, scale,
                                          needs=(True, False, False), **rest)[0]
         assert torch.equal(dX.cpu(), dx.to(dX.dtype))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("T", [64, 1000])
+def test_gradients_of_values_that_cancel(T, dtype):
+    """P and dP of 22 bits (fp16: 21) whose column sums cancel to their last one: whole numbers below
+    2^24 in every partial sum, so the small sum is exact."""
+    K, N, r, top = 80, 96, 8, 2.0**21 if dtype is torch.bfloat16 else 2.0**20
+    X, W, A, B, _, _, dY = operands(T, K, N, 1, r, dtype=dtype, seed=T)
+    big = top + 2.0**10 + 1
+    for M in (X, dY):
+        M.zero_()
+    X[3], X[T - 2] = 1, -1
+    dY[3], dY[T - 2] = 1, -1
+    P = torch.zeros(T, r, device="cuda")
+    P[3], P[T - 2] = big, big - 1
+    dB = ti.low_rank_matmul_backward(dY, X, W, A, B, P=P)[2]
+    assert (dB == 1).all()
+    # dP of the same values: dY B with the three parts of the number in three columns of dY
+    B.zero_()
+    B[0, :, :3] = 1
+    dY.zero_()
+    dY[3, 0], dY[3, 1], dY[3, 2] = 2.0**11, 2.0**10, 1
+    dY[T - 2, 0], dY[T - 2, 1] = 2.0**11, 2.0**10
+    B[0, :, 0] = top / 2.0**11
+    dA = ti.low_rank_matmul_backward(dY, X, W, A, B, P=P)[1]
+    assert (dA == 1).all()
