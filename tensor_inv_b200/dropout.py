@@ -12,6 +12,7 @@ import ctypes
 import numbers
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _native as nat
 
@@ -54,6 +55,16 @@ def refuse_capture(what):
     if torch.cuda.is_current_stream_capturing():
         raise RuntimeError(f"{what} does not record gradients inside a CUDA graph capture; "
                            f"call it under torch.no_grad() and call {what}_backward")
+
+
+def refuse_tangents(what, *operands):
+    """The kernels read a dual tensor's value only, so its tangent would be lost without a word."""
+    if forward_ad._current_level < 0:  # no dual_level is open
+        return
+    for M in operands:
+        if isinstance(M, torch.Tensor) and M.is_floating_point() and \
+                forward_ad.unpack_dual(M).tangent is not None:
+            raise RuntimeError(f"{what} has no forward-mode derivative: an operand has a tangent")
 
 
 def _dropout(X, p, seed, offset):
@@ -113,9 +124,10 @@ def dropout(X, p, seed=None, offset=0):
     read when the kernel runs (a captured graph then draws another mask at each replay whose seed
     was changed).  ``offset``: an integer in [0, 2^64) that tells apart the calls of one seed.
 
-    Differentiable: the gradient is ``dropout_backward``.  Returns a new contiguous tensor.
+    Differentiable in reverse mode: the gradient is ``dropout_backward``.  Returns a new contiguous tensor.
     """
     _check_input(X, "dropout")
+    refuse_tangents("dropout", X)
     if torch.is_grad_enabled() and X.requires_grad:
         if X.is_cuda:
             refuse_capture("dropout")
@@ -126,5 +138,6 @@ def dropout(X, p, seed=None, offset=0):
 def dropout_backward(dY, p, seed=None, offset=0):
     """The gradient of ``dropout`` with respect to its input: the same map applied to ``dY``."""
     _check_input(dY, "dropout_backward")
+    refuse_tangents("dropout_backward", dY)
     with torch.no_grad():
         return _dropout(dY, p, seed, offset)

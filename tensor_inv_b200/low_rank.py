@@ -19,7 +19,7 @@ import numbers
 import torch
 
 from . import _native as nat
-from .dropout import drop_numbers, refuse_capture
+from .dropout import drop_numbers, refuse_capture, refuse_tangents
 
 _TYPE_CODES = {torch.float16: nat.TI_TYPE_F16, torch.bfloat16: nat.TI_TYPE_BF16}
 MAX_RANK = 256
@@ -205,10 +205,11 @@ def low_rank_matmul(X, W, A, B, index=None, scale=None, *, alpha=1.0, p=0.0, see
     Sums are held in float32, Y is rounded once.  A row is touched by its own adapter only: NaN
     or infinities in another adapter do not reach it.  The result does not change from run to run.
 
-    Differentiable in X, A and B (W is fixed and may not require a gradient, nor may ``scale``).
+    Differentiable in reverse mode in X, A and B (W is fixed and may not require a gradient, nor may ``scale``).
     ``return_projection=True`` returns ``(Y, P)``: P (T, r) float32 is what ``low_rank_matmul_backward``
     reads; ``torch.no_grad()`` code, such as a captured training step, passes it there itself.
     """
+    refuse_tangents("low_rank_matmul", X, W, A, B, scale)
     A, B, _ = _batched(A, B)
     if torch.is_grad_enabled() and any(getattr(M, "requires_grad", False)
                                        for M in (X, A, B, W, scale)):
@@ -235,6 +236,7 @@ def low_rank_matmul_backward(dY, X, W, A, B, index=None, scale=None, *, P=None, 
     """
     if len(needs) != 3:
         raise ValueError("needs has three entries: dX, dA, dB")
+    refuse_tangents("low_rank_matmul_backward", dY, X, W, A, B, scale, P)
     A, B, single = _batched(A, B)
     with torch.no_grad():
         dX, dA, dB = _backward(dY, X, W, A, B, index, scale, alpha, p, seed, offset, P,
