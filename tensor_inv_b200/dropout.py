@@ -74,6 +74,7 @@ def _dropout(X, p, seed, offset):
     out = X.new_empty(X.shape)
     if X.numel() == 0:
         return out
+    X = X.resolve_neg()  # a negative view holds its values unnegated
     flat = X if X.dim() == 2 else X.reshape(-1, X.shape[-1])  # a view where the strides allow it
     rows, cols = flat.shape
     if rows >= 2**32 or cols >= 2**34:

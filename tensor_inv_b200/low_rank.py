@@ -66,6 +66,9 @@ def _describe(X, W, A, B, index, scale, alpha, p, seed, offset):
     if not fits:
         _refuse(X, W, A, B)
         raise ValueError("low_rank_matmul: operands do not fit together")
+    # a negative view (such as the imaginary part of a conjugate) holds its values unnegated
+    if X.is_neg() or W.is_neg() or A.is_neg() or B.is_neg():
+        X, W, A, B = X.resolve_neg(), W.resolve_neg(), A.resolve_neg(), B.resolve_neg()
     if index is None:
         if S != 1:
             raise ValueError(f"{S} adapters need an index that says which one each row takes")
@@ -86,7 +89,7 @@ def _describe(X, W, A, B, index, scale, alpha, p, seed, offset):
         if scale.dim() != 1 or len(scale) != S or scale.get_device() != at:
             raise ValueError(f"scale must have shape ({S},) on {X.device}, got "
                              f"{tuple(scale.shape)} on {scale.device}")
-        scale = scale.contiguous()
+        scale = (scale.resolve_neg() if scale.is_neg() else scale).contiguous()
         scale_ptr = scale.data_ptr()
     if type(alpha) is not float and not isinstance(alpha, numbers.Real):
         raise TypeError("alpha must be a number")
@@ -128,6 +131,7 @@ def _backward(dY, X, W, A, B, index, scale, alpha, p, seed, offset, P, needs):
     if dY.shape != (op.t, op.n) or dY.device != dev:
         raise ValueError(f"dY must have shape {(op.t, op.n)} on {dev}, got "
                          f"{tuple(dY.shape)} on {dY.device}")
+    dY = dY.resolve_neg()
     want_x, want_a, want_b = needs
     if P is None and want_b:
         P = _forward(X, W[:, :0], A, B[:, :, :0], index, scale, alpha, p, seed, offset, True)[1]
@@ -137,7 +141,7 @@ def _backward(dY, X, W, A, B, index, scale, alpha, p, seed, offset, P, needs):
         if P.shape != (op.t, op.r) or P.device != dev:
             raise ValueError(f"P must have shape {(op.t, op.r)} on {dev}, got {tuple(P.shape)} "
                              f"on {P.device}")
-        P = P.contiguous()
+        P = P.resolve_neg().contiguous()
     dX = torch.empty((op.t, op.k), dtype=X.dtype, device=dev) if want_x else None
     # the gradients take the layout of A and B (their strides, where those are dense)
     dA = torch.empty_like(A) if want_a else None

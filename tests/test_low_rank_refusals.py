@@ -26,3 +26,21 @@ def test_tangents(at):
                 fn(ops[at], 0.5, 1)
         with pytest.raises(ValueError, match="CUDA"):  # an open level alone refuses nothing
             ti.low_rank_matmul(*plain[:6])
+
+
+@pytest.mark.gpu
+def test_negative_views():
+    """Tensors that hold their values unnegated (torch marks them so) count as what they stand for."""
+    ops = operands(40, 64, 72, 2, 8)
+    X, W, A, B, index, scale, dY = ops
+    P = torch.arange(40.0 * 8, device="cuda").view(40, 8)
+    want = (ti.low_rank_matmul(X, W, A, B, index, scale),
+            *ti.low_rank_matmul_backward(dY, X, W, A, B, index, scale, P=P), ti.dropout(X, 0.5, 1))
+    X, W, A, B, scale, dY, P = (torch._neg_view(-M) for M in (X, W, A, B, scale, dY, P))
+    assert X.is_neg() and torch.equal(X, ops[0])
+    got = (ti.low_rank_matmul(X, W, A, B, index, scale),
+           *ti.low_rank_matmul_backward(dY, X, W, A, B, index, scale, P=P), ti.dropout(X, 0.5, 1))
+    for G, E in zip(got, want):
+        assert torch.equal(G, E)
+    Z = torch.randn(6, 10, dtype=torch.complex64, device="cuda")
+    assert torch.equal(ti.dropout(Z.conj().imag, 0.5, 1), -ti.dropout(Z.imag, 0.5, 1))
