@@ -58,7 +58,8 @@ inline int64_t expand_rows_limit(int64_t adapters) {
 enum { kFScalar = 0, kFC = 1, kFR = 2 };
 
 inline int factor_mode(const Factor16 &F) {
-    const bool base = (reinterpret_cast<uintptr_t>(F.p) & 15) == 0 && F.ss % 8 == 0;
+    // (a copy engine's strides are not negative)
+    const bool base = (reinterpret_cast<uintptr_t>(F.p) & 15) == 0 && F.ss % 8 == 0 && F.ss >= 0;
     if (base && F.sc == 1 && F.sr % 8 == 0 && F.sr > 0) return kFC;
     if (base && F.sr == 1 && F.sc % 8 == 0 && F.sc > 0) return kFR;
     return kFScalar;
