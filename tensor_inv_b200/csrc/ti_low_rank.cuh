@@ -47,10 +47,6 @@ template <>
 __device__ __forceinline__ float to_float<__nv_bfloat16>(__nv_bfloat16 v) {
     return __bfloat162float(v);
 }
-template <>
-__device__ __forceinline__ float to_float<float>(float v) {
-    return v;
-}
 
 template <typename T>
 __device__ __forceinline__ T from_float(float v);
@@ -61,10 +57,6 @@ __device__ __forceinline__ __half from_float<__half>(float v) {
 template <>
 __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float v) {
     return __float2bfloat16_rn(v);
-}
-template <>
-__device__ __forceinline__ float from_float<float>(float v) {
-    return v;
 }
 
 }  // namespace ti
