@@ -96,3 +96,20 @@ def test_gradients_of_values_that_cancel(T, dtype):
     B[0, :, 0] = top / 2.0**11
     dA = ti.low_rank_matmul_backward(dY, X, W, A, B, P=P)[1]
     assert (dA == 1).all()
+
+
+@pytest.mark.gpu
+def test_results_past_32_bits():
+    """Y and dX of more than 2^31 elements (4.3 GB), in rows that are not 16-byte aligned: the first
+    rows, those around element 2^31 and the last against float64."""
+    T, wide, r = 33000, 66001, 8
+    X, W, A, B, index, scale, dY = operands(T, 40, wide, 2, r, seed=1)
+    near = 2**31 // wide
+    rows = torch.cat([torch.arange(at, at + 5) for at in (0, near - 2, T - 5)]).cuda()
+    Y = ti.low_rank_matmul(X, W, A, B, index, scale)
+    exact, _ = ref.forward(X[rows], W, A, B, index[rows], scale)
+    assert torch.equal(Y[rows].cpu(), exact.to(Y.dtype))
+    del Y
+    back = W.t(), B.transpose(1, 2), A.transpose(1, 2)  # the same product as a gradient
+    dX = ti.low_rank_matmul_backward(X, dY, *back, index, scale, needs=(True, False, False))[0]
+    assert torch.equal(dX[rows].cpu(), exact.to(dX.dtype))
