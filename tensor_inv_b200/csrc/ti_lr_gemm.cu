@@ -59,10 +59,10 @@ constexpr int kGroupM = 8;                       // raster: 8 row tiles (2048 ro
 constexpr int kRankStep = 16;
 constexpr int kFixSlots = 16;
 constexpr size_t kSmem = size_t(kStages) * kStageBytes + 2 * kLowBytes + 1024 + 512;
-// Rows that leave through shared memory: a warp's 32 rows of 16 words, one word apart.  Such calls
-// use a ring of kStages - 1 stages, and four warps each share the last stage of sA and of sB.
-constexpr int kTurnWords = 32 * 17;
-static_assert(4 * kTurnWords * 4 <= kABytes && kABytes == kBBytes,
+// Rows that leave through shared memory: a warp's 32 rows of 16 words, in the last stage of sA; such
+// calls use a ring of kStages - 1 stages.
+constexpr int kTurnWords = 32 * 16;
+static_assert(kEpiWarps * kTurnWords * 4 <= kABytes,
               "the warps' rows do not fit the stage that is left to them");
 
 struct Params {
@@ -203,7 +203,8 @@ __device__ __forceinline__ void store_flag(uint32_t addr) {
 
 // Stores a warp's 32 rows x 32 packed columns (lane = row), as far as they exist.  Rows that are
 // not 16-byte aligned would leave in pieces of 8, 4 or 2 bytes, 32 rows at a time; they go through
-// `turn` (32 rows of 17 words, this warp's own) instead, so that a store covers consecutive bytes.
+// `turn` (32 rows of 16 words, this warp's own) instead, so that a store covers consecutive bytes.
+// Word j of row r lies at j ^ (r / 2), which keeps both directions free of bank conflicts.
 template <typename T>
 __device__ __forceinline__ void store_block(const Params &P, T *out, uint32_t *turn, int64_t row0,
                                             int64_t col0, int lane, const uint32_t (&pk)[16]) {
@@ -226,19 +227,20 @@ __device__ __forceinline__ void store_block(const Params &P, T *out, uint32_t *t
         return;
     }
 #pragma unroll
-    for (int j = 0; j < 16; ++j) turn[lane * 17 + j] = pk[j];
+    for (int j = 0; j < 16; ++j) turn[lane * 16 + (j ^ (lane >> 1))] = pk[j];
     __syncwarp();
     const int rows = static_cast<int>(min(int64_t(32), P.rows - row0));
     if (P.align >= 4 && col0 + 32 <= P.cols) {  // words: two rows at a time
         uint32_t *dst = reinterpret_cast<uint32_t *>(out + row0 * P.ldo + col0) + (lane & 15);
 #pragma unroll 4
-        for (int r = lane >> 4; r < rows; r += 2) dst[r * (P.ldo >> 1)] = turn[r * 17 + (lane & 15)];
+        for (int r = lane >> 4; r < rows; r += 2)
+            dst[r * (P.ldo >> 1)] = turn[r * 16 + ((lane ^ (r >> 1)) & 15)];
     } else {
         uint16_t *dst = reinterpret_cast<uint16_t *>(out + row0 * P.ldo + col0) + lane;
-        const uint16_t *src = reinterpret_cast<const uint16_t *>(turn) + lane;
+        const uint16_t *src = reinterpret_cast<const uint16_t *>(turn);
         if (col0 + lane < P.cols)
 #pragma unroll 4
-            for (int r = 0; r < rows; ++r) dst[r * P.ldo] = src[r * 34];
+            for (int r = 0; r < rows; ++r) dst[r * P.ldo] = src[r * 32 + (lane ^ (r & ~1))];
     }
     __syncwarp();
 }
@@ -436,8 +438,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         int64_t unit = 0;
         const DropoutKeys key(kDrop ? dropout_key(P.drop) : 0);
         T *out = static_cast<T *>(P.out);
-        uint32_t *turn = reinterpret_cast<uint32_t *>((part ? sB : sA) + (kStages - 1) * kABytes) +
-                         q * kTurnWords;
+        uint32_t *turn = reinterpret_cast<uint32_t *>(sA + (kStages - 1) * kABytes) +
+                         (warp - 2) * kTurnWords;
         // the whole warp has read its accumulator rows: one arrive per warp on CTA 0
         auto release = [&](int acc) {
             tc_fence_before();
