@@ -32,9 +32,10 @@
 // order, so results repeat bit for bit, and far enough apart that the loaders are ready (8192^3,
 // r = 32, whole call: 990 us with 4, 935 us with 16).  The kernel may start before the projection has finished
 // (programmatic launch); the loaders wait for it.
-// Measured on a B200 (bf16): 8192^3 787 us without adapters (1398 TFLOP/s; cuBLAS on the plain
-// product 677 us), 802 us with rank 32; 4096^3 110 us (cuBLAS 94 us), 114 us with rank 16, 125 us with
-// rank 64, 132 us with rank 16 and dropout.  4096^3 is 256 tiles on 74 pairs: the fourth wave is half
+// Measured on a B200 (bf16, this kernel alone): 8192^3 787 to 800 us without adapters (1398 TFLOP/s;
+// cuBLAS on the plain product 680 us), 802 to 840 us with rank 32, fp16 880 us (the power cap; a whole
+// call in a long run takes 887 to 1058 us); 4096^3 110 us (cuBLAS 92 us), 114 to 117 us with rank 16,
+// 126 us with rank 64, 135 us with rank 16 and dropout; 4096 x 4096 x 4097 122 us.  4096^3 is 256 tiles on 74 pairs: the fourth wave is half
 // empty.
 // All waits are bounded; on timeout the error word is raised and the CTA leaves its loops.
 #include <atomic>

@@ -22,11 +22,11 @@
 //          that occur without gaps in either direction.
 //   join   adds an adapter's slots in order and rounds once.  One chunk needs no join.
 //
-// Measured on a B200: 4096 rows, 4096 + 4096 columns, r = 16: 22 us (3.0 TB/s of M), 38 us with
-// dropout, 35 us for fp16 (its scales take a pass over V); 8192 rows, r = 64: 56 us (144 us in a form
-// on mma.sync that kept M in registers).  Copies of four rows at a time cost more than boxes, so 64
+// Measured on a B200, the wgrad kernel alone behind the dX pass: 4096 rows, 4096 + 4096 columns, r = 16:
+// 27 us (2.5 TB/s of M), 39 us with dropout, 40 us for fp16 (its scales take a pass over V); 8192 rows,
+// r = 64: 71 us (25, 38 and 58 us with two parts of bf16).  Copies of four rows at a time cost more than boxes, so 64
 // consecutive rows go as one box: the first case's shape with rows of 16 adapters in random order,
-// which cannot, takes 55 us.
+// which cannot, takes 57 us.
 //
 // Infinities and NaN: an infinity in M meets every part of V, and infinity * 0 or infinity - infinity
 // is NaN where the formula has an infinity (and a V near float32's end rounds to one).  So a CTA that
